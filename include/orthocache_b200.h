@@ -446,6 +446,84 @@ int oc_score_from_metadata_paged(const float* dc_pool, const float* e_ac_pool, c
                                  float zeta_max, float* bound_max, float* bounds, uint8_t* keep, oc_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Token-level attention over a KV cache.  The reference attends to whole
+ * 512-token blocks without a mask (src/orthocache/indirect_attention.py:
+ * 29-170); these entry points attend to single tokens: sequences of any
+ * length, drafted tokens, causal chunks, capped and biased scores.
+ *
+ * All of them: q (B, Sq, Hq, D), keys / values (B, S, Hkv, D) of one dtype
+ * (OC_F32 or OC_BF16), D in {64, 128, 256}, Hq a multiple of Hkv (query head
+ * hq reads KV head hq / G, G = Hq / Hkv); seq_len = S is the capacity of a
+ * batch row and lengths (B, nullable = S; clamped to [0, S]) the tokens it
+ * holds: what lies behind them is never used, whatever its value.  Scores
+ * are scale * q.k in float32; cap > 0 turns them into cap * tanh(s / cap).
+ * A query row that sees no key gives zeros.  A key or value that some rows of
+ * a call see and others do not must be finite for the others.  out
+ * (B, Sq, Hq, D) in out_dtype.  k and v may be NULL when seq_len is 0.
+ * Workspace: oc_token_attention_workspace_bytes (q_len: Sq or the drafted
+ * tokens; accumulate: nonzero for oc_accumulate_attention), 16-byte aligned;
+ * nothing in it needs to start at zero.  Calls that share one must not
+ * overlap on the GPU.
+ */
+size_t oc_token_attention_workspace_bytes(int dtype, int batch, int q_len, int q_heads, int kv_heads, int head_dim,
+                                          int seq_len, int accumulate);
+
+/* Attention of a tree of drafted tokens over a cache: node i of batch row b
+ * (q row i; 1 <= nodes <= 256) sees every cache token j < lengths[b] and the
+ * drafted tokens s with tree_mask[b, i, s] != 0 (its ancestors and itself).
+ * draft_k / draft_v (B, nodes, Hkv, D); tree_mask uint8 (B, nodes, nodes), or
+ * (nodes, nodes) for the whole batch when mask_batched is 0.
+ * block_table (B, table_stride) int32 makes k / v a pool of num_pages pages of
+ * block_size tokens (a multiple of 128) shared by the batch, as in
+ * oc_indirect_attention_paged; then seq_len = table_stride * block_size, and
+ * the tokens of a page outside [0, num_pages) are seen by nobody.  NULL:
+ * contiguous keys and values. */
+int oc_tree_attention(const void* q, const void* k, const void* v, int dtype, const int32_t* block_table,
+                      int table_stride, int num_pages, int block_size, const int32_t* lengths, const void* draft_k,
+                      const void* draft_v, const uint8_t* tree_mask, int mask_batched, int batch, int nodes,
+                      int q_heads, int kv_heads, int head_dim, int seq_len, float cap, float scale, void* out,
+                      int out_dtype, void* workspace, size_t workspace_bytes, oc_stream_t stream);
+
+/* Attention of a query chunk over its cache, which already holds the chunk's
+ * own keys and values: query i of batch row b sits at position pos =
+ * lengths[b] - q_len + i (a row with pos < 0 sees nothing) and sees key j <
+ * lengths[b] iff
+ *   (!causal, or j <= pos, or prefix and j < prefix[b]) and
+ *   (no documents, or documents[b, j] == documents[b, pos] >= 0).
+ * prefix (B), documents (B, S) int32 (negative: padding) and slopes (Hq)
+ * float32 are nullable; slopes subtract slopes[hq] * |pos - j| from the
+ * (capped) score. */
+int oc_chunk_attention(const void* q, const void* k, const void* v, int dtype, const int32_t* lengths, int causal,
+                       const int32_t* prefix, const int32_t* documents, const float* slopes, int batch, int q_len,
+                       int q_heads, int kv_heads, int head_dim, int seq_len, float cap, float scale, void* out,
+                       int out_dtype, void* workspace, size_t workspace_bytes, oc_stream_t stream);
+
+/* Causal chunk attention (as above) that also sums the attention weights of
+ * every key over the query rows of its KV head:
+ *   weights_out[b, h, j] = weights_in[b, h, j] + sum over i, g of
+ *   softmax(s)[b, i, h * G + g, j];
+ * weights (B, Hkv, S) float32; weights_in NULL counts as zero and may equal
+ * weights_out.  Entries behind lengths[b] are copied.  The sums are taken in
+ * a fixed order: the same call gives the same bits. */
+int oc_accumulate_attention(const void* q, const void* k, const void* v, int dtype, const int32_t* lengths,
+                            const float* weights_in, float* weights_out, int batch, int q_len, int q_heads,
+                            int kv_heads, int head_dim, int seq_len, float cap, float scale, void* out, int out_dtype,
+                            void* workspace, size_t workspace_bytes, oc_stream_t stream);
+
+/* Eviction of tokens by accumulated weight.  Of the n = lengths[b] tokens of
+ * (b, h) the `recent` last stay and, of the others, the keep - recent with
+ * the largest weights[b, h, j] (ties: the lower position; NaN is the
+ * largest); all stay when n <= keep.  The kept tokens are written in order of
+ * position: k_out / v_out (B, keep, Hkv, D), weights_out and index (their
+ * source positions) (B, Hkv, keep), new_lengths (B) = min(n, keep); behind
+ * them zeros, and index -1.  1 <= keep <= seq_len, 0 <= recent <= keep;
+ * head_dim * sizeof(dtype) a multiple of 16.  The outputs must not overlap the
+ * inputs. */
+int oc_evict_tokens(const void* k, const void* v, int dtype, const float* weights, const int32_t* lengths, int batch,
+                    int seq_len, int kv_heads, int head_dim, int keep, int recent, void* k_out, void* v_out,
+                    float* weights_out, int32_t* index, int32_t* new_lengths, oc_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Sequence-parallel exchange over NCCL (one rank per GPU).  `comm` is an
  * ncclComm_t created by the caller (any NCCL 2.x: the library resolves NCCL
  * at run time, preferring the copy already loaded in the process, else

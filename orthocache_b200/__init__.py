@@ -27,6 +27,7 @@ from .indirect_attention import indirect_attention, compile_indirect_attention
 from .adaptive_attention import orthocache_attention, orthocache_attention_batched
 from .metadata_cache import SpectralMetadataCache
 from .paged import PagedKVCache
+from .token_attention import tree_attention, chunk_attention, accumulate_attention, evict_tokens
 from . import nvlink_model
 
 __all__ = [
@@ -36,4 +37,5 @@ __all__ = [
     "compile_pallas_sparse_attention", "stream_compact", "stream_decompact", "compact_and_attend",
     "orthocache_forward", "indirect_attention", "compile_indirect_attention", "orthocache_attention",
     "orthocache_attention_batched", "SpectralMetadataCache", "PagedKVCache",
+    "tree_attention", "chunk_attention", "accumulate_attention", "evict_tokens",
 ]

@@ -71,6 +71,14 @@ SIGNATURES = {
                                         _p, _i, _p, _sz, _p]),
     "oc_score_from_metadata_paged": (_i, [_p, _p, _p, _i, _p, _i, _p, _i, _i, _i, _i, _i, _i, _i, _f, _f, _p, _p,
                                           _p, _p]),
+    "oc_token_attention_workspace_bytes": (_sz, [_i] * 8),
+    "oc_tree_attention": (_i, [_p, _p, _p, _i, _p, _i, _i, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _f, _f, _p,
+                               _i, _p, _sz, _p]),
+    "oc_chunk_attention": (_i, [_p, _p, _p, _i, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _i, _f, _f, _p, _i, _p, _sz,
+                                _p]),
+    "oc_accumulate_attention": (_i, [_p, _p, _p, _i, _p, _p, _p, _i, _i, _i, _i, _i, _i, _f, _f, _p, _i, _p, _sz,
+                                     _p]),
+    "oc_evict_tokens": (_i, [_p, _p, _i, _p, _p, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p]),
     "oc_indirect_attention_noalloc_max_scratch_bytes": (_sz, []),
     "oc_indirect_attention_noalloc": (_i, [_p, _p, _p, _i, _p, _i, _i, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i,
                                            _i, _p, _i, _p]),

@@ -1,0 +1,112 @@
+// Token-level attention over a KV cache: what the tree, chunk and
+// accumulating forms share.
+//
+// For batch row b and KV head h the query rows of the G = Hq / Hkv heads that
+// read it are numbered r = i * G + g (query position i, head h * G + g).  Row
+// r may see key j of the cache iff
+//     j < hi_r   and   (no documents, or documents[b, j] == doc_r),
+// where hi_r folds the sequence length, the causal limit and the prefix (a
+// row that has no position, or lies in padding, has hi_r = 0), and drafted
+// key s iff tree[b, i, s].  Its score is, in log2 units,
+//     s2 = log2(e) * (cap * tanh(scale * q.k / cap) - slope * |pos_r - j|)
+// (without the tanh when cap is 0), and the output softmax(s) . v; a row that
+// sees nothing is zero.
+#pragma once
+
+#include "oc_common.cuh"
+
+namespace oc {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxNodes = 256;  // drafted tokens of one tree
+
+struct TokArgs {
+  const void *q, *k, *v;
+  const void *dk, *dv;        // drafted keys / values (B, Sq, Hkv, D); NULL: chunk form
+  const uint8_t* tree;        // (1 or B, Sq, Sq)
+  int64_t tree_bstride;       // 0 or Sq * Sq
+  const int32_t* lengths;     // (B) or NULL (= S)
+  const int32_t* table;       // (B, table_stride) pool pages, or NULL: k, v are (B, S, Hkv, D)
+  int table_stride, page, num_pages;
+  const int32_t *prefix, *docs;  // (B), (B, S); nullable
+  const float* slopes;           // (Hq) nullable
+  int causal;
+  int B, Sq, Hq, Hkv, G, R, S;   // R = Sq * G rows per KV head; S keys of capacity per batch row
+  float scale, cap;
+  void* out;
+  int out_dtype;
+  // split over the keys: chunk c covers tokens [c * chunk, (c + 1) * chunk)
+  int chunk, nchunk, nrt;        // nrt row tiles per (b, h)
+  float *pm, *pl, *po;           // partials: [(bh * nrt + rt) * nchunk + c][row tile][(D)]
+  float* lse;                    // (B * Hkv, R) log2 of the softmax denominator, +inf for empty rows; nullable
+};
+
+__device__ __forceinline__ int tok_len(const TokArgs& a, int b) {
+  if (!a.lengths) return a.S;
+  const int n = a.lengths[b];
+  return n < 0 ? 0 : (n > a.S ? a.S : n);
+}
+
+// What one query row may see and how its scores are biased.
+struct TokRow {
+  int hi;       // keys [0, hi)
+  int pos;      // position of the query in its sequence
+  int doc;      // document of the query (only with documents)
+  float slope2; // slope * log2(e), 0 without a bias
+};
+
+__device__ __forceinline__ TokRow tok_row(const TokArgs& a, int b, int h, int r, int len) {
+  TokRow w;
+  w.hi = 0;
+  w.pos = 0;
+  w.doc = 0;
+  w.slope2 = 0.f;
+  if (r >= a.R) return w;
+  const int i = r / a.G;
+  if (a.dk) {
+    w.hi = len;
+    w.pos = len;
+    return w;
+  }
+  w.pos = len - a.Sq + i;
+  if (a.slopes) w.slope2 = a.slopes[h * a.G + r % a.G] * kLog2e;
+  if (w.pos < 0) return w;
+  int hi = len;
+  if (a.causal) {
+    hi = w.pos + 1;
+    if (a.prefix && a.prefix[b] > hi) hi = a.prefix[b];
+    if (hi > len) hi = len;
+  }
+  if (a.docs) {
+    w.doc = a.docs[(size_t)b * a.S + w.pos];
+    if (w.doc < 0) hi = 0;
+  }
+  w.hi = hi;
+  return w;
+}
+
+// Row (of the (rows, Hkv, D) view of k / v) of token j of batch row b; -1 for
+// a token whose page lies outside the pool.
+__device__ __forceinline__ int64_t tok_kv_row(const TokArgs& a, int b, int j) {
+  if (!a.table) return (int64_t)b * a.S + j;
+  const int p = a.table[(size_t)b * a.table_stride + j / a.page];
+  return p < 0 || p >= a.num_pages ? -1 : (int64_t)p * a.page + j % a.page;
+}
+
+// Element offset of the first channel of output / query row r of (b, h).
+__device__ __forceinline__ int64_t tok_q_offset(const TokArgs& a, int b, int h, int r, int D) {
+  return (((int64_t)b * a.Sq + r / a.G) * a.Hq + (int64_t)h * a.G + r % a.G) * D;
+}
+
+// The score in log2 units from the dot product (accurate form).
+__device__ __forceinline__ float tok_score(const TokArgs& a, float dot, float slope2, int pos, int j) {
+  float x = dot * a.scale;
+  if (a.cap > 0.f) x = a.cap * tanhf(x / a.cap);
+  x *= kLog2e;
+  return slope2 != 0.f ? fmaf(-slope2, fabsf((float)(pos - j)), x) : x;
+}
+
+// Merge of the partials of all chunks (oc_token_attention.cu).
+int tok_merge(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st);
+
+}  // namespace oc

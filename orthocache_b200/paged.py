@@ -109,3 +109,12 @@ class PagedKVCache:
                   self.num_pages, PAGE, nb, _lib.ptr(out), _lib.dtype_code(out), _lib.ptr(ws), ws_bytes,
                   _lib.stream_ptr(self.device))
         return out, keep, perm, count
+
+    def attend_tree(self, q, draft_keys, draft_values, tree_mask, block_table, lengths, cap=0.0, scale=None):
+        """Attention of drafted tokens (``token_attention.tree_attention``) over
+        the first lengths[b] tokens of the pages in block_table[b]; the last
+        page may be filled in part.  q (B, T, Hq, D), draft_keys and
+        draft_values (B, T, kv_heads, D).  Returns (B, T, Hq, D)."""
+        from .token_attention import tree_attention
+        return tree_attention(q, self.k, self.v, draft_keys, draft_values, tree_mask, lengths,
+                              block_table=block_table, cap=cap, scale=scale)

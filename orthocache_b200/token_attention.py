@@ -1,0 +1,262 @@
+"""Token-level attention over a KV cache.
+
+The block operators of this package attend to whole 512-token blocks without
+a mask, like the reference (``src/orthocache/indirect_attention.py:29-170``).
+The three operators here attend to single tokens of a cache that holds
+``lengths[b]`` of its capacity of tokens:
+
+* ``tree_attention``: drafted tokens arranged in a tree, over a contiguous or
+  paged cache (``PagedKVCache.attend_tree``); one decoded token is a tree of
+  one node;
+* ``chunk_attention``: the last ``Sq`` tokens of every sequence over its cache,
+  with a causal, prefix or document mask, scores capped by a tanh and a bias
+  that grows with the distance;
+* ``accumulate_attention``: causal chunk attention that also adds every key's
+  attention weight to a running sum, the input of ``evict_tokens``.
+
+Shapes: q (B, Sq, Hq, D), keys and values (B, S, Hkv, D), float32 or bfloat16,
+D in {64, 128, 256}, Hq a multiple of Hkv; without the batch dimension all
+per-row arguments lose theirs too.  q is brought to the keys' type and the output
+has it.  Inputs on the CPU are copied to the GPU.  Nothing waits for the GPU.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _core, _lib
+from .paged import PAGE
+
+
+def _int_rows(x, shape, device, what):
+    """An int32 device tensor of ``shape`` (None stays None; a number fills it)."""
+    if x is None:
+        return None
+    if isinstance(x, int):
+        return torch.full(shape, x, dtype=torch.int32, device=device)
+    t = _lib.as_device(x, device=device)
+    if t.dtype.is_floating_point or t.dtype == torch.bool:
+        raise TypeError(f"{what} must be integers, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} {tuple(t.shape)}, expected {tuple(shape)}")
+    return t.to(torch.int32).contiguous()
+
+
+def _cap_scale(cap, scale, dim):
+    cap = float(cap or 0.0)
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    if not (math.isfinite(cap) and cap >= 0.0):
+        raise ValueError(f"cap must be finite and >= 0 (0: none), got {cap}")
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
+    return cap, scale
+
+
+def _workspace(q, kv_heads, seq_len, accumulate):
+    B, Sq, Hq, D = q.shape
+    n = _lib.query("oc_token_attention_workspace_bytes", _lib.dtype_code(q), B, Sq, Hq, kv_heads, D, seq_len,
+                   int(accumulate))
+    return torch.empty((n,), dtype=torch.uint8, device=q.device), n
+
+
+def _check_heads(q, kv_heads):
+    if kv_heads == 0 or q.shape[2] % kv_heads or q.shape[2] == 0:
+        raise ValueError(f"{q.shape[2]} query heads are not a multiple of {kv_heads} KV heads")
+    if q.shape[3] not in (64, 128, 256):
+        raise ValueError(f"head_dim {q.shape[3]} is not 64, 128 or 256")
+    if q.shape[0] == 0 or q.shape[1] == 0:
+        raise ValueError(f"empty query {tuple(q.shape)}")
+
+
+def tree_attention(q, keys, values, draft_keys, draft_values, tree_mask, lengths=None, *, block_table=None, cap=0.0,
+                   scale=None):
+    """Attention of drafted tokens over a cache and their own ancestors.
+
+    Node i (row i of q (B, T, Hq, D), T <= 256) sees every cache token
+    j < lengths[b] (default: all) and the drafted tokens s with tree_mask[b, i, s]
+    (bool (T, T) or (B, T, T): its ancestors and, usually, itself).
+    draft_keys, draft_values: (B, T, Hkv, D).  With ``block_table`` (B, blocks)
+    int32, keys and values are a pool of 512-token pages (pages * 512, Hkv, D)
+    and logical block j of row b is page block_table[b, j]; tokens of pages
+    outside the pool are seen by nobody.  ``cap`` > 0: scores become
+    cap * tanh(score / cap); ``scale`` defaults to 1 / sqrt(D).  A row that
+    sees no token is zero.  Returns (B, T, Hq, D) in the cache's type.
+    """
+    k = _lib.as_device(keys)
+    if k.dtype not in (torch.float32, torch.bfloat16):
+        k = k.float()
+    dev, dt = k.device, k.dtype
+    v = _lib.as_device(values, device=dev, dtype=dt)
+    qq, dk, dv = (_lib.as_device(x, device=dev, dtype=dt) for x in (q, draft_keys, draft_values))
+    batched = qq.dim() == 4
+    if not batched:
+        qq, dk, dv = qq.unsqueeze(0), dk.unsqueeze(0), dv.unsqueeze(0)
+        if block_table is None:
+            k, v = k.unsqueeze(0), v.unsqueeze(0)
+    kdim = 3 if block_table is not None else 4
+    if qq.dim() != 4 or k.dim() != kdim or k.shape != v.shape or dk.dim() != 4 or dk.shape != dv.shape:
+        raise ValueError(f"incompatible shapes q {tuple(qq.shape)}, keys {tuple(k.shape)}, values {tuple(v.shape)}, "
+                         f"draft {tuple(dk.shape)}, {tuple(dv.shape)}")
+    B, T, Hq, D = qq.shape
+    Hkv = k.shape[-2]
+    _check_heads(qq, Hkv)
+    if k.shape[-1] != D or tuple(dk.shape) != (B, T, Hkv, D):
+        raise ValueError(f"incompatible shapes q {tuple(qq.shape)}, keys {tuple(k.shape)}, draft {tuple(dk.shape)}")
+    table = None
+    if block_table is None:
+        if k.shape[0] != B:
+            raise ValueError(f"keys {tuple(k.shape)} for {B} batch rows")
+        S, pages, stride = k.shape[1], 0, 0
+    else:
+        if k.shape[0] % PAGE or k.shape[0] == 0:
+            raise ValueError(f"a pool of {k.shape[0]} tokens is not a whole number of {PAGE}-token pages")
+        table = _lib.as_device(block_table, device=dev)
+        if table.dim() == 1:
+            table = table.unsqueeze(0)
+        table = _int_rows(table, (B, table.shape[-1]), dev, "block_table")
+        pages, stride = k.shape[0] // PAGE, table.shape[1]
+        S = stride * PAGE
+    mask = _lib.as_device(tree_mask, device=dev)
+    mask_batched = mask.dim() == 3
+    if tuple(mask.shape) != ((B, T, T) if mask_batched else (T, T)):
+        raise ValueError(f"tree_mask {tuple(mask.shape)}, expected ({T}, {T}) or ({B}, {T}, {T})")
+    if mask.dtype not in (torch.bool, torch.uint8):
+        raise TypeError(f"tree_mask must be bool, got {mask.dtype}")
+    lens = _int_rows(lengths, (B,), dev, "lengths")
+    cap, scale = _cap_scale(cap, scale, D)
+    with torch.cuda.device(dev):
+        out = torch.empty((B, T, Hq, D), dtype=dt, device=dev)
+        ws, ws_bytes = _workspace(qq, Hkv, S, False)
+        _lib.call("oc_tree_attention", _lib.ptr(qq), _lib.ptr(k), _lib.ptr(v), _lib.dtype_code(k), _lib.ptr(table),
+                  stride, pages, PAGE, _lib.ptr(lens), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(mask), int(mask_batched),
+                  B, T, Hq, Hkv, D, S, cap, scale, _lib.ptr(out), _lib.dtype_code(out), _lib.ptr(ws), ws_bytes,
+                  _lib.stream_ptr(dev))
+    return out if batched else out[0]
+
+
+def _chunk_inputs(q, keys, values, lengths):
+    qq, k, v, batched = _core.batched_qkv(q, keys, values)
+    _check_heads(qq, k.shape[2])
+    return qq, k, v, batched, _int_rows(lengths, (k.shape[0],), k.device, "lengths")
+
+
+def chunk_attention(q, keys, values, lengths=None, *, causal=True, prefix=None, documents=None, slopes=None, cap=0.0,
+                    scale=None):
+    """Attention of the last Sq tokens of every sequence over its cache.
+
+    The cache already holds the chunk: query i of row b sits at position
+    pos = lengths[b] - Sq + i (lengths default to the capacity S; a row with
+    pos < 0 sees nothing, as in a batch padded on the left) and sees key
+    j < lengths[b] iff it is allowed by
+
+    * the causal mask: not ``causal``, or j <= pos, or j < prefix[b]
+      (``prefix`` (B,): tokens that every query may see);
+    * the document mask: ``documents`` (B, S) int, equal at pos and j and not
+      negative (negative: padding, seen by nobody).
+
+    Scores: scale * q.k (1 / sqrt(D) by default), then cap * tanh(score / cap)
+    if ``cap`` > 0, then minus slopes[head] * |pos - j| (``slopes`` (Hq,)
+    float).  A row that sees no key is zero.  Returns (B, Sq, Hq, D) in the
+    cache's type.
+    """
+    qq, k, v, batched, lens = _chunk_inputs(q, keys, values, lengths)
+    B, Sq, Hq, D = qq.shape
+    S, Hkv, dev = k.shape[1], k.shape[2], k.device
+    cap, scale = _cap_scale(cap, scale, D)
+    pre = _int_rows(prefix, (B,), dev, "prefix")
+    docs = None
+    if documents is not None:
+        docs = _lib.as_device(documents, device=dev)
+        docs = _int_rows(docs if batched or docs.dim() != 1 else docs.unsqueeze(0), (B, S), dev, "documents")
+    sl = None
+    if slopes is not None:
+        sl = _lib.as_device(slopes, device=dev, dtype=torch.float32)
+        if tuple(sl.shape) != (Hq,):
+            raise ValueError(f"slopes {tuple(sl.shape)}, expected ({Hq},)")
+    with torch.cuda.device(dev):
+        out = torch.empty((B, Sq, Hq, D), dtype=k.dtype, device=dev)
+        ws, ws_bytes = _workspace(qq, Hkv, S, False)
+        _lib.call("oc_chunk_attention", _lib.ptr(qq), _lib.ptr(k), _lib.ptr(v), _lib.dtype_code(k), _lib.ptr(lens),
+                  int(bool(causal)), _lib.ptr(pre), _lib.ptr(docs), _lib.ptr(sl), B, Sq, Hq, Hkv, D, S, cap, scale,
+                  _lib.ptr(out), _lib.dtype_code(out), _lib.ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+    return out if batched else out[0]
+
+
+def accumulate_attention(q, keys, values, weights=None, lengths=None, *, cap=0.0, scale=None, out_weights=None):
+    """Causal ``chunk_attention`` that also sums every key's attention weight.
+
+    Returns (out, new) with new[b, h, j] = weights[b, h, j] + the softmax
+    weights that the query rows of KV head h give key j, summed over the Sq
+    queries and the Hq / Hkv heads.  ``weights``: (B, Hkv, S) float32, None for
+    zeros; entries behind lengths[b] are copied.  ``out_weights``: a contiguous
+    float32 CUDA tensor that receives the sums (``weights`` itself to add in
+    place); a new one by default.
+    """
+    qq, k, v, batched, lens = _chunk_inputs(q, keys, values, lengths)
+    B, Sq, Hq, D = qq.shape
+    S, Hkv, dev = k.shape[1], k.shape[2], k.device
+    cap, scale = _cap_scale(cap, scale, D)
+    shape = (B, Hkv, S) if batched else (Hkv, S)
+    w = None
+    if weights is not None:
+        w = _lib.as_device(weights, device=dev, dtype=torch.float32)
+        if tuple(w.shape) != shape:
+            raise ValueError(f"weights {tuple(w.shape)}, expected {shape}")
+    if out_weights is not None:
+        o = out_weights
+        if not (isinstance(o, torch.Tensor) and o.device == dev and o.dtype == torch.float32 and o.is_contiguous() and
+                tuple(o.shape) == shape):
+            raise ValueError(f"out_weights must be a contiguous float32 tensor {shape} on {dev}")
+    with torch.cuda.device(dev):
+        if out_weights is None:
+            out_weights = torch.empty(shape, dtype=torch.float32, device=dev)
+        out = torch.empty((B, Sq, Hq, D), dtype=k.dtype, device=dev)
+        ws, ws_bytes = _workspace(qq, Hkv, S, True)
+        _lib.call("oc_accumulate_attention", _lib.ptr(qq), _lib.ptr(k), _lib.ptr(v), _lib.dtype_code(k),
+                  _lib.ptr(lens), _lib.ptr(w), _lib.ptr(out_weights), B, Sq, Hq, Hkv, D, S, cap, scale, _lib.ptr(out),
+                  _lib.dtype_code(out), _lib.ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+    return (out if batched else out[0]), out_weights
+
+
+def evict_tokens(keys, values, weights, keep, recent=0, lengths=None):
+    """Cut a cache down to ``keep`` tokens per KV head.
+
+    keys, values (B, S, Hkv, D), weights (B, Hkv, S) float32 (the sums of
+    ``accumulate_attention``).  Of the n = lengths[b] tokens (default S) of
+    each head the ``recent`` last stay and, of the others, the keep - recent
+    with the largest weights (ties: the lower position; NaN is the largest);
+    all stay when n <= keep.  Returns (keys, values, weights, index, lengths) of
+    the new cache: (B, keep, Hkv, D) twice, (B, Hkv, keep), the tokens' old
+    positions (B, Hkv, keep) int32 in ascending order, and min(n, keep) (B,)
+    int32; behind the last kept token zeros and index -1.
+    """
+    k = _lib.as_device(keys)
+    if k.dtype not in (torch.float32, torch.bfloat16):
+        k = k.float()
+    v = _lib.as_device(values, device=k.device, dtype=k.dtype)
+    w = _lib.as_device(weights, device=k.device, dtype=torch.float32)
+    batched = k.dim() == 4
+    if not batched:
+        k, v, w = k.unsqueeze(0), v.unsqueeze(0), w.unsqueeze(0)
+    if k.dim() != 4 or k.shape != v.shape or tuple(w.shape) != (k.shape[0], k.shape[2], k.shape[1]):
+        raise ValueError(f"incompatible shapes keys {tuple(k.shape)}, values {tuple(v.shape)}, weights "
+                         f"{tuple(w.shape)}")
+    B, S, H, D = k.shape
+    keep, recent = int(keep), int(recent)
+    if not 1 <= keep <= S:
+        raise ValueError(f"keep {keep} of {S} tokens")
+    if not 0 <= recent <= keep:
+        raise ValueError(f"recent {recent}, keep {keep}")
+    dev = k.device
+    lens = _int_rows(lengths, (B,), dev, "lengths")
+    with torch.cuda.device(dev):
+        ko = torch.empty((B, keep, H, D), dtype=k.dtype, device=dev)
+        vo = torch.empty_like(ko)
+        wo = torch.empty((B, H, keep), dtype=torch.float32, device=dev)
+        index = torch.empty((B, H, keep), dtype=torch.int32, device=dev)
+        left = torch.empty((B,), dtype=torch.int32, device=dev)
+        _lib.call("oc_evict_tokens", _lib.ptr(k), _lib.ptr(v), _lib.dtype_code(k), _lib.ptr(w), _lib.ptr(lens), B, S,
+                  H, D, keep, recent, _lib.ptr(ko), _lib.ptr(vo), _lib.ptr(wo), _lib.ptr(index), _lib.ptr(left),
+                  _lib.stream_ptr(dev))
+    return (ko, vo, wo, index, left) if batched else (ko[0], vo[0], wo[0], index[0], left[0])
