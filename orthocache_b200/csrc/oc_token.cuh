@@ -106,6 +106,9 @@ __device__ __forceinline__ float tok_score(const TokArgs& a, float dot, float sl
   return slope2 != 0.f ? fmaf(-slope2, fabsf((float)(pos - j)), x) : x;
 }
 
+// The bfloat16 kernel for few rows (oc_token_mma.cu); row_tile 16, 32 or 64.
+int tok_mma(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st);
+
 // Merge of the partials of all chunks (oc_token_attention.cu).
 int tok_merge(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st);
 

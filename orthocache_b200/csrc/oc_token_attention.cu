@@ -415,23 +415,34 @@ struct TokPlan {
 
 inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Split the keys while the (row tile, batch row, KV head) units alone do not
-// fill the GPU: about four CTAs per SM in all, at least 256 keys each (below
-// that a CTA's set-up outweighs its keys).
+// Rows per tile: 16, 32 or 64 for bfloat16 (what the rows fill), 16 or 64 for
+// float32.  Split the keys so that the CTAs of all (row tile, batch row, KV
+// head, chunk) fill whole waves of two CTAs per SM: of the possible numbers of
+// chunks the one with the least waves x (keys of a chunk + 160), 160 keys
+// being about what a CTA's set-up and its partial cost.
 TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int head_dim, int seq_len, bool lse) {
   TokPlan p;
   const int64_t R = (int64_t)q_len * (q_heads / kv_heads);
-  p.row_tile = R <= 32 ? 16 : 64;
+  p.row_tile = R <= 16 ? 16 : R <= 32 ? (dtype == OC_BF16 ? 32 : 16) : 64;
   p.nrt = (int)((R + p.row_tile - 1) / p.row_tile);
   const int64_t units = (int64_t)batch * kv_heads * p.nrt;
-  int64_t want = (4 * 148 + units - 1) / units;
-  const int64_t most = (seq_len + 255) / 256;
-  if (want > most) want = most;
-  if (want < 1) want = 1;
-  p.chunk = (int)(((seq_len + want - 1) / want + 63) / 64 * 64);
-  if (p.chunk < 64) p.chunk = 64;
-  p.nchunk = (seq_len + p.chunk - 1) / p.chunk;
+  const int64_t slots = 2 * (int64_t)device_sm_count();
+  int64_t most = seq_len / 128;
+  if (most > 2 * slots / units + 1) most = 2 * slots / units + 1;
+  int64_t best = 0;
+  p.nchunk = 1;
+  p.chunk = seq_len < 64 ? 64 : (seq_len + 63) / 64 * 64;
+  for (int64_t n = 1; n <= most; ++n) {
+    const int64_t keys = ((seq_len + n - 1) / n + 63) / 64 * 64;
+    const int64_t cost = (units * n + slots - 1) / slots * (keys + (n > 1 ? 160 : 0));
+    if (n == 1 || cost < best) {
+      best = cost;
+      p.chunk = (int)keys;
+      p.nchunk = (int)((seq_len + keys - 1) / keys);
+    }
+  }
   if (p.nchunk < 1) p.nchunk = 1;
+  if (p.chunk < 64) p.chunk = 64;
   const size_t parts = p.nchunk > 1 ? (size_t)units * p.nchunk * p.row_tile : 0;
   size_t off = 0;
   p.lse_off = off;
@@ -544,8 +555,7 @@ int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void*
   a.pl = reinterpret_cast<float*>(w + p.l_off);
   a.po = reinterpret_cast<float*>(w + p.o_off);
   a.lse = lse ? reinterpret_cast<float*>(w + p.lse_off) : nullptr;
-  int rc = dtype == OC_BF16 ? dispatch_simt<__nv_bfloat16>(a, head_dim, p.row_tile, st)
-                            : dispatch_simt<float>(a, head_dim, p.row_tile, st);
+  int rc = dtype == OC_BF16 ? tok_mma(a, head_dim, p.row_tile, st) : dispatch_simt<float>(a, head_dim, p.row_tile, st);
   if (rc) return rc;
   if (p.nchunk > 1) rc = tok_merge(a, head_dim, p.row_tile, st);
   return rc;
