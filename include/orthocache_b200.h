@@ -57,7 +57,8 @@ const char* oc_last_error(void);
 /* Device-side status of the pipelined kernels: nonzero if a bounded wait on
  * an asynchronous copy gave up (the kernel then skipped its remaining work
  * instead of hanging).  Bit 0: scorer / fused decode layer; bit 1: split-KV
- * attention; bit 2: chunked-prefill attention.  Synchronises the current device; reset != 0 clears it.
+ * attention; bit 2: chunked-prefill attention; bit 3:
+ * token-level attention.  Synchronises the current device; reset != 0 clears it.
  * Returns the status (>= 0) or an OC_ERR_* code. */
 int oc_device_status(int reset);
 

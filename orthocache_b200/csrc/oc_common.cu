@@ -187,6 +187,7 @@ extern "C" int oc_set_wait_limit_ns(uint64_t ns) {
   int e = oc::wait_limit_score(ns);
   if (!e) e = oc::wait_limit_attn(ns);
   if (!e) e = oc::wait_limit_prefill(ns);
+  if (!e) e = oc::wait_limit_token(ns);
   if (e) return oc::set_error(OC_ERR_CUDA, "oc_set_wait_limit_ns: %s", cudaGetErrorString((cudaError_t)e));
   return OC_OK;
 }
@@ -200,5 +201,8 @@ extern "C" int oc_device_status(int reset) {
   int s3 = 0;
   rc = oc::prefill_status(&s3, reset);
   if (rc) return rc;
-  return s1 | (s2 << 1) | (s3 << 2);
+  int s4 = 0;
+  rc = oc::token_status(&s4, reset);
+  if (rc) return rc;
+  return s1 | (s2 << 1) | (s3 << 2) | (s4 << 3);
 }

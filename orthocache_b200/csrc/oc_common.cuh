@@ -31,11 +31,13 @@ int score_status(int* status, int reset);
 int score_status_meta(int* status, int reset);  // the metadata form of the fused layer (oc_score_meta.cu)
 int attn_status(int* status, int reset);
 int prefill_status(int* status, int reset);
+int token_status(int* status, int reset);
 // Set the bounded-wait limit of the kernels of each translation unit.
 int wait_limit_score(unsigned long long ns);
 int wait_limit_score_meta(unsigned long long ns);
 int wait_limit_attn(unsigned long long ns);
 int wait_limit_prefill(unsigned long long ns);
+int wait_limit_token(unsigned long long ns);
 
 // Fused decode layer (score, compact, attend and merge in one persistent
 // kernel; oc_score.cu).  decode_fused_bytes: workspace it needs; it must be

@@ -109,6 +109,17 @@ __device__ __forceinline__ float tok_score(const TokArgs& a, float dot, float sl
 // The bfloat16 kernel for few rows (oc_token_mma.cu); row_tile 16, 32 or 64.
 int tok_mma(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st);
 
+// The bfloat16 kernel on the tcgen05 tensor cores (oc_token_tc.cu) for
+// head_dim 64 and 128 and a positive scale.  chunk is a multiple of 128;
+// partials are indexed [(bh * nchunk + c) * R + r].  prep: tok_tc_prep_bytes
+// of scratch.
+struct TokTcShape {
+  int Gp, nhs, P, npt, npairs;  // heads and positions of a row tile; head groups, position tiles, pairs of row tiles
+};
+TokTcShape tok_tc_shape(int q_len, int G);
+size_t tok_tc_prep_bytes(int batch, int q_len, int G, int seq_len);
+int tok_tc(const char* fn, const TokArgs& a, int head_dim, void* prep, cudaStream_t st);
+
 // Merge of the partials of all chunks (oc_token_attention.cu).
 int tok_merge(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st);
 

@@ -407,34 +407,56 @@ int tok_merge(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st) {
 
 namespace {
 
-// How a call is cut: rows per tile, row tiles, keys per chunk, chunks.
+// How a call is cut.
 struct TokPlan {
-  int row_tile, nrt, chunk, nchunk;
-  size_t lse_off, m_off, l_off, o_off, bytes;
+  bool tc;            // the tcgen05 kernel
+  int row_tile, nrt;  // rows per tile, row tiles per (b, h)
+  int chunk, nchunk;  // keys per chunk, chunks
+  size_t lse_off, m_off, l_off, o_off, prep_off, bytes;
 };
 
 inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Rows per tile: 16, 32 or 64 for bfloat16 (what the rows fill), 16 or 64 for
-// float32.  Split the keys so that the CTAs of all (row tile, batch row, KV
-// head, chunk) fill whole waves of two CTAs per SM: of the possible numbers of
-// chunks the one with the least waves x (keys of a chunk + 160), 160 keys
-// being about what a CTA's set-up and its partial cost.
-TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int head_dim, int seq_len, bool lse) {
+// Kernel: float32 takes the float32-arithmetic kernel (row tiles of 16 or 64);
+// bfloat16 the m16n8k16 kernel (16, 32 or 64 rows, what the rows fill) or, for
+// more than kTcRows rows per KV head at head_dim 64 and 128, the tcgen05 one.
+//
+// Split of the keys: the CTAs of all (row tile, batch row, KV head, chunk) run
+// in waves of one (tcgen05) or two per SM; of the possible numbers of chunks
+// the one with the least waves x (keys of a chunk + what a CTA's set-up and its
+// partial cost, in keys) is taken.
+constexpr int kTcRows = 64;
+
+TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int head_dim, int seq_len, float scale,
+                 bool lse) {
   TokPlan p;
-  const int64_t R = (int64_t)q_len * (q_heads / kv_heads);
-  p.row_tile = R <= 16 ? 16 : R <= 32 ? (dtype == OC_BF16 ? 32 : 16) : 64;
-  p.nrt = (int)((R + p.row_tile - 1) / p.row_tile);
-  const int64_t units = (int64_t)batch * kv_heads * p.nrt;
-  const int64_t slots = 2 * (int64_t)device_sm_count();
-  int64_t most = seq_len / 128;
-  if (most > 2 * slots / units + 1) most = 2 * slots / units + 1;
+  const int G = q_heads / kv_heads;
+  const int64_t R = (int64_t)q_len * G;
+  p.tc = dtype == OC_BF16 && head_dim <= 128 && R > kTcRows && scale > 0.f;
+  int64_t units, slots = device_sm_count();
+  int step, setup;
+  if (p.tc) {
+    units = (int64_t)batch * kv_heads * tok_tc_shape(q_len, G).npairs;
+    p.row_tile = (int)R;
+    p.nrt = 1;
+    step = 128;
+    setup = 512;
+  } else {
+    p.row_tile = R <= 16 ? 16 : R <= 32 ? (dtype == OC_BF16 ? 32 : 16) : 64;
+    p.nrt = (int)((R + p.row_tile - 1) / p.row_tile);
+    units = (int64_t)batch * kv_heads * p.nrt;
+    slots *= 2;
+    step = 64;
+    setup = dtype == OC_BF16 ? 160 : 32;
+  }
+  int64_t most = seq_len / (2 * step);
+  if (most > 2 * slots / units + 4) most = 2 * slots / units + 4;
   int64_t best = 0;
   p.nchunk = 1;
-  p.chunk = seq_len < 64 ? 64 : (seq_len + 63) / 64 * 64;
+  p.chunk = seq_len < step ? step : (seq_len + step - 1) / step * step;
   for (int64_t n = 1; n <= most; ++n) {
-    const int64_t keys = ((seq_len + n - 1) / n + 63) / 64 * 64;
-    const int64_t cost = (units * n + slots - 1) / slots * (keys + (n > 1 ? 160 : 0));
+    const int64_t keys = ((seq_len + n - 1) / n + step - 1) / step * step;
+    const int64_t cost = (units * n + slots - 1) / slots * (keys + (n > 1 ? setup : 0));
     if (n == 1 || cost < best) {
       best = cost;
       p.chunk = (int)keys;
@@ -442,8 +464,7 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
     }
   }
   if (p.nchunk < 1) p.nchunk = 1;
-  if (p.chunk < 64) p.chunk = 64;
-  const size_t parts = p.nchunk > 1 ? (size_t)units * p.nchunk * p.row_tile : 0;
+  const size_t parts = p.nchunk > 1 ? (size_t)batch * kv_heads * p.nrt * p.nchunk * p.row_tile : 0;
   size_t off = 0;
   p.lse_off = off;
   if (lse) off += up256((size_t)batch * kv_heads * R * sizeof(float));
@@ -453,6 +474,8 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
   off += up256(parts * sizeof(float));
   p.o_off = off;
   off += up256(parts * head_dim * sizeof(float));
+  p.prep_off = off;
+  if (p.tc) off += up256(tok_tc_prep_bytes(batch, q_len, G, seq_len));
   p.bytes = off;
   return p;
 }
@@ -540,9 +563,10 @@ int tok_common(const char* fn, TokArgs& a, const void* q, const void* k, const v
 
 int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void* workspace, size_t workspace_bytes,
             cudaStream_t st) {
-  const TokPlan p = tok_plan(dtype, a.B, a.Sq, a.Hq, a.Hkv, head_dim, a.S, lse);
-  OC_REQUIRE((int64_t)a.B * a.Hkv * p.nrt * p.nchunk < INT32_MAX && p.nchunk <= 65535, OC_ERR_SHAPE,
-             "%s: too many work units", fn);
+  const TokPlan p = tok_plan(dtype, a.B, a.Sq, a.Hq, a.Hkv, head_dim, a.S, a.scale, lse);
+  OC_REQUIRE((int64_t)a.B * a.Hkv * p.nchunk * (p.tc ? tok_tc_shape(a.Sq, a.G).npairs : p.nrt) < INT32_MAX &&
+                 p.nchunk <= 65535,
+             OC_ERR_SHAPE, "%s: too many work units", fn);
   OC_REQUIRE(workspace_bytes >= p.bytes, OC_ERR_CAPACITY, "%s: workspace %zu < %zu bytes", fn, workspace_bytes,
              p.bytes);
   OC_REQUIRE(p.bytes == 0 || (workspace && aligned16(workspace)), p.bytes && !workspace ? OC_ERR_NULL : OC_ERR_ALIGN,
@@ -555,7 +579,9 @@ int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void*
   a.pl = reinterpret_cast<float*>(w + p.l_off);
   a.po = reinterpret_cast<float*>(w + p.o_off);
   a.lse = lse ? reinterpret_cast<float*>(w + p.lse_off) : nullptr;
-  int rc = dtype == OC_BF16 ? tok_mma(a, head_dim, p.row_tile, st) : dispatch_simt<float>(a, head_dim, p.row_tile, st);
+  int rc = p.tc ? tok_tc(fn, a, head_dim, w + p.prep_off, st)
+           : dtype == OC_BF16 ? tok_mma(a, head_dim, p.row_tile, st)
+                              : dispatch_simt<float>(a, head_dim, p.row_tile, st);
   if (rc) return rc;
   if (p.nchunk > 1) rc = tok_merge(a, head_dim, p.row_tile, st);
   return rc;
@@ -571,7 +597,10 @@ extern "C" size_t oc_token_attention_workspace_bytes(int dtype, int batch, int q
   if (batch < 1 || q_len < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || seq_len < 0 ||
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return 0;
-  return tok_plan(dtype, batch, q_len, q_heads, kv_heads, head_dim, seq_len, accumulate != 0).bytes;
+  // the larger of what a positive scale and any other need
+  const size_t pos = tok_plan(dtype, batch, q_len, q_heads, kv_heads, head_dim, seq_len, 1.f, accumulate != 0).bytes;
+  const size_t any = tok_plan(dtype, batch, q_len, q_heads, kv_heads, head_dim, seq_len, 0.f, accumulate != 0).bytes;
+  return pos > any ? pos : any;
 }
 
 extern "C" int oc_tree_attention(const void* q, const void* k, const void* v, int dtype, const int32_t* block_table,

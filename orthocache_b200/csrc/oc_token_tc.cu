@@ -1,0 +1,885 @@
+// Token-level attention on the 5th-generation tensor cores (bfloat16, head_dim
+// 64 or 128): drafted trees and query chunks with enough rows per KV head to
+// fill 128-row tiles.
+//
+// Mathematics and masks: oc_token.cuh.  Bound by the tensor cores and the
+// exponentials together: 4 D multiply-adds and one exponential (with a cap, a
+// five-term polynomial more) per row and key, 64 D bytes of keys and values per
+// 128-row tile and key.
+//
+// Layout (one persistent CTA of 384 threads per SM):
+//   * a row tile is 128 rows of one KV head: Gp neighbouring heads (the largest
+//     power of two that divides G = Hq / Hkv) x 128 / Gp query positions, so
+//     that few drafted tokens of many heads still fill a tile; a work unit is two
+//     row tiles that share every key tile, and one chunk of the keys;
+//   * warp 8 loads by TMA (128-byte swizzle): the two query tiles, then K and V
+//     tiles of 128 tokens into a ring; from the cache, its pages, or the drafted
+//     tokens;
+//   * warp 9 issues the tcgen05.mma: S_t = Q_t K^T into tensor memory, O_t +=
+//     P_t V with P_t from tensor memory; per key tile j in the order PV_0(j-1),
+//     S_0(j), PV_1(j-1), S_1(j), so that one tile's softmax runs under the other
+//     tile's products.  Before a V tile with tokens that nobody may see (behind
+//     the sequence, padding) is multiplied, the warp writes zeros over them:
+//     their weights are zero, but zero times whatever memory holds may not be;
+//   * warps 0-3 / 4-7 are the softmax of tile 0 / 1, a thread per row with all
+//     128 scores in registers (setmaxnreg moves registers to them from the
+//     other warps): one tensor-memory read per score.  The running maximum is
+//     left stale until a row's maximum has grown by 2^8 (exact: numerator and
+//     denominator use the same one), so O is rarely rescaled.  P is rounded to
+//     bfloat16 (half a step, 2^-8 of each weight); row sums are float32, taken
+//     before the rounding.
+//   * only key tiles that some row's limit or a document border cuts are masked
+//     element by element; tiles without a visible key are never loaded (causal
+//     limits; with documents, the span of tiles that hold a unit's documents,
+//     found by two small kernels beforehand).
+//   * cap tanh(x / cap): the score is odd in x, y = x (1 + u (a1 + ...)), u =
+//     (x / cap)^2, a least-squares fit of tanh(z) / z in z^2 on |z| <= 0.6 with
+//     equalised error (2.0e-8); a warp whose scores go beyond 0.6 cap takes cap -
+//     2 cap / (1 + e^(2 z)) instead, two MUFU operations a score more.
+// Every wait is bounded; one that gives up sets a status and an abort flag, and
+// the CTA frees its tensor memory and returns.
+#include <cuda.h>
+
+#include "oc_mma.cuh"
+#include "oc_tcgen05.cuh"
+#include "oc_token.cuh"
+
+namespace oc {
+
+__device__ int g_token_status = 0;
+
+namespace {
+
+constexpr int kRows = 128;  // rows of a tile (UMMA M)
+constexpr int kTok = 128;   // keys of a tile
+constexpr int kThreads = 384;
+constexpr int kProducerWarp = 8, kMmaWarp = 9;
+constexpr int kTmemCols = 512;
+
+template <int D> struct TcCfg {
+  static constexpr int kTileBytes = kRows * D * 2;
+  static constexpr int kBox = kRows * 128;               // one 128-row x 64-channel box
+  static constexpr int kSlots = D == 128 ? 5 : 10;
+};
+
+template <int D>
+struct TcSmem {
+  unsigned char q[2][TcCfg<D>::kTileBytes];
+  unsigned char kv[TcCfg<D>::kSlots][TcCfg<D>::kTileBytes];
+  uint64_t kv_full[TcCfg<D>::kSlots], kv_empty[TcCfg<D>::kSlots];
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2], p_full[2], o_free[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+
+struct TcArgs {
+  TokArgs t;
+  int Gp, nhs, P, tiles, npairs, units;  // row tiles per (b, h): nhs head groups x position tiles of P
+  int chunk_tiles;
+  const uint4* tree_bits;   // [(b, node)][2] ancestor bits; row T of each batch row: seen by any node
+  const int2* key_docs;     // [(b, key tile)] least and largest document
+  const int4* query_docs;   // [(b, position tile)] least, largest document; first key tile, last + 1
+  int nkt, npt;
+  float k_in;               // scale / cap
+};
+
+struct TcUnit {
+  int b, h, bh, chunk, len;
+  int ntile;
+  int p0[2], hs[2], min_hi[2];
+  int jt0, ncache, n;  // first cache tile, cache tiles, all tiles
+};
+
+__device__ __forceinline__ TcUnit tc_unit(const TcArgs& x, int u) {
+  const TokArgs& a = x.t;
+  TcUnit w;
+  const int per = x.npairs * a.nchunk;
+  w.bh = u / per;
+  const int rem = u % per;
+  const int pair = x.npairs - 1 - rem / a.nchunk;  // the rows with most keys first
+  w.chunk = rem % a.nchunk;
+  w.b = w.bh / a.Hkv;
+  w.h = w.bh % a.Hkv;
+  w.len = tok_len(a, w.b);
+  w.ntile = 2 * pair + 1 < x.tiles ? 2 : 1;
+  int first = INT32_MAX, last = 0, top = 0;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int r = 2 * pair + t, pt = r / x.nhs;
+    w.hs[t] = r % x.nhs;
+    w.p0[t] = pt * x.P;
+    w.min_hi[t] = 0;
+    if (t >= w.ntile) continue;
+    int hi = w.len, lo = w.len;
+    if (!a.dk) {
+      const int pos0 = w.len - a.Sq + w.p0[t], pos1 = w.len - a.Sq + min(w.p0[t] + x.P, a.Sq) - 1;
+      if (a.causal) {
+        const int pre = a.prefix ? a.prefix[w.b] : 0;
+        hi = min(w.len, max(pos1 + 1, pre));
+        lo = min(w.len, max(pos0 + 1, pre));
+      }
+      if (pos0 < 0) lo = 0;
+      if (pos1 < 0) hi = 0;
+    }
+    w.min_hi[t] = lo;
+    int t0 = 0, t1 = (hi + kTok - 1) / kTok;
+    if (a.docs) {
+      const int4 q = x.query_docs[(size_t)w.b * x.npt + pt];
+      t0 = q.z;
+      t1 = min(t1, q.w);
+    }
+    if (t0 < t1) {
+      first = min(first, t0);
+      last = max(last, t1);
+    }
+    top = max(top, hi);
+  }
+  const int c0 = w.chunk * x.chunk_tiles;
+  w.jt0 = max(first, c0);
+  w.ncache = max(0, min(last, c0 + x.chunk_tiles) - w.jt0);
+  if (first == INT32_MAX) w.ncache = 0;
+  w.n = w.ncache + (a.dk && w.chunk == a.nchunk - 1 ? (a.Sq + kTok - 1) / kTok : 0);
+  return w;
+}
+
+// First key row of cache tile jt in the (rows, Hkv, D) view; -1: no such page.
+__device__ __forceinline__ int tc_key_row(const TokArgs& a, int b, int jt) { return (int)tok_kv_row(a, b, jt * kTok); }
+
+template <int D>
+__device__ __forceinline__ bool tc_wait(TcSmem<D>& sm, uint64_t* bar, uint32_t parity) {
+  if (*(volatile int*)&sm.abort == 0 && mbar_wait(bar, parity)) return true;
+  if (atomicExch(&sm.abort, 1) == 0) atomicExch(&g_token_status, 1);
+  return false;
+}
+// The same for a whole warp, with one answer for all its lanes.
+template <int D>
+__device__ __forceinline__ bool tc_wait_warp(TcSmem<D>& sm, uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, tc_wait<D>(sm, bar, parity));
+}
+
+__device__ __forceinline__ uint64_t pk2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void up2(uint64_t r, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The cap in log2 units: cap' tanh(k s) with cap' = cap log2(e), k = scale / cap.
+struct CapFn {
+  float k, cap2;             // k_in, cap * log2(e)
+  float a0, a1, a2, a3, a4;  // the polynomial's coefficients in s^2, times cap' k
+  __device__ __forceinline__ CapFn(const TcArgs& x) {
+    k = x.k_in;
+    cap2 = x.t.cap * kLog2e;
+    const float k2 = k * k, c = cap2 * k;
+    a0 = c * 0.9999996423721313f;
+    a1 = c * k2 * -0.33331209421157837f;
+    a2 = c * k2 * k2 * 0.13299210369586945f;
+    a3 = c * k2 * k2 * k2 * -0.051696740090847015f;
+    a4 = c * k2 * k2 * k2 * k2 * 0.014976956881582737f;
+  }
+  __device__ __forceinline__ float exact(float s) const {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(2.f * kLog2e * k * s)));
+    return fmaf(-2.f * cap2, r, cap2);
+  }
+  __device__ __forceinline__ uint64_t poly2(uint64_t s, uint64_t off) const {  // cap' tanh(k s) + off
+    const uint64_t u = mul2(s, s);
+    uint64_t p = fma2(pk2(a4, a4), u, pk2(a3, a3));
+    p = fma2(p, u, pk2(a2, a2));
+    p = fma2(p, u, pk2(a1, a1));
+    p = fma2(p, u, pk2(a0, a0));
+    return fma2(p, s, off);
+  }
+};
+
+template <int D, bool CAP, bool BIAS>
+__device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem) {
+  const TokArgs& a = x.t;
+  const int rl = threadIdx.x & 127, lane = threadIdx.x & 31;
+  const uint32_t t_s = tmem + ((uint32_t)(threadIdx.x & 96) << 16) + t * 256;
+  const uint32_t t_o = t_s + 128;
+  const float c_scale = a.scale * kLog2e;
+  uint32_t ph = 0;
+  for (int u = blockIdx.x; u < x.units; u += gridDim.x) {
+    const TcUnit w = tc_unit(x, u);
+    if (t >= w.ntile) continue;
+    const int p0 = t ? w.p0[1] : w.p0[0], min_hi = t ? w.min_hi[1] : w.min_hi[0];
+    const int pos_i = p0 + rl / x.Gp;  // query position of this row
+    const int r = pos_i * a.G + (t ? w.hs[1] : w.hs[0]) * x.Gp + rl % x.Gp;
+    const bool real = pos_i < a.Sq;
+    const TokRow row = tok_row(a, w.b, w.h, real ? r : a.R, w.len);
+    int4 qd = make_int4(0, 0, 0, 0);
+    if (a.docs) qd = x.query_docs[(size_t)w.b * x.npt + p0 / x.P];
+    float m_used = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < w.n; ++j) {
+      // is every key of the tile visible to every row of it?
+      const bool draft = j >= w.ncache;
+      const int jt = draft ? j - w.ncache : w.jt0 + j, j0 = jt * kTok;
+      bool part = draft || j0 + kTok > min_hi || (a.table && tc_key_row(a, w.b, jt) < 0);
+      if (a.docs && !draft) {
+        const int2 kd = x.key_docs[(size_t)w.b * x.nkt + jt];
+        part = part || kd.x != kd.y || qd.x != kd.x || qd.y != kd.x;
+      }
+      if (!tc_wait_warp<D>(sm, &sm.s_full[t], ph)) {
+        ok = false;
+        break;
+      }
+      ph ^= 1;
+      tc_fence_after();
+      float s[128];
+      tmem_ld128_wait(t_s, s);
+      float mx;
+      bool far = false;  // a capped score beyond the polynomial
+      if (CAP) {
+        float hi8[4], lo8[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          hi8[k] = s[k];
+          lo8[k] = s[k];
+        }
+#pragma unroll
+        for (int i = 4; i < 124; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            hi8[k] = max3(hi8[k], s[i + k], s[i + 4 + k]);
+            lo8[k] = min3(lo8[k], s[i + k], s[i + 4 + k]);
+          }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          hi8[k] = fmaxf(hi8[k], s[124 + k]);
+          lo8[k] = fminf(lo8[k], s[124 + k]);
+        }
+        mx = fmaxf(fmaxf(hi8[0], hi8[1]), fmaxf(hi8[2], hi8[3]));
+        const float mn = fminf(fminf(lo8[0], lo8[1]), fminf(lo8[2], lo8[3]));
+        far = __any_sync(0xffffffffu, !(fmaxf(mx, -mn) * x.k_in <= 0.6f));
+      } else if (!BIAS && !part) {
+        float m8[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m8[k] = s[k];
+#pragma unroll
+        for (int i = 8; i < 120; i += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) m8[k] = max3(m8[k], s[i + k], s[i + 8 + k]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m8[k] = fmaxf(m8[k], s[120 + k]);
+        mx = fmaxf(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], max3(m8[5], m8[6], m8[7])));
+      }
+      const CapFn cap(x);
+      const bool direct = !BIAS && !part && !far;  // the exponent straight from the products
+      if (direct) {
+        if (CAP) {
+          float y0, y1;
+          up2(cap.poly2(pk2(mx, mx), 0), y0, y1);
+          mx = y0;
+        } else {
+          mx *= c_scale;
+        }
+      } else {
+        // scores in log2 units, biased and masked, in place
+        if (CAP) {
+          if (far) {
+#pragma unroll
+            for (int i = 0; i < 128; ++i) s[i] = cap.exact(s[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 128; i += 2) up2(cap.poly2(pk2(s[i], s[i + 1]), 0), s[i], s[i + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 128; ++i) s[i] *= c_scale;
+        }
+        if (BIAS) {
+          const float d0 = (float)(row.pos - j0);
+#pragma unroll
+          for (int i = 0; i < 128; ++i) s[i] = fmaf(-row.slope2, fabsf(d0 - (float)i), s[i]);
+        }
+        if (part) {
+          if (draft) {
+            const uint4 bits = real ? x.tree_bits[((size_t)w.b * (a.Sq + 1) + pos_i) * 2 + jt] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 128; ++i) {
+              const uint32_t word = i < 32 ? bits.x : i < 64 ? bits.y : i < 96 ? bits.z : bits.w;
+              if (!(word >> (i & 31) & 1)) s[i] = -INFINITY;
+            }
+          } else {
+            const int lim = a.table && tc_key_row(a, w.b, jt) < 0 ? 0 : row.hi - j0;
+#pragma unroll
+            for (int i = 0; i < 128; ++i)
+              if (i >= lim) s[i] = -INFINITY;
+            if (a.docs) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int jj = j0 + 32 * k + lane;
+                const int d = jj < a.S ? a.docs[(size_t)w.b * a.S + jj] : -1;
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  if (__shfl_sync(0xffffffffu, d, i) != row.doc) s[32 * k + i] = -INFINITY;
+              }
+            }
+          }
+        }
+        float m8[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m8[k] = s[k];
+#pragma unroll
+        for (int i = 8; i < 120; i += 16)
+#pragma unroll
+          for (int k = 0; k < 8; ++k) m8[k] = max3(m8[k], s[i + k], s[i + 8 + k]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m8[k] = fmaxf(m8[k], s[120 + k]);
+        mx = fmaxf(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], max3(m8[5], m8[6], m8[7])));
+      }
+      const bool need = mx > m_used + 8.f;
+      if (__any_sync(0xffffffffu, need)) {
+        const float alpha = need ? ex2(m_used - mx) : 1.f;  // 0 on a row's first visible tile
+        if (j > 0) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            tmem_ld32_wait(t_o + 32 * c, o);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= alpha;
+            tmem_st32(t_o + 32 * c, o);
+          }
+        }
+        l *= alpha;
+        if (need) m_used = mx;
+      }
+      const float base = m_used == -INFINITY ? 0.f : m_used;
+      // P = 2^(s - m) as bfloat16 pairs over the scores in tensor memory
+      uint64_t r2[4] = {0, 0, 0, 0};
+      const uint64_t nm2 = pk2(-base, -base), sc2 = pk2(c_scale, c_scale);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const uint64_t v = pk2(s[64 * half + 2 * i], s[64 * half + 2 * i + 1]);
+          uint64_t e;
+          if (!direct)
+            e = add2(v, nm2);
+          else if (CAP)
+            e = cap.poly2(v, nm2);
+          else
+            e = fma2(v, sc2, nm2);
+          float e0, e1;
+          up2(e, e0, e1);
+          e0 = ex2(e0);
+          e1 = ex2(e1);
+          r2[i & 3] = add2(r2[i & 3], pk2(e0, e1));
+          pk[i] = pack_bf16x2(e0, e1);
+        }
+        tmem_st32u(t_s + 32 * half, pk);
+      }
+      tc_wait_st();
+      {
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) up2(r2[i], q[2 * i], q[2 * i + 1]);
+        l += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+      }
+      tc_fence_before();
+      mbar_arrive(&sm.p_full[t]);
+    }
+    if (!ok) return;
+    if (w.n > 0) {
+      // the unit's last commit covers its last PV: O is complete
+      if (!tc_wait_warp<D>(sm, &sm.s_full[t], ph)) return;
+      ph ^= 1;
+      tc_fence_after();
+    }
+    if (w.n == 0) m_used = -INFINITY;
+    const int64_t part = ((int64_t)w.bh * a.nchunk + w.chunk) * a.R + r;
+    const int64_t at = tok_q_offset(a, w.b, w.h, real ? r : 0, D);
+    if (real) {
+      if (a.nchunk > 1) {
+        a.pm[part] = m_used;
+        a.pl[part] = l;
+      } else if (a.lse) {
+        a.lse[(int64_t)w.bh * a.R + r] = l == 0.f ? INFINITY : m_used + log2f(l);
+      }
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll 1
+    for (int c = 0; c < D / 32; ++c) {
+      float o[32];
+      if (w.n > 0) {
+        tmem_ld32_wait(t_o + 32 * c, o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0.f;
+      }
+      if (!real) continue;
+      if (a.nchunk > 1) {
+        if (m_used != -INFINITY) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(a.po + part * D + 32 * c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        }
+      } else if (a.out_dtype == OC_BF16) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8)
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + at + 32 * c + i) =
+              make_uint4(pack_bf16x2(o[i] * inv, o[i + 1] * inv), pack_bf16x2(o[i + 2] * inv, o[i + 3] * inv),
+                         pack_bf16x2(o[i + 4] * inv, o[i + 5] * inv), pack_bf16x2(o[i + 6] * inv, o[i + 7] * inv));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at + 32 * c + i) =
+              make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
+      }
+    }
+    if (w.n > 0) {
+      tc_fence_before();
+      mbar_arrive(&sm.o_free[t]);  // the next unit may overwrite S and O
+    }
+  }
+}
+
+template <int D>
+__device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* mq, const CUtensorMap* mk,
+                            const CUtensorMap* mv, const CUtensorMap* mdk, const CUtensorMap* mdv) {
+  using C = TcCfg<D>;
+  const TokArgs& a = x.t;
+  uint32_t q_ph = 0, L = 0;
+  // after a wait that gave up: let the copies in flight land (bounded) before
+  // the CTA ends
+  auto drain = [&]() {
+    for (uint32_t s = 0; s < C::kSlots && s < L; ++s)
+      mbar_wait(&sm.kv_full[s], ((L - s - 1) / C::kSlots) & 1);
+    mbar_wait(&sm.q_full, q_ph ^ 1);
+  };
+  for (int u = blockIdx.x; u < x.units; u += gridDim.x) {
+    const TcUnit w = tc_unit(x, u);
+    if (w.n == 0) continue;
+    if (!tc_wait<D>(sm, &sm.q_empty, q_ph ^ 1)) return drain();
+    q_ph ^= 1;
+    mbar_expect_tx(&sm.q_full, (uint32_t)(w.ntile * C::kTileBytes));
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (t < w.ntile)
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_3d(sm.q[t] + c * C::kBox, mq, &sm.q_full, 64 * c, w.h * a.G + w.hs[t] * x.Gp, w.b * a.Sq + w.p0[t]);
+    for (int j = 0; j < w.n; ++j) {
+      const bool draft = j >= w.ncache;
+      int key = draft ? w.b * a.Sq + (j - w.ncache) * kTok : tc_key_row(a, w.b, w.jt0 + j);
+      if (key < 0) key = 0;  // a page outside the pool: loaded from page 0, masked and zeroed
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv, ++L) {
+        const uint32_t slot = L % C::kSlots;
+        if (!tc_wait<D>(sm, &sm.kv_empty[slot], ((L / C::kSlots) & 1) ^ 1)) return drain();
+        mbar_expect_tx(&sm.kv_full[slot], C::kTileBytes);
+        const CUtensorMap* m = kv ? (draft ? mdv : mv) : (draft ? mdk : mk);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_3d(sm.kv[slot] + c * C::kBox, m, &sm.kv_full[slot], 64 * c, w.h, key);
+      }
+    }
+  }
+}
+
+// Zero the rows of the V tile in `slot` that no query may see.
+template <int D>
+__device__ __forceinline__ void tc_clean_values(TcSmem<D>& sm, const TcArgs& x, const TcUnit& w, int j, uint32_t slot) {
+  const TokArgs& a = x.t;
+  const int lane = threadIdx.x & 31;
+  const bool draft = j >= w.ncache;
+  const int jt = draft ? j - w.ncache : w.jt0 + j, j0 = jt * kTok;
+  uint4 seen = make_uint4(~0u, ~0u, ~0u, ~0u);
+  bool bad_page = false, pads = false;
+  if (draft) {
+    seen = x.tree_bits[((size_t)w.b * (a.Sq + 1) + a.Sq) * 2 + jt];
+    if ((seen.x & seen.y & seen.z & seen.w) == ~0u) return;
+  } else {
+    bad_page = a.table && tc_key_row(a, w.b, jt) < 0;
+    pads = a.docs && x.key_docs[(size_t)w.b * x.nkt + jt].x < 0;
+    if (j0 + kTok <= w.len && !bad_page && !pads) return;
+  }
+  for (int it = 0; it < kTok / 4; ++it) {
+    const int rr = it * 4 + (lane >> 3);
+    bool keep;
+    if (draft) {
+      const uint32_t word = rr < 32 ? seen.x : rr < 64 ? seen.y : rr < 96 ? seen.z : seen.w;
+      keep = word >> (rr & 31) & 1;
+    } else {
+      keep = j0 + rr < w.len && !bad_page && (!pads || a.docs[(size_t)w.b * a.S + j0 + rr] >= 0);
+    }
+    if (!keep)
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+        *reinterpret_cast<uint4*>(sm.kv[slot] + c * TcCfg<D>::kBox + rr * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async();
+}
+
+template <int D>
+__device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
+  using C = TcCfg<D>;
+  constexpr uint32_t kIdQK = tc_idesc_bf16(kRows, kTok, 0), kIdPV = tc_idesc_bf16(kRows, D, 1);
+  const bool lead = (threadIdx.x & 31) == 0;
+  uint32_t q_ph = 0, p_ph = 0, o_ph = 0, L = 0;
+  for (int u = blockIdx.x; u < x.units; u += gridDim.x) {
+    const TcUnit w = tc_unit(x, u);
+    if (w.n == 0) continue;
+    if (!tc_wait_warp<D>(sm, &sm.q_full, q_ph)) return;
+    q_ph ^= 1;
+    tc_fence_after();
+    uint32_t vslot = 0;
+    for (int j = 0; j <= w.n; ++j) {
+      uint32_t kslot = 0;
+      if (j < w.n) {
+        kslot = L % C::kSlots;
+        if (!tc_wait_warp<D>(sm, &sm.kv_full[kslot], (L / C::kSlots) & 1)) return;
+        tc_fence_after();
+      }
+      if (j > 0) {  // V of tile j - 1 is load L - 1
+        if (!tc_wait_warp<D>(sm, &sm.kv_full[vslot], ((L - 1) / C::kSlots) & 1)) return;
+        tc_clean_values<D>(sm, x, w, j - 1, vslot);
+        __syncwarp();
+        tc_fence_after();
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (t >= w.ntile) break;
+        const uint32_t d_s = tmem + t * 256, d_o = d_s + 128;
+        if (j > 0) {
+          if (!tc_wait_warp<D>(sm, &sm.p_full[t], (p_ph >> t) & 1)) return;
+          p_ph ^= 1u << t;
+          tc_fence_after();
+          if (lead) {
+            const uint32_t vb = smem_u32(sm.kv[vslot]);
+#pragma unroll
+            for (int kk = 0; kk < kTok / 16; ++kk)
+              umma_bf16_ts(d_o, d_s + kk * 8, sdesc(vb + kk * 2048, C::kBox, 1024), kIdPV, (j > 1 || kk > 0) ? 1 : 0);
+            if (t == w.ntile - 1) umma_commit(&sm.kv_empty[vslot]);
+          }
+        }
+        if (j == 0) {  // the softmax has read the previous unit's O_t
+          if (!tc_wait_warp<D>(sm, &sm.o_free[t], ((o_ph >> t) & 1) ^ 1)) return;
+          o_ph ^= 1u << t;
+          tc_fence_after();
+        }
+        if (lead) {
+          if (j < w.n) {
+            const uint32_t qa = smem_u32(sm.q[t]), kb = smem_u32(sm.kv[kslot]);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk >> 2) * C::kBox + (kk & 3) * 32;
+              umma_bf16(d_s, sdesc(qa + off, 16, 1024), sdesc(kb + off, 16, 1024), kIdQK, kk > 0 ? 1 : 0);
+            }
+          }
+          umma_commit(&sm.s_full[t]);
+          if (j < w.n && t == w.ntile - 1) {
+            umma_commit(&sm.kv_empty[kslot]);
+            if (j == w.n - 1) umma_commit(&sm.q_empty);
+          }
+        }
+        __syncwarp();
+      }
+      if (j < w.n) {
+        vslot = (L + 1) % C::kSlots;
+        L += 2;
+      }
+    }
+  }
+}
+
+template <int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1)
+    tok_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                  const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdk,
+                  const __grid_constant__ CUtensorMap mdv, const __grid_constant__ TcArgs x) {
+  extern __shared__ unsigned char raw[];
+  TcSmem<D>& sm = *reinterpret_cast<TcSmem<D>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < TcCfg<D>::kSlots; ++i) {
+      mbar_init(&sm.kv_full[i], 1);
+      mbar_init(&sm.kv_empty[i], 1);
+    }
+    mbar_init(&sm.q_full, 1);
+    mbar_init(&sm.q_empty, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&sm.s_full[t], 1);
+      mbar_init(&sm.p_full[t], 128);
+      mbar_init(&sm.o_free[t], 128);
+    }
+    mbar_init(&sm.drain, 1);
+    sm.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+
+  // 384 threads x 168 registers = 256 x 208 + 128 x 88
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    tc_softmax<D, CAP, BIAS>(sm, x, warp >> 2, tmem);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == kProducerWarp) {
+      if ((threadIdx.x & 31) == 0) tc_producer<D>(sm, x, &mq, &mk, &mv, &mdk, &mdv);
+      __syncwarp();
+    } else if (warp == kMmaWarp) {
+      tc_mma<D>(sm, x, tmem);
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) {
+        umma_commit(&sm.drain);  // every MMA in flight, before the memory is freed
+        if (!mbar_wait(&sm.drain, 0)) atomicExch(&g_token_status, 1);
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+// Ancestor bits of a tree's nodes (row i: 256 bits) and, in row T, the drafted
+// tokens that any node sees.  One CTA per batch row, a warp per node.
+__global__ void __launch_bounds__(1024) tok_tree_bits_kernel(const uint8_t* tree, int64_t bstride, int T, uint32_t* bits) {
+  __shared__ uint32_t seen[8];
+  if (threadIdx.x < 8) seen[threadIdx.x] = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  const uint8_t* tm = tree + blockIdx.x * bstride;
+  uint32_t* out = bits + (size_t)blockIdx.x * (T + 1) * 8;
+  for (int i = threadIdx.x >> 5; i < T; i += 32) {
+    uint32_t mine = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      const int s = w * 32 + lane;
+      const uint32_t word = __ballot_sync(0xffffffffu, s < T && tm[(int64_t)i * T + s] != 0);
+      if (lane == w) mine = word;
+    }
+    if (lane < 8) {
+      out[i * 8 + lane] = mine;
+      if (mine) atomicOr(&seen[lane], mine);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 8) out[T * 8 + threadIdx.x] = seen[threadIdx.x];
+}
+
+// Least and largest document of every 128-key tile (keys behind the sequence
+// count as padding); one warp per tile.
+__global__ void __launch_bounds__(128) tok_key_docs_kernel(const TokArgs a, int nkt, int2* key_docs) {
+  const int tile = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (tile >= a.B * nkt) return;
+  const int b = tile / nkt, j0 = tile % nkt * kTok, len = tok_len(a, b);
+  int lo = INT32_MAX, hi = -1;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int j = j0 + 32 * k + lane;
+    const int d = j < len ? a.docs[(size_t)b * a.S + j] : -1;
+    lo = min(lo, d < 0 ? -1 : d);
+    hi = max(hi, d);
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) key_docs[tile] = make_int2(lo, hi);
+}
+
+// Least (-1 with padding among them) and largest document of the P query
+// positions of a position tile, and the span of key tiles that hold any
+// document between; one warp per tile.
+__global__ void __launch_bounds__(128) tok_query_docs_kernel(const TokArgs a, int P, int npt, int nkt,
+                                                             const int2* key_docs, int4* query_docs) {
+  pdl_wait();
+  const int tile = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (tile >= a.B * npt) return;
+  const int b = tile / npt, p0 = tile % npt * P, len = tok_len(a, b);
+  int lo = INT32_MAX, least = INT32_MAX, hi = -1;
+  for (int i = p0 + lane; i < min(p0 + P, a.Sq); i += 32) {
+    const int pos = len - a.Sq + i;
+    const int d = pos >= 0 ? a.docs[(size_t)b * a.S + pos] : -1;
+    lo = min(lo, d < 0 ? -1 : d);
+    if (d >= 0) least = min(least, d);
+    hi = max(hi, d);
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  least = __reduce_min_sync(0xffffffffu, least);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  int first = INT32_MAX, last = 0;
+  for (int k = lane; k < nkt; k += 32) {
+    const int2 kd = key_docs[(size_t)b * nkt + k];
+    if (kd.x <= hi && kd.y >= least) {
+      first = min(first, k);
+      last = max(last, k + 1);
+    }
+  }
+  first = __reduce_min_sync(0xffffffffu, first);
+  last = __reduce_max_sync(0xffffffffu, last);
+  if (lane == 0) query_docs[tile] = make_int4(lo, hi, first, last);
+}
+
+int tc_map(CUtensorMap* m, const void* base, int D, int heads, int64_t rows, int box_heads, int box_rows,
+           const char* fn) {
+  const uint64_t dims[3] = {(uint64_t)D, (uint64_t)heads, (uint64_t)rows};
+  const uint64_t strides[2] = {(uint64_t)D * 2, (uint64_t)heads * D * 2};
+  const uint32_t box[3] = {64, (uint32_t)box_heads, (uint32_t)box_rows};
+  const int r = encode_map_3d(m, base, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, dims, strides, box, true);
+  if (r) return set_error(OC_ERR_CUDA, "%s: tensor map failed (CUresult %d)", fn, r);
+  return OC_OK;
+}
+
+template <int D, bool CAP, bool BIAS>
+int launch_tc(const CUtensorMap (&m)[5], const TcArgs& x, cudaStream_t st) {
+  const size_t smem = sizeof(TcSmem<D>) + 1024;
+  auto kern = tok_tc_kernel<D, CAP, BIAS>;
+  static std::atomic<uint64_t> done{0};
+  if (first_on_device(done)) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_tc_kernel: %s", cudaGetErrorString(e));
+  }
+  const int sms = device_sm_count();
+  const dim3 grid((unsigned)(x.units < sms ? x.units : sms));
+  cudaError_t e;
+  if (x.tree_bits || x.query_docs) {
+    e = launch_pdl(kern, grid, dim3(kThreads), smem, st, m[0], m[1], m[2], m[3], m[4], x);
+  } else {
+    kern<<<grid, kThreads, smem, st>>>(m[0], m[1], m[2], m[3], m[4], x);
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_tc_kernel: %s", cudaGetErrorString(e));
+  return OC_OK;
+}
+
+template <int D>
+int launch_tc_form(const CUtensorMap (&m)[5], const TcArgs& x, cudaStream_t st) {
+  if (x.t.cap > 0.f) return x.t.slopes ? launch_tc<D, true, true>(m, x, st) : launch_tc<D, true, false>(m, x, st);
+  return x.t.slopes ? launch_tc<D, false, true>(m, x, st) : launch_tc<D, false, false>(m, x, st);
+}
+
+}  // namespace
+
+// Row tiles: Gp heads x P positions.
+TokTcShape tok_tc_shape(int q_len, int G) {
+  TokTcShape s;
+  s.Gp = 1;
+  while (s.Gp < kRows && G % (2 * s.Gp) == 0) s.Gp *= 2;
+  s.nhs = G / s.Gp;
+  s.P = kRows / s.Gp;
+  s.npt = (q_len + s.P - 1) / s.P;
+  s.npairs = (s.npt * s.nhs + 1) / 2;
+  return s;
+}
+
+size_t tok_tc_prep_bytes(int batch, int q_len, int G, int seq_len) {
+  const TokTcShape s = tok_tc_shape(q_len, G);
+  const size_t tree = q_len <= kMaxNodes ? (size_t)batch * (q_len + 1) * 32 : 0;
+  const size_t docs = (size_t)batch * s.npt * sizeof(int4) + (size_t)batch * ((seq_len + kTok - 1) / kTok) * sizeof(int2);
+  return tree > docs ? tree : docs;
+}
+
+int tok_tc(const char* fn, const TokArgs& a, int head_dim, void* prep, cudaStream_t st) {
+  const TokTcShape s = tok_tc_shape(a.Sq, a.G);
+  TcArgs x = {};
+  x.t = a;
+  x.Gp = s.Gp;
+  x.nhs = s.nhs;
+  x.P = s.P;
+  x.tiles = s.npt * s.nhs;
+  x.npairs = s.npairs;
+  x.units = a.B * a.Hkv * s.npairs * a.nchunk;
+  x.chunk_tiles = a.chunk / kTok;
+  x.nkt = (a.S + kTok - 1) / kTok;
+  x.npt = s.npt;
+  x.k_in = a.cap > 0.f ? a.scale / a.cap : 0.f;
+  CUtensorMap m[5];
+  int rc = tc_map(&m[0], a.q, head_dim, a.Hq, (int64_t)a.B * a.Sq, s.Gp, s.P, fn);
+  if (rc) return rc;
+  m[1] = m[2] = m[3] = m[4] = m[0];
+  if (a.S > 0) {
+    const int64_t rows = a.table ? (int64_t)a.num_pages * a.page : (int64_t)a.B * a.S;
+    rc = tc_map(&m[1], a.k, head_dim, a.Hkv, rows, 1, kTok, fn);
+    if (!rc) rc = tc_map(&m[2], a.v, head_dim, a.Hkv, rows, 1, kTok, fn);
+    if (rc) return rc;
+  }
+  if (a.dk) {
+    rc = tc_map(&m[3], a.dk, head_dim, a.Hkv, (int64_t)a.B * a.Sq, 1, kTok, fn);
+    if (!rc) rc = tc_map(&m[4], a.dv, head_dim, a.Hkv, (int64_t)a.B * a.Sq, 1, kTok, fn);
+    if (rc) return rc;
+    x.tree_bits = static_cast<const uint4*>(prep);
+    tok_tree_bits_kernel<<<a.B, 1024, 0, st>>>(a.tree, a.tree_bstride, a.Sq, static_cast<uint32_t*>(prep));
+    rc = check_launch("tok_tree_bits_kernel");
+    if (rc) return rc;
+  } else if (a.docs && a.S > 0) {
+    int4* qd = static_cast<int4*>(prep);
+    int2* kd = reinterpret_cast<int2*>(qd + (size_t)a.B * s.npt);
+    x.query_docs = qd;
+    x.key_docs = kd;
+    tok_key_docs_kernel<<<(unsigned)(((int64_t)a.B * x.nkt + 3) / 4), 128, 0, st>>>(a, x.nkt, kd);
+    rc = check_launch("tok_key_docs_kernel");
+    if (rc) return rc;
+    cudaError_t e = launch_pdl(tok_query_docs_kernel, dim3((unsigned)(((int64_t)a.B * s.npt + 3) / 4)), dim3(128), 0, st,
+                               a, s.P, s.npt, x.nkt, static_cast<const int2*>(kd), qd);
+    if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_query_docs_kernel: %s", cudaGetErrorString(e));
+  } else if (a.docs) {
+    x.t.docs = nullptr;  // an empty cache: no row sees anything
+  }
+  return head_dim == 64 ? launch_tc_form<64>(m, x, st) : launch_tc_form<128>(m, x, st);
+}
+
+int wait_limit_token(unsigned long long ns) { return set_wait_limit_here(ns); }
+int token_status(int* status, int reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_token_status, sizeof(int));
+  if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "oc_device_status: %s", cudaGetErrorString(e));
+  if (reset) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_token_status, &zero, sizeof(int));
+    if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "oc_device_status: %s", cudaGetErrorString(e));
+  }
+  return OC_OK;
+}
+
+}  // namespace oc
