@@ -38,6 +38,8 @@ struct TokArgs {
   // split over the keys: chunk c covers tokens [c * chunk, (c + 1) * chunk)
   int chunk, nchunk, nrt;        // nrt row tiles per (b, h)
   float *pm, *pl, *po;           // partials: [(bh * nrt + rt) * nchunk + c][row tile][(D)]
+  float* logits;                 // (B * Hkv, R, logit_stride) scores in log2 units, -inf where masked; nullable
+  int64_t logit_stride;
   float* lse;                    // (B * Hkv, R) log2 of the softmax denominator, +inf for empty rows; nullable
 };
 
@@ -119,6 +121,10 @@ struct TokTcShape {
 TokTcShape tok_tc_shape(int q_len, int G);
 size_t tok_tc_prep_bytes(int batch, int q_len, int G, int seq_len);
 int tok_tc(const char* fn, const TokArgs& a, int head_dim, void* prep, cudaStream_t st);
+
+// Column sums of the softmax on the tcgen05 tensor cores, from a.lse
+// (bfloat16, head_dim 64 or 128, contiguous keys, positive scale).
+int tok_tc_weights(const char* fn, const TokArgs& a, int head_dim, const float* w_in, float* w_out, cudaStream_t st);
 
 // Merge of the partials of all chunks (oc_token_attention.cu).
 int tok_merge(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st);

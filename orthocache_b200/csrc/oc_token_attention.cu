@@ -389,6 +389,23 @@ __global__ void __launch_bounds__(kSimtThreads) tok_weights_kernel(const TokArgs
   }
 }
 
+// Column sums from stored scores (few rows): a thread per key, rows in order.
+__global__ void __launch_bounds__(256) tok_sum_kernel(const TokArgs a, const float* w_in, float* w_out) {
+  const int bh = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= a.S) return;
+  const int64_t at = (int64_t)bh * a.S + j;
+  const int len = tok_len(a, bh / a.Hkv);
+  pdl_wait();
+  const float before = w_in ? w_in[at] : 0.f;
+  float sum = 0.f;
+  if (j < len) {
+    const float* s = a.logits + (int64_t)bh * a.R * a.logit_stride + j;
+#pragma unroll 8
+    for (int r = 0; r < a.R; ++r) sum += exp2f(s[r * a.logit_stride] - a.lse[(int64_t)bh * a.R + r]);
+  }
+  w_out[at] = before + sum;
+}
+
 }  // namespace
 
 int tok_merge(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st) {
@@ -412,7 +429,7 @@ struct TokPlan {
   bool tc;            // the tcgen05 kernel
   int row_tile, nrt;  // rows per tile, row tiles per (b, h)
   int chunk, nchunk;  // keys per chunk, chunks
-  size_t lse_off, m_off, l_off, o_off, prep_off, bytes;
+  size_t lse_off, m_off, l_off, o_off, prep_off, logit_off, logit_stride, bytes;  // logit_stride 0: none
 };
 
 inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -426,6 +443,12 @@ inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // the one with the least waves x (keys of a chunk + what a CTA's set-up and its
 // partial cost, in keys) is taken.
 constexpr int kTcRows = 64;
+
+// The accumulating form needs every score again once the denominators are
+// known.  Up to kLogitRows rows per KV head the bfloat16 kernel stores them
+// (4 bytes a row and key, against 2 D bytes of a key to multiply again: at 16
+// rows and 128 channels 64 against 256); beyond, they are recomputed.
+constexpr int kLogitRows = 16;
 
 TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int head_dim, int seq_len, float scale,
                  bool lse) {
@@ -476,6 +499,12 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
   off += up256(parts * head_dim * sizeof(float));
   p.prep_off = off;
   if (p.tc) off += up256(tok_tc_prep_bytes(batch, q_len, G, seq_len));
+  p.logit_off = off;
+  p.logit_stride = 0;
+  if (lse && dtype == OC_BF16 && R <= kLogitRows) {
+    p.logit_stride = (seq_len + 63) / 64 * 64;  // whole tiles
+    off += up256((size_t)batch * kv_heads * R * p.logit_stride * sizeof(float));
+  }
   p.bytes = off;
   return p;
 }
@@ -562,7 +591,7 @@ int tok_common(const char* fn, TokArgs& a, const void* q, const void* k, const v
 }
 
 int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void* workspace, size_t workspace_bytes,
-            cudaStream_t st) {
+            cudaStream_t st, const float* w_in = nullptr, float* w_out = nullptr) {
   const TokPlan p = tok_plan(dtype, a.B, a.Sq, a.Hq, a.Hkv, head_dim, a.S, a.scale, lse);
   OC_REQUIRE((int64_t)a.B * a.Hkv * p.nchunk * (p.tc ? tok_tc_shape(a.Sq, a.G).npairs : p.nrt) < INT32_MAX &&
                  p.nchunk <= 65535,
@@ -579,12 +608,25 @@ int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void*
   a.pl = reinterpret_cast<float*>(w + p.l_off);
   a.po = reinterpret_cast<float*>(w + p.o_off);
   a.lse = lse ? reinterpret_cast<float*>(w + p.lse_off) : nullptr;
+  a.logits = p.logit_stride ? reinterpret_cast<float*>(w + p.logit_off) : nullptr;
+  a.logit_stride = (int64_t)p.logit_stride;
   int rc = p.tc ? tok_tc(fn, a, head_dim, w + p.prep_off, st)
            : dtype == OC_BF16 ? tok_mma(a, head_dim, p.row_tile, st)
                               : dispatch_simt<float>(a, head_dim, p.row_tile, st);
   if (rc) return rc;
   if (p.nchunk > 1) rc = tok_merge(a, head_dim, p.row_tile, st);
-  return rc;
+  if (rc || !w_out || a.S == 0) return rc;
+  // the column sums
+  if (a.logits) {
+    const dim3 grid((unsigned)((a.S + 255) / 256), (unsigned)(a.B * a.Hkv));
+    OC_REQUIRE(grid.y <= 65535, OC_ERR_SHAPE, "%s: too many heads", fn);
+    cudaError_t e = launch_pdl(tok_sum_kernel, grid, dim3(256), 0, st, a, w_in, w_out);
+    if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_sum_kernel: %s", cudaGetErrorString(e));
+    return OC_OK;
+  }
+  if (dtype == OC_BF16 && head_dim <= 128 && a.scale > 0.f) return tok_tc_weights(fn, a, head_dim, w_in, w_out, st);
+  return dtype == OC_BF16 ? dispatch_weights<__nv_bfloat16>(a, head_dim, w_in, w_out, st)
+                          : dispatch_weights<float>(a, head_dim, w_in, w_out, st);
 }
 
 }  // namespace
@@ -667,9 +709,6 @@ extern "C" int oc_accumulate_attention(const void* q, const void* k, const void*
   OC_REQUIRE(weights_out || seq_len == 0, OC_ERR_NULL, "oc_accumulate_attention: NULL pointer");
   a.lengths = lengths;
   a.causal = 1;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  rc = tok_run("oc_accumulate_attention", a, dtype, head_dim, true, workspace, workspace_bytes, st);
-  if (rc || seq_len == 0) return rc;
-  return dtype == OC_BF16 ? dispatch_weights<__nv_bfloat16>(a, head_dim, weights_in, weights_out, st)
-                          : dispatch_weights<float>(a, head_dim, weights_in, weights_out, st);
+  return tok_run("oc_accumulate_attention", a, dtype, head_dim, true, workspace, workspace_bytes,
+                 reinterpret_cast<cudaStream_t>(stream), weights_in, weights_out);
 }

@@ -270,6 +270,17 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
         }
     }
 
+    if (WR == 1 && a.logits && wd == 0) {  // kept for the column sums (few rows only)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = rt * RT + wr * 16 + g + 8 * i;
+        if (r >= a.R) continue;
+        float* dst = a.logits + ((int64_t)bh * a.R + r) * a.logit_stride + j0 + c2;
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(s[n][2 * i], s[n][2 * i + 1]);
+      }
+    }
+
     // running softmax of the warp's 16 rows (a row's tokens lie in 4 lanes)
     uint32_t p[C::NT][2];
     float alpha[2];

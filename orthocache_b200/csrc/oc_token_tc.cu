@@ -684,6 +684,289 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// ---------------------------------------------------------------------------
+// Column sums of the softmax, for the accumulating form with more rows than
+// the scores are worth storing for: with the denominators known, the scores
+// are multiplied again with the keys as the rows of the tile, S^T = K Q^T, so
+// that a thread (a tensor-memory lane) owns one key and adds its weights over
+// all query rows in its own registers, in the order of the rows: no exchange
+// between threads, no atomics.  One MMA and one exponential per row and key:
+// bound by the exponentials.  A unit is two tiles of 128 keys of one (b, h)
+// that share every query tile; two score buffers per key tile in tensor memory
+// let the products run ahead of the exponentials.
+// ---------------------------------------------------------------------------
+constexpr int kWqSlots = 4;
+
+template <int D>
+struct TwSmem {
+  unsigned char k[2][TcCfg<D>::kTileBytes];
+  unsigned char q[kWqSlots][TcCfg<D>::kTileBytes];
+  float lse[kWqSlots][kRows];
+  uint64_t k_full, k_empty;
+  uint64_t q_full[kWqSlots], q_empty[kWqSlots];
+  uint64_t s_full[2][2], s_empty[2][2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+
+struct TwUnit {
+  int b, h, bh, len, j0, ntile, r0, n;  // first key, key tiles with keys, first row tile, row tiles
+};
+
+__device__ __forceinline__ TwUnit tw_unit(const TcArgs& x, int u) {
+  const TokArgs& a = x.t;
+  TwUnit w;
+  const int BH = a.B * a.Hkv;
+  w.bh = u % BH;
+  w.b = w.bh / a.Hkv;
+  w.h = w.bh % a.Hkv;
+  w.len = tok_len(a, w.b);
+  w.j0 = u / BH * 2 * kTok;  // the first keys, which most rows see, come first
+  w.ntile = w.j0 + kTok < w.len ? 2 : 1;
+  const int before = w.j0 - (w.len - a.Sq);  // query positions that lie before the unit's first key
+  w.r0 = (before > 0 ? before / x.P : 0) * x.nhs;
+  w.n = w.j0 < w.len ? max(0, x.tiles - w.r0) : 0;
+  return w;
+}
+
+template <int D>
+__device__ __forceinline__ bool tw_wait(TwSmem<D>& sm, uint64_t* bar, uint32_t parity) {
+  const bool ok = *(volatile int*)&sm.abort == 0 && mbar_wait(bar, parity);
+  if (!ok && atomicExch(&sm.abort, 1) == 0) atomicExch(&g_token_status, 1);
+  return __all_sync(0xffffffffu, ok);
+}
+
+template <int D>
+__device__ void tw_producer(TwSmem<D>& sm, const TcArgs& x, const CUtensorMap* mq, const CUtensorMap* mk) {
+  using C = TcCfg<D>;
+  const TokArgs& a = x.t;
+  const int lane = threadIdx.x & 31;
+  uint32_t k_ph = 0, L = 0;
+  auto drain = [&]() {  // let the copies in flight land (bounded)
+    for (uint32_t s = 0; s < kWqSlots && s < L; ++s) mbar_wait(&sm.q_full[s], ((L - s - 1) / kWqSlots) & 1);
+    mbar_wait(&sm.k_full, k_ph ^ 1);
+  };
+  for (int u = blockIdx.x; u < x.units; u += gridDim.x) {
+    const TwUnit w = tw_unit(x, u);
+    if (w.n == 0) continue;
+    if (!tw_wait<D>(sm, &sm.k_empty, k_ph ^ 1)) return drain();
+    k_ph ^= 1;
+    if (lane == 0) {
+      mbar_expect_tx(&sm.k_full, (uint32_t)(w.ntile * C::kTileBytes));
+      for (int t = 0; t < w.ntile; ++t)
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_3d(sm.k[t] + c * C::kBox, mk, &sm.k_full, 64 * c, w.h, w.b * a.S + w.j0 + t * kTok);
+    }
+    for (int i = 0; i < w.n; ++i, ++L) {
+      const int r = w.r0 + i, p0 = r / x.nhs * x.P, hs = r % x.nhs;
+      float lse[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int col = 32 * k + lane, pos = p0 + col / x.Gp;
+        lse[k] = pos < a.Sq ? a.lse[(int64_t)w.bh * a.R + (int64_t)pos * a.G + hs * x.Gp + col % x.Gp] : INFINITY;
+      }
+      const uint32_t slot = L % kWqSlots;
+      if (!tw_wait<D>(sm, &sm.q_empty[slot], ((L / kWqSlots) & 1) ^ 1)) return drain();
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sm.lse[slot][32 * k + lane] = lse[k];
+      if (lane == 0) {
+        mbar_expect_tx(&sm.q_full[slot], C::kTileBytes);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_3d(sm.q[slot] + c * C::kBox, mq, &sm.q_full[slot], 64 * c, w.h * a.G + hs * x.Gp, w.b * a.Sq + p0);
+      } else {
+        mbar_arrive(&sm.q_full[slot]);
+      }
+    }
+  }
+}
+
+template <int D>
+__device__ void tw_mma(TwSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
+  using C = TcCfg<D>;
+  constexpr uint32_t kId = tc_idesc_bf16(kTok, kRows, 0);
+  const bool lead = (threadIdx.x & 31) == 0;
+  uint32_t k_ph = 0, L = 0, use[2] = {0, 0};
+  for (int u = blockIdx.x; u < x.units; u += gridDim.x) {
+    const TwUnit w = tw_unit(x, u);
+    if (w.n == 0) continue;
+    if (!tw_wait<D>(sm, &sm.k_full, k_ph)) return;
+    k_ph ^= 1;
+    for (int i = 0; i < w.n; ++i, ++L) {
+      const uint32_t slot = L % kWqSlots;
+      if (!tw_wait<D>(sm, &sm.q_full[slot], (L / kWqSlots) & 1)) return;
+      tc_fence_after();
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (t >= w.ntile) break;
+        const uint32_t buf = use[t] & 1;
+        if (!tw_wait<D>(sm, &sm.s_empty[t][buf], ((use[t] >> 1) & 1) ^ 1)) return;
+        ++use[t];
+        tc_fence_after();
+        if (lead) {
+          const uint32_t ka = smem_u32(sm.k[t]), qb = smem_u32(sm.q[slot]);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * C::kBox + (kk & 3) * 32;
+            umma_bf16(tmem + t * 256 + buf * 128, sdesc(ka + off, 16, 1024), sdesc(qb + off, 16, 1024), kId, kk > 0 ? 1 : 0);
+          }
+          umma_commit(&sm.s_full[t][buf]);
+        }
+        __syncwarp();
+      }
+      if (lead) {
+        umma_commit(&sm.q_empty[slot]);
+        if (i == w.n - 1) umma_commit(&sm.k_empty);
+      }
+      __syncwarp();
+    }
+  }
+}
+
+template <int D, bool CAP>
+__device__ void tw_sum(TwSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem, const float* w_in, float* w_out) {
+  const TokArgs& a = x.t;
+  const int lane = threadIdx.x & 31, kl = threadIdx.x & 127;
+  const uint32_t t_s = tmem + ((uint32_t)(threadIdx.x & 96) << 16) + t * 256;
+  const float c_scale = a.scale * kLog2e;
+  const CapFn cap(x);
+  uint32_t L = 0, use = 0;
+  for (int u = blockIdx.x; u < x.units; u += gridDim.x) {
+    const TwUnit w = tw_unit(x, u);
+    const int j = w.j0 + t * kTok + kl;
+    uint64_t acc[4] = {0, 0, 0, 0};
+    float edge = 0.f;
+    for (int i = 0; i < w.n; ++i, ++L) {
+      const uint32_t slot = L % kWqSlots;
+      if (!tw_wait<D>(sm, &sm.q_full[slot], (L / kWqSlots) & 1)) return;  // the denominators
+      if (t < w.ntile) {
+        const uint32_t buf = use & 1;
+        if (!tw_wait<D>(sm, &sm.s_full[t][buf], (use >> 1) & 1)) return;
+        ++use;
+        tc_fence_after();
+        float s[128];
+        tmem_ld128_wait(t_s + buf * 128, s);
+        tc_fence_before();
+        mbar_arrive(&sm.s_empty[t][buf]);
+        const int r = w.r0 + i, p0 = r / x.nhs * x.P, pos0 = w.len - a.Sq + p0;
+        const float4* lse = reinterpret_cast<const float4*>(sm.lse[slot]);
+        // rows [lo, hi) of the tile see this thread's key
+        const bool part = w.j0 + t * kTok + kTok - 1 > pos0 || p0 + x.P > a.Sq;
+        bool far = false;
+        if (CAP) {
+          float top[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 128; k += 4)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) top[y] = fmaxf(top[y], fabsf(s[k + y]));
+          far = __any_sync(0xffffffffu, !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * x.k_in <= 0.6f));
+        }
+        if (!part && !far) {
+          const uint64_t sc2 = pk2(c_scale, c_scale);
+#pragma unroll
+          for (int k = 0; k < 128; k += 4) {
+            const float4 z = lse[k / 4];
+            const uint64_t n0 = pk2(-z.x, -z.y), n1 = pk2(-z.z, -z.w);
+            uint64_t e0, e1;
+            if (CAP) {
+              e0 = cap.poly2(pk2(s[k], s[k + 1]), n0);
+              e1 = cap.poly2(pk2(s[k + 2], s[k + 3]), n1);
+            } else {
+              e0 = fma2(pk2(s[k], s[k + 1]), sc2, n0);
+              e1 = fma2(pk2(s[k + 2], s[k + 3]), sc2, n1);
+            }
+            float a0, a1, b0, b1;
+            up2(e0, a0, a1);
+            up2(e1, b0, b1);
+            acc[(k / 2) & 3] = add2(acc[(k / 2) & 3], pk2(ex2(a0), ex2(a1)));
+            acc[(k / 2 + 1) & 3] = add2(acc[(k / 2 + 1) & 3], pk2(ex2(b0), ex2(b1)));
+          }
+        } else {
+          const int lo = max(0, (j - pos0) * x.Gp), hi = min(kRows, (a.Sq - p0) * x.Gp);
+#pragma unroll
+          for (int k = 0; k < 128; ++k) {
+            const float v = CAP ? cap.exact(s[k]) : s[k] * c_scale;
+            const float z = sm.lse[slot][k];
+            if (k >= lo && k < hi && z != INFINITY) edge += ex2(v - z);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.q_empty[slot]);
+    }
+    if (j < a.S) {
+      const int64_t at = (int64_t)w.bh * a.S + j;
+      float q[8];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) up2(acc[y], q[2 * y], q[2 * y + 1]);
+      float sum = ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7])) + edge;
+      if (j >= w.len) sum = 0.f;
+      w_out[at] = (w_in ? w_in[at] : 0.f) + sum;
+    }
+  }
+}
+
+template <int D, bool CAP>
+__global__ void __launch_bounds__(kThreads, 1)
+    tok_tc_weights_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                          const __grid_constant__ TcArgs x, const float* w_in, float* w_out) {
+  extern __shared__ unsigned char raw[];
+  TwSmem<D>& sm = *reinterpret_cast<TwSmem<D>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    mbar_init(&sm.k_full, 1);
+    mbar_init(&sm.k_empty, 1);
+    for (int i = 0; i < kWqSlots; ++i) {
+      mbar_init(&sm.q_full[i], 32);  // 31 lanes, and the one that announces the copy
+      mbar_init(&sm.q_empty[i], 9);  // eight summing warps and the tensor cores
+    }
+    for (int t = 0; t < 2; ++t)
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&sm.s_full[t][i], 1);
+        mbar_init(&sm.s_empty[t][i], 128);
+      }
+    mbar_init(&sm.drain, 1);
+    sm.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    tw_sum<D, CAP>(sm, x, warp >> 2, tmem, w_in, w_out);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == kProducerWarp) {
+      tw_producer<D>(sm, x, &mq, &mk);
+      __syncwarp();
+    } else if (warp == kMmaWarp) {
+      tw_mma<D>(sm, x, tmem);
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) {
+        umma_commit(&sm.drain);
+        if (!mbar_wait(&sm.drain, 0)) atomicExch(&g_token_status, 1);
+      }
+      __syncwarp();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
 // Ancestor bits of a tree's nodes (row i: 256 bits) and, in row T, the drafted
 // tokens that any node sees.  One CTA per batch row, a warp per node.
 __global__ void __launch_bounds__(1024) tok_tree_bits_kernel(const uint8_t* tree, int64_t bstride, int T, uint32_t* bits) {
@@ -868,6 +1151,46 @@ int tok_tc(const char* fn, const TokArgs& a, int head_dim, void* prep, cudaStrea
     x.t.docs = nullptr;  // an empty cache: no row sees anything
   }
   return head_dim == 64 ? launch_tc_form<64>(m, x, st) : launch_tc_form<128>(m, x, st);
+}
+
+namespace {
+template <int D, bool CAP>
+int launch_tw(const CUtensorMap& mq, const CUtensorMap& mk, const TcArgs& x, const float* w_in, float* w_out,
+              cudaStream_t st) {
+  const size_t smem = sizeof(TwSmem<D>) + 1024;
+  auto kern = tok_tc_weights_kernel<D, CAP>;
+  static std::atomic<uint64_t> done{0};
+  if (first_on_device(done)) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_tc_weights_kernel: %s", cudaGetErrorString(e));
+  }
+  const int sms = device_sm_count();
+  kern<<<(unsigned)(x.units < sms ? x.units : sms), kThreads, smem, st>>>(mq, mk, x, w_in, w_out);
+  return check_launch("tok_tc_weights_kernel");
+}
+}  // namespace
+
+int tok_tc_weights(const char* fn, const TokArgs& a, int head_dim, const float* w_in, float* w_out, cudaStream_t st) {
+  const TokTcShape s = tok_tc_shape(a.Sq, a.G);
+  TcArgs x = {};
+  x.t = a;
+  x.Gp = s.Gp;
+  x.nhs = s.nhs;
+  x.P = s.P;
+  x.tiles = s.npt * s.nhs;
+  const int64_t units = (int64_t)((a.S + 2 * kTok - 1) / (2 * kTok)) * a.B * a.Hkv;
+  OC_REQUIRE(units < INT32_MAX, OC_ERR_SHAPE, "%s: too many work units", fn);
+  x.units = (int)units;
+  x.k_in = a.cap > 0.f ? a.scale / a.cap : 0.f;
+  CUtensorMap mq, mk;
+  int rc = tc_map(&mq, a.q, head_dim, a.Hq, (int64_t)a.B * a.Sq, s.Gp, s.P, fn);
+  if (!rc) rc = tc_map(&mk, a.k, head_dim, a.Hkv, (int64_t)a.B * a.S, 1, kTok, fn);
+  if (rc) return rc;
+  if (head_dim == 64)
+    return a.cap > 0.f ? launch_tw<64, true>(mq, mk, x, w_in, w_out, st)
+                       : launch_tw<64, false>(mq, mk, x, w_in, w_out, st);
+  return a.cap > 0.f ? launch_tw<128, true>(mq, mk, x, w_in, w_out, st)
+                     : launch_tw<128, false>(mq, mk, x, w_in, w_out, st);
 }
 
 int wait_limit_token(unsigned long long ns) { return set_wait_limit_here(ns); }
