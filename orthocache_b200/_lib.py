@@ -128,7 +128,7 @@ def load():
 
 def call(name, *args):
     """Call entry point ``name``; raise OrthoCacheError on a nonzero status."""
-    lib = load()
+    lib = _lib if _lib is not None else load()
     rc = getattr(lib, name)(*args)
     if rc != 0:
         msg = lib.oc_last_error().decode(errors="replace")

@@ -15,12 +15,14 @@
 //   * warp 8 loads by TMA (128-byte swizzle): the two query tiles, then K and V
 //     tiles of 128 tokens into a ring; from the cache, its pages, or the drafted
 //     tokens;
-//   * warp 9 issues the tcgen05.mma: S_t = Q_t K^T into tensor memory, O_t +=
-//     P_t V with P_t from tensor memory; per key tile j in the order PV_0(j-1),
-//     S_0(j), PV_1(j-1), S_1(j), so that one tile's softmax runs under the other
-//     tile's products.  Before a V tile with tokens that nobody may see (behind
-//     the sequence, padding) is multiplied, the warp writes zeros over them:
-//     their weights are zero, but zero times whatever memory holds may not be;
+//   * one thread of warp 9 issues the tcgen05.mma: S_t = Q_t K^T into tensor
+//     memory, O_t += P_t V with P_t from tensor memory; per key tile j in the
+//     order PV_0(j-1), S_0(j), PV_1(j-1), S_1(j), so that one tile's softmax runs
+//     under the other tile's products, and the next unit's first S under the
+//     output of the last;
+//   * V of tokens that nobody may see (behind the sequence, padding) is
+//     overwritten with zeros before the tile is multiplied: their weights are
+//     zero, but zero times whatever memory holds may not be;
 //   * warps 0-3 / 4-7 are the softmax of tile 0 / 1, a thread per row with all
 //     128 scores in registers (setmaxnreg moves registers to them from the
 //     other warps): one tensor-memory read per score.  The running maximum is
@@ -68,7 +70,7 @@ struct TcSmem {
   unsigned char kv[TcCfg<D>::kSlots][TcCfg<D>::kTileBytes];
   uint64_t kv_full[TcCfg<D>::kSlots], kv_empty[TcCfg<D>::kSlots];
   uint64_t q_full, q_empty;
-  uint64_t s_full[2], p_full[2], o_free[2];
+  uint64_t s_full[2], p_full[2], o_full[2], o_free[2];
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
@@ -92,14 +94,19 @@ struct TcUnit {
   int jt0, ncache, n;  // first cache tile, cache tiles, all tiles
 };
 
+// The k-th unit of this CTA.  Units are ordered by falling work and dealt out
+// in a snake (0 .. n-1, n-1 .. 0, ...), which evens out a linear fall.
+__device__ __forceinline__ int tc_deal(int k) {
+  return k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+
 __device__ __forceinline__ TcUnit tc_unit(const TcArgs& x, int u) {
   const TokArgs& a = x.t;
   TcUnit w;
-  const int per = x.npairs * a.nchunk;
-  w.bh = u / per;
-  const int rem = u % per;
-  const int pair = x.npairs - 1 - rem / a.nchunk;  // the rows with most keys first
-  w.chunk = rem % a.nchunk;
+  const int BH = a.B * a.Hkv;
+  w.bh = u % BH;
+  w.chunk = u / BH % a.nchunk;
+  const int pair = x.npairs - 1 - u / BH / a.nchunk;  // the rows with most keys first
   w.b = w.bh / a.Hkv;
   w.h = w.bh % a.Hkv;
   w.len = tok_len(a, w.b);
@@ -187,9 +194,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-__device__ __forceinline__ float min3(float a, float b, float c) {
+__device__ __forceinline__ float absmax3(float a, float b, float c) {
   float r;
-  asm("min.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -227,15 +234,125 @@ struct CapFn {
   }
 };
 
-template <int D, bool CAP, bool BIAS>
+// Is any of the warp's 128 x 32 scores beyond the polynomial?  (NaN: yes.)
+__device__ __forceinline__ bool cap_far(const float* s, float k_in) {
+  float top[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) top[k] = absmax3(s[k], s[4 + k], s[8 + k]);
+#pragma unroll
+  for (int i = 12; i < 124; i += 8)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top[k] = absmax3(top[k], s[i + k], s[i + 4 + k]);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) top[k] = absmax3(top[k], s[124 + k], 0.f);
+  return __any_sync(0xffffffffu, !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * k_in <= 0.6f));
+}
+
+__device__ __forceinline__ float row_max(const float* s) {
+  float m8[8];  // independent chains
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m8[k] = s[k];
+#pragma unroll
+  for (int i = 8; i < 120; i += 16)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m8[k] = max3(m8[k], s[i + k], s[i + 8 + k]);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) m8[k] = fmaxf(m8[k], s[120 + k]);
+  return fmaxf(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], max3(m8[5], m8[6], m8[7])));
+}
+
+// P = 2^(score - m) of 128 scores as bfloat16 pairs over the scores in tensor
+// memory; returns their sum.  FORM 0: scores in log2 units already; 1: raw
+// products, times c; 2: raw products, capped (m = 0).
+template <int FORM>
+__device__ __forceinline__ float exp_pack(const float* s, uint32_t t_s, float c, float m, const CapFn& cap) {
+  uint64_t r2[4] = {0, 0, 0, 0};
+  const uint64_t nm2 = pk2(-m, -m), c2 = pk2(c, c);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint32_t pk[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const uint64_t v = pk2(s[64 * half + 2 * i], s[64 * half + 2 * i + 1]);
+      const uint64_t e = FORM == 0 ? add2(v, nm2) : FORM == 1 ? fma2(v, c2, nm2) : cap.poly2(v, 0);
+      float e0, e1;
+      up2(e, e0, e1);
+      e0 = ex2(e0);
+      e1 = ex2(e1);
+      r2[i & 3] = add2(r2[i & 3], pk2(e0, e1));
+      pk[i] = pack_bf16x2(e0, e1);
+    }
+    tmem_st32u(t_s + 32 * half, pk);
+  }
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) up2(r2[i], q[2 * i], q[2 * i + 1]);
+  return ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+}
+
+// Does tile j of the unit hold tokens that no query may see?
+__device__ __forceinline__ bool tc_dirty(const TcArgs& x, const TcUnit& w, int j) {
+  const TokArgs& a = x.t;
+  if (j >= w.ncache) {
+    const uint4 seen = x.tree_bits[((size_t)w.b * (a.Sq + 1) + a.Sq) * 2 + j - w.ncache];
+    return (seen.x & seen.y & seen.z & seen.w) != ~0u;
+  }
+  const int jt = w.jt0 + j;
+  return jt * kTok + kTok > w.len || (a.table && tc_key_row(a, w.b, jt) < 0) ||
+         (a.docs && x.key_docs[(size_t)w.b * x.nkt + jt].x < 0);
+}
+
+// Zeros over the values of such tokens, by the 128 threads of the first tile's
+// softmax before they publish P of tile j (no PV of the tile is issued earlier).
+// V of the tile is load `load`; its slot's earlier loads were used up by products
+// that S(j) waited for, and the slot is not refilled before PV(j), so the parity
+// is unambiguous.
+template <int D>
+__device__ __forceinline__ bool tc_clean(TcSmem<D>& sm, const TcArgs& x, const TcUnit& w, int j, uint32_t load) {
+  using C = TcCfg<D>;
+  const TokArgs& a = x.t;
+  const uint32_t slot = load % C::kSlots;
+  if (!tc_wait_warp<D>(sm, &sm.kv_full[slot], (load / C::kSlots) & 1)) return false;
+  const int rr = threadIdx.x & 127;  // a token per thread
+  bool keep;
+  if (j >= w.ncache) {
+    const int s = (j - w.ncache) * kTok + rr;
+    const uint32_t* seen = reinterpret_cast<const uint32_t*>(x.tree_bits) + ((size_t)w.b * (a.Sq + 1) + a.Sq) * 8;
+    keep = seen[s >> 5] >> (s & 31) & 1;
+  } else {
+    const int jj = (w.jt0 + j) * kTok + rr;
+    keep = jj < w.len && !(a.table && tc_key_row(a, w.b, w.jt0 + j) < 0) &&
+           (!a.docs || a.docs[(size_t)w.b * a.S + jj] >= 0);
+  }
+  if (!keep)
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+      for (int y = 0; y < 8; ++y)
+        *reinterpret_cast<uint4*>(sm.kv[slot] + c * C::kBox + rr * 128 + y * 16) = make_uint4(0, 0, 0, 0);
+  fence_proxy_async();  // the tensor cores read through the async proxy
+  return true;
+}
+
+// CAP 0: no cap.  CAP 1 (cap <= kCapFixed, no bias): a capped score lies within
+// cap log2(e) <= 90 of zero in log2 units, so neither 2^score nor its sums leave
+// float32: the reference point of the softmax is 0 for every row, with no
+// maximum to find and nothing to rescale.  CAP 2: larger caps, or with a bias; a
+// running maximum.
+constexpr float kCapFixed = 62.f;
+
+template <int D, int CAP, bool BIAS>
 __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem) {
   const TokArgs& a = x.t;
   const int rl = threadIdx.x & 127, lane = threadIdx.x & 31;
   const uint32_t t_s = tmem + ((uint32_t)(threadIdx.x & 96) << 16) + t * 256;
   const uint32_t t_o = t_s + 128;
   const float c_scale = a.scale * kLog2e;
-  uint32_t ph = 0;
-  for (int u = blockIdx.x; u < x.units; u += gridDim.x) {
+  const CapFn cap(x);
+  uint32_t s_ph = 0, o_ph = 0, L = 0;  // L: K and V tiles loaded before this unit
+  for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
+    const int u = tc_deal(k);
+    if (u >= x.units) continue;
     const TcUnit w = tc_unit(x, u);
     if (t >= w.ntile) continue;
     const int p0 = t ? w.p0[1] : w.p0[0], min_hi = t ? w.min_hi[1] : w.min_hi[0];
@@ -245,8 +362,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
     const TokRow row = tok_row(a, w.b, w.h, real ? r : a.R, w.len);
     int4 qd = make_int4(0, 0, 0, 0);
     if (a.docs) qd = x.query_docs[(size_t)w.b * x.npt + p0 / x.P];
-    float m_used = -INFINITY, l = 0.f;
-    bool ok = true;
+    float m_used = CAP == 1 ? 0.f : -INFINITY, l = 0.f;
     for (int j = 0; j < w.n; ++j) {
       // is every key of the tile visible to every row of it?
       const bool draft = j >= w.ncache;
@@ -256,78 +372,40 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
         const int2 kd = x.key_docs[(size_t)w.b * x.nkt + jt];
         part = part || kd.x != kd.y || qd.x != kd.x || qd.y != kd.x;
       }
-      if (!tc_wait_warp<D>(sm, &sm.s_full[t], ph)) {
-        ok = false;
-        break;
-      }
-      ph ^= 1;
+      if (!tc_wait_warp<D>(sm, &sm.s_full[t], s_ph)) return;
+      s_ph ^= 1;
       tc_fence_after();
       float s[128];
       tmem_ld128_wait(t_s, s);
-      float mx;
-      bool far = false;  // a capped score beyond the polynomial
-      if (CAP) {
-        float hi8[4], lo8[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          hi8[k] = s[k];
-          lo8[k] = s[k];
-        }
-#pragma unroll
-        for (int i = 4; i < 124; i += 8)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            hi8[k] = max3(hi8[k], s[i + k], s[i + 4 + k]);
-            lo8[k] = min3(lo8[k], s[i + k], s[i + 4 + k]);
-          }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          hi8[k] = fmaxf(hi8[k], s[124 + k]);
-          lo8[k] = fminf(lo8[k], s[124 + k]);
-        }
-        mx = fmaxf(fmaxf(hi8[0], hi8[1]), fmaxf(hi8[2], hi8[3]));
-        const float mn = fminf(fminf(lo8[0], lo8[1]), fminf(lo8[2], lo8[3]));
-        far = __any_sync(0xffffffffu, !(fmaxf(mx, -mn) * x.k_in <= 0.6f));
-      } else if (!BIAS && !part) {
-        float m8[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) m8[k] = s[k];
-#pragma unroll
-        for (int i = 8; i < 120; i += 16)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) m8[k] = max3(m8[k], s[i + k], s[i + 8 + k]);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) m8[k] = fmaxf(m8[k], s[120 + k]);
-        mx = fmaxf(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], max3(m8[5], m8[6], m8[7])));
-      }
-      const CapFn cap(x);
-      const bool direct = !BIAS && !part && !far;  // the exponent straight from the products
-      if (direct) {
-        if (CAP) {
-          float y0, y1;
-          up2(cap.poly2(pk2(mx, mx), 0), y0, y1);
-          mx = y0;
-        } else {
-          mx *= c_scale;
-        }
-      } else {
+      const bool far = CAP && cap_far(s, x.k_in);
+      const bool raw = CAP != 2 && !BIAS && !part && !far;  // the exponent straight from the products
+      if (!raw) {
         // scores in log2 units, biased and masked, in place
-        if (CAP) {
-          if (far) {
+        if (CAP && far) {
 #pragma unroll
-            for (int i = 0; i < 128; ++i) s[i] = cap.exact(s[i]);
-          } else {
+          for (int i = 0; i < 128; ++i) s[i] = cap.exact(s[i]);
+        } else if (CAP) {
 #pragma unroll
-            for (int i = 0; i < 128; i += 2) up2(cap.poly2(pk2(s[i], s[i + 1]), 0), s[i], s[i + 1]);
-          }
-        } else {
+          for (int i = 0; i < 128; i += 2) up2(cap.poly2(pk2(s[i], s[i + 1]), 0), s[i], s[i + 1]);
+        } else if (!BIAS) {
 #pragma unroll
           for (int i = 0; i < 128; ++i) s[i] *= c_scale;
         }
         if (BIAS) {
+          const uint64_t c2 = CAP ? pk2(1.f, 1.f) : pk2(c_scale, c_scale);
           const float d0 = (float)(row.pos - j0);
+          if (a.causal && !a.prefix) {  // what a row sees lies behind it: |d| = d, linear along the tile
+            const uint64_t sl2 = pk2(row.slope2, row.slope2), b0 = pk2(-row.slope2 * d0, -row.slope2 * d0);
 #pragma unroll
-          for (int i = 0; i < 128; ++i) s[i] = fmaf(-row.slope2, fabsf(d0 - (float)i), s[i]);
+            for (int i = 0; i < 128; i += 2)
+              up2(fma2(pk2(s[i], s[i + 1]), c2, fma2(pk2((float)i, (float)(i + 1)), sl2, b0)), s[i], s[i + 1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 128; ++i) {
+              if (!CAP) s[i] *= c_scale;
+              s[i] = fmaf(-row.slope2, fabsf(d0 - (float)i), s[i]);
+            }
+          }
         }
         if (part) {
           if (draft) {
@@ -344,87 +422,55 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
               if (i >= lim) s[i] = -INFINITY;
             if (a.docs) {
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int jj = j0 + 32 * k + lane;
+              for (int y = 0; y < 4; ++y) {
+                const int jj = j0 + 32 * y + lane;
                 const int d = jj < a.S ? a.docs[(size_t)w.b * a.S + jj] : -1;
 #pragma unroll
                 for (int i = 0; i < 32; ++i)
-                  if (__shfl_sync(0xffffffffu, d, i) != row.doc) s[32 * k + i] = -INFINITY;
+                  if (__shfl_sync(0xffffffffu, d, i) != row.doc) s[32 * y + i] = -INFINITY;
               }
             }
           }
         }
-        float m8[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) m8[k] = s[k];
-#pragma unroll
-        for (int i = 8; i < 120; i += 16)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) m8[k] = max3(m8[k], s[i + k], s[i + 8 + k]);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) m8[k] = fmaxf(m8[k], s[120 + k]);
-        mx = fmaxf(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], max3(m8[5], m8[6], m8[7])));
       }
-      const bool need = mx > m_used + 8.f;
-      if (__any_sync(0xffffffffu, need)) {
-        const float alpha = need ? ex2(m_used - mx) : 1.f;  // 0 on a row's first visible tile
-        if (j > 0) {
+      if (CAP != 1) {
+        const float mx = raw ? row_max(s) * c_scale : row_max(s);
+        const bool need = mx > m_used + 8.f;
+        if (__any_sync(0xffffffffu, need)) {
+          const float alpha = need ? ex2(m_used - mx) : 1.f;  // 0 on a row's first visible tile
+          if (j > 0) {
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            float o[32];
-            tmem_ld32_wait(t_o + 32 * c, o);
+            for (int c = 0; c < D / 32; ++c) {
+              float o[32];
+              tmem_ld32_wait(t_o + 32 * c, o);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= alpha;
-            tmem_st32(t_o + 32 * c, o);
+              for (int i = 0; i < 32; ++i) o[i] *= alpha;
+              tmem_st32(t_o + 32 * c, o);
+            }
           }
+          l *= alpha;
+          if (need) m_used = mx;
         }
-        l *= alpha;
-        if (need) m_used = mx;
       }
       const float base = m_used == -INFINITY ? 0.f : m_used;
-      // P = 2^(s - m) as bfloat16 pairs over the scores in tensor memory
-      uint64_t r2[4] = {0, 0, 0, 0};
-      const uint64_t nm2 = pk2(-base, -base), sc2 = pk2(c_scale, c_scale);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t pk[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const uint64_t v = pk2(s[64 * half + 2 * i], s[64 * half + 2 * i + 1]);
-          uint64_t e;
-          if (!direct)
-            e = add2(v, nm2);
-          else if (CAP)
-            e = cap.poly2(v, nm2);
-          else
-            e = fma2(v, sc2, nm2);
-          float e0, e1;
-          up2(e, e0, e1);
-          e0 = ex2(e0);
-          e1 = ex2(e1);
-          r2[i & 3] = add2(r2[i & 3], pk2(e0, e1));
-          pk[i] = pack_bf16x2(e0, e1);
-        }
-        tmem_st32u(t_s + 32 * half, pk);
-      }
+      if (!raw)
+        l += exp_pack<0>(s, t_s, c_scale, base, cap);
+      else if (CAP)
+        l += exp_pack<2>(s, t_s, c_scale, base, cap);
+      else
+        l += exp_pack<1>(s, t_s, c_scale, base, cap);
+      if (t == 0 && tc_dirty(x, w, j) && !tc_clean<D>(sm, x, w, j, L + 2 * j + 1)) return;
       tc_wait_st();
-      {
-        float q[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) up2(r2[i], q[2 * i], q[2 * i + 1]);
-        l += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
-      }
       tc_fence_before();
       mbar_arrive(&sm.p_full[t]);
     }
-    if (!ok) return;
+    L += 2 * w.n;
     if (w.n > 0) {
-      // the unit's last commit covers its last PV: O is complete
-      if (!tc_wait_warp<D>(sm, &sm.s_full[t], ph)) return;
-      ph ^= 1;
+      if (!tc_wait_warp<D>(sm, &sm.o_full[t], o_ph)) return;
+      o_ph ^= 1;
       tc_fence_after();
     }
-    if (w.n == 0) m_used = -INFINITY;
+    if (l == 0.f) m_used = -INFINITY;
     const int64_t part = ((int64_t)w.bh * a.nchunk + w.chunk) * a.R + r;
     const int64_t at = tok_q_offset(a, w.b, w.h, real ? r : 0, D);
     if (real) {
@@ -467,7 +513,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
     }
     if (w.n > 0) {
       tc_fence_before();
-      mbar_arrive(&sm.o_free[t]);  // the next unit may overwrite S and O
+      mbar_arrive(&sm.o_free[t]);  // the next unit may overwrite O
     }
   }
 }
@@ -485,7 +531,9 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
       mbar_wait(&sm.kv_full[s], ((L - s - 1) / C::kSlots) & 1);
     mbar_wait(&sm.q_full, q_ph ^ 1);
   };
-  for (int u = blockIdx.x; u < x.units; u += gridDim.x) {
+  for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
+    const int u = tc_deal(k);
+    if (u >= x.units) continue;
     const TcUnit w = tc_unit(x, u);
     if (w.n == 0) continue;
     if (!tc_wait<D>(sm, &sm.q_empty, q_ph ^ 1)) return drain();
@@ -515,50 +563,17 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
   }
 }
 
-// Zero the rows of the V tile in `slot` that no query may see.
-template <int D>
-__device__ __forceinline__ void tc_clean_values(TcSmem<D>& sm, const TcArgs& x, const TcUnit& w, int j, uint32_t slot) {
-  const TokArgs& a = x.t;
-  const int lane = threadIdx.x & 31;
-  const bool draft = j >= w.ncache;
-  const int jt = draft ? j - w.ncache : w.jt0 + j, j0 = jt * kTok;
-  uint4 seen = make_uint4(~0u, ~0u, ~0u, ~0u);
-  bool bad_page = false, pads = false;
-  if (draft) {
-    seen = x.tree_bits[((size_t)w.b * (a.Sq + 1) + a.Sq) * 2 + jt];
-    if ((seen.x & seen.y & seen.z & seen.w) == ~0u) return;
-  } else {
-    bad_page = a.table && tc_key_row(a, w.b, jt) < 0;
-    pads = a.docs && x.key_docs[(size_t)w.b * x.nkt + jt].x < 0;
-    if (j0 + kTok <= w.len && !bad_page && !pads) return;
-  }
-  for (int it = 0; it < kTok / 4; ++it) {
-    const int rr = it * 4 + (lane >> 3);
-    bool keep;
-    if (draft) {
-      const uint32_t word = rr < 32 ? seen.x : rr < 64 ? seen.y : rr < 96 ? seen.z : seen.w;
-      keep = word >> (rr & 31) & 1;
-    } else {
-      keep = j0 + rr < w.len && !bad_page && (!pads || a.docs[(size_t)w.b * a.S + j0 + rr] >= 0);
-    }
-    if (!keep)
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c)
-        *reinterpret_cast<uint4*>(sm.kv[slot] + c * TcCfg<D>::kBox + rr * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-  }
-  fence_proxy_async();
-}
-
 template <int D>
 __device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
   using C = TcCfg<D>;
   constexpr uint32_t kIdQK = tc_idesc_bf16(kRows, kTok, 0), kIdPV = tc_idesc_bf16(kRows, D, 1);
-  const bool lead = (threadIdx.x & 31) == 0;
-  uint32_t q_ph = 0, p_ph = 0, o_ph = 0, L = 0;
-  for (int u = blockIdx.x; u < x.units; u += gridDim.x) {
+  uint32_t q_ph = 0, p_ph = 0, o_ph = 0, L = 0;  // phases: bit t
+  for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
+    const int u = tc_deal(k);
+    if (u >= x.units) continue;
     const TcUnit w = tc_unit(x, u);
     if (w.n == 0) continue;
-    if (!tc_wait_warp<D>(sm, &sm.q_full, q_ph)) return;
+    if (!tc_wait<D>(sm, &sm.q_full, q_ph)) return;
     q_ph ^= 1;
     tc_fence_after();
     uint32_t vslot = 0;
@@ -566,52 +581,46 @@ __device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
       uint32_t kslot = 0;
       if (j < w.n) {
         kslot = L % C::kSlots;
-        if (!tc_wait_warp<D>(sm, &sm.kv_full[kslot], (L / C::kSlots) & 1)) return;
+        if (!tc_wait<D>(sm, &sm.kv_full[kslot], (L / C::kSlots) & 1)) return;
         tc_fence_after();
       }
       if (j > 0) {  // V of tile j - 1 is load L - 1
-        if (!tc_wait_warp<D>(sm, &sm.kv_full[vslot], ((L - 1) / C::kSlots) & 1)) return;
-        tc_clean_values<D>(sm, x, w, j - 1, vslot);
-        __syncwarp();
+        if (!tc_wait<D>(sm, &sm.kv_full[vslot], ((L - 1) / C::kSlots) & 1)) return;
         tc_fence_after();
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (t >= w.ntile) break;
         const uint32_t d_s = tmem + t * 256, d_o = d_s + 128;
+        if (j == 1) {  // the softmax has read the previous unit's O_t
+          if (!tc_wait<D>(sm, &sm.o_free[t], ((o_ph >> t) & 1) ^ 1)) return;
+          o_ph ^= 1u << t;
+        }
         if (j > 0) {
-          if (!tc_wait_warp<D>(sm, &sm.p_full[t], (p_ph >> t) & 1)) return;
+          if (!tc_wait<D>(sm, &sm.p_full[t], (p_ph >> t) & 1)) return;
           p_ph ^= 1u << t;
           tc_fence_after();
-          if (lead) {
-            const uint32_t vb = smem_u32(sm.kv[vslot]);
+          const uint32_t vb = smem_u32(sm.kv[vslot]);
 #pragma unroll
-            for (int kk = 0; kk < kTok / 16; ++kk)
-              umma_bf16_ts(d_o, d_s + kk * 8, sdesc(vb + kk * 2048, C::kBox, 1024), kIdPV, (j > 1 || kk > 0) ? 1 : 0);
-            if (t == w.ntile - 1) umma_commit(&sm.kv_empty[vslot]);
-          }
+          for (int kk = 0; kk < kTok / 16; ++kk)
+            umma_bf16_ts(d_o, d_s + kk * 8, sdesc(vb + kk * 2048, C::kBox, 1024), kIdPV, (j > 1 || kk > 0) ? 1 : 0);
+          if (t == w.ntile - 1) umma_commit(&sm.kv_empty[vslot]);
         }
-        if (j == 0) {  // the softmax has read the previous unit's O_t
-          if (!tc_wait_warp<D>(sm, &sm.o_free[t], ((o_ph >> t) & 1) ^ 1)) return;
-          o_ph ^= 1u << t;
-          tc_fence_after();
-        }
-        if (lead) {
-          if (j < w.n) {
-            const uint32_t qa = smem_u32(sm.q[t]), kb = smem_u32(sm.kv[kslot]);
+        if (j < w.n) {
+          const uint32_t qa = smem_u32(sm.q[t]), kb = smem_u32(sm.kv[kslot]);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = (kk >> 2) * C::kBox + (kk & 3) * 32;
-              umma_bf16(d_s, sdesc(qa + off, 16, 1024), sdesc(kb + off, 16, 1024), kIdQK, kk > 0 ? 1 : 0);
-            }
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * C::kBox + (kk & 3) * 32;
+            umma_bf16(d_s, sdesc(qa + off, 16, 1024), sdesc(kb + off, 16, 1024), kIdQK, kk > 0 ? 1 : 0);
           }
-          umma_commit(&sm.s_full[t]);
-          if (j < w.n && t == w.ntile - 1) {
+          umma_commit(&sm.s_full[t]);  // covers PV of tile j - 1 too: O_t may be rescaled
+          if (t == w.ntile - 1) {
             umma_commit(&sm.kv_empty[kslot]);
             if (j == w.n - 1) umma_commit(&sm.q_empty);
           }
+        } else {
+          umma_commit(&sm.o_full[t]);
         }
-        __syncwarp();
       }
       if (j < w.n) {
         vslot = (L + 1) % C::kSlots;
@@ -621,7 +630,7 @@ __device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
   }
 }
 
-template <int D, bool CAP, bool BIAS>
+template <int D, int CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1)
     tok_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                   const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdk,
@@ -639,6 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sm.s_full[t], 1);
       mbar_init(&sm.p_full[t], 128);
+      mbar_init(&sm.o_full[t], 1);
       mbar_init(&sm.o_free[t], 128);
     }
     mbar_init(&sm.drain, 1);
@@ -667,9 +677,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if ((threadIdx.x & 31) == 0) tc_producer<D>(sm, x, &mq, &mk, &mv, &mdk, &mdv);
       __syncwarp();
     } else if (warp == kMmaWarp) {
-      tc_mma<D>(sm, x, tmem);
-      __syncwarp();
       if ((threadIdx.x & 31) == 0) {
+        tc_mma<D>(sm, x, tmem);
         umma_commit(&sm.drain);  // every MMA in flight, before the memory is freed
         if (!mbar_wait(&sm.drain, 0)) atomicExch(&g_token_status, 1);
       }
@@ -747,7 +756,9 @@ __device__ void tw_producer(TwSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
     for (uint32_t s = 0; s < kWqSlots && s < L; ++s) mbar_wait(&sm.q_full[s], ((L - s - 1) / kWqSlots) & 1);
     mbar_wait(&sm.k_full, k_ph ^ 1);
   };
-  for (int u = blockIdx.x; u < x.units; u += gridDim.x) {
+  for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
+    const int u = tc_deal(k);
+    if (u >= x.units) continue;
     const TwUnit w = tw_unit(x, u);
     if (w.n == 0) continue;
     if (!tw_wait<D>(sm, &sm.k_empty, k_ph ^ 1)) return drain();
@@ -789,7 +800,9 @@ __device__ void tw_mma(TwSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
   constexpr uint32_t kId = tc_idesc_bf16(kTok, kRows, 0);
   const bool lead = (threadIdx.x & 31) == 0;
   uint32_t k_ph = 0, L = 0, use[2] = {0, 0};
-  for (int u = blockIdx.x; u < x.units; u += gridDim.x) {
+  for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
+    const int u = tc_deal(k);
+    if (u >= x.units) continue;
     const TwUnit w = tw_unit(x, u);
     if (w.n == 0) continue;
     if (!tw_wait<D>(sm, &sm.k_full, k_ph)) return;
@@ -833,7 +846,9 @@ __device__ void tw_sum(TwSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem, con
   const float c_scale = a.scale * kLog2e;
   const CapFn cap(x);
   uint32_t L = 0, use = 0;
-  for (int u = blockIdx.x; u < x.units; u += gridDim.x) {
+  for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
+    const int u = tc_deal(k);
+    if (u >= x.units) continue;
     const TwUnit w = tw_unit(x, u);
     const int j = w.j0 + t * kTok + kl;
     uint64_t acc[4] = {0, 0, 0, 0};
@@ -854,15 +869,7 @@ __device__ void tw_sum(TwSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem, con
         const float4* lse = reinterpret_cast<const float4*>(sm.lse[slot]);
         // rows [lo, hi) of the tile see this thread's key
         const bool part = w.j0 + t * kTok + kTok - 1 > pos0 || p0 + x.P > a.Sq;
-        bool far = false;
-        if (CAP) {
-          float top[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int k = 0; k < 128; k += 4)
-#pragma unroll
-            for (int y = 0; y < 4; ++y) top[y] = fmaxf(top[y], fabsf(s[k + y]));
-          far = __any_sync(0xffffffffu, !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * x.k_in <= 0.6f));
-        }
+        const bool far = CAP && cap_far(s, x.k_in);
         if (!part && !far) {
           const uint64_t sc2 = pk2(c_scale, c_scale);
 #pragma unroll
@@ -1055,7 +1062,7 @@ int tc_map(CUtensorMap* m, const void* base, int D, int heads, int64_t rows, int
   return OC_OK;
 }
 
-template <int D, bool CAP, bool BIAS>
+template <int D, int CAP, bool BIAS>
 int launch_tc(const CUtensorMap (&m)[5], const TcArgs& x, cudaStream_t st) {
   const size_t smem = sizeof(TcSmem<D>) + 1024;
   auto kern = tok_tc_kernel<D, CAP, BIAS>;
@@ -1079,8 +1086,10 @@ int launch_tc(const CUtensorMap (&m)[5], const TcArgs& x, cudaStream_t st) {
 
 template <int D>
 int launch_tc_form(const CUtensorMap (&m)[5], const TcArgs& x, cudaStream_t st) {
-  if (x.t.cap > 0.f) return x.t.slopes ? launch_tc<D, true, true>(m, x, st) : launch_tc<D, true, false>(m, x, st);
-  return x.t.slopes ? launch_tc<D, false, true>(m, x, st) : launch_tc<D, false, false>(m, x, st);
+  const bool bias = x.t.slopes != nullptr;
+  if (x.t.cap > 0.f && bias) return launch_tc<D, 2, true>(m, x, st);
+  if (x.t.cap > 0.f) return x.t.cap > kCapFixed ? launch_tc<D, 2, false>(m, x, st) : launch_tc<D, 1, false>(m, x, st);
+  return bias ? launch_tc<D, 0, true>(m, x, st) : launch_tc<D, 0, false>(m, x, st);
 }
 
 }  // namespace

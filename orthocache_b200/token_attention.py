@@ -21,21 +21,49 @@ has it.  Inputs on the CPU are copied to the GPU.  Nothing waits for the GPU.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
 
-from . import _core, _lib
+from . import _lib
 from .paged import PAGE
+
+
+def _on(x, device=None, dtype=None):
+    """``_lib.as_device``, without its checks for a tensor that is already right (a decode step is a few
+    microseconds)."""
+    if (isinstance(x, torch.Tensor) and x.is_cuda and (device is None or x.device == device) and
+            (x.dtype == dtype if dtype is not None else x.dtype != torch.float64) and x.is_contiguous()):
+        return x
+    return _lib.as_device(x, device=device, dtype=dtype)
+
+
+class _Device:
+    """``torch.cuda.device`` that does nothing on the current device."""
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *args):
+        if self.guard is not None:
+            self.guard.__exit__(*args)
 
 
 def _int_rows(x, shape, device, what):
     """An int32 device tensor of ``shape`` (None stays None; a number fills it)."""
     if x is None:
         return None
+    if isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.shape == shape and x.device == device and \
+            x.is_contiguous():
+        return x
     if isinstance(x, int):
         return torch.full(shape, x, dtype=torch.int32, device=device)
-    t = _lib.as_device(x, device=device)
+    t = _on(x, device)
     if t.dtype.is_floating_point or t.dtype == torch.bool:
         raise TypeError(f"{what} must be integers, got {t.dtype}")
     if tuple(t.shape) != tuple(shape):
@@ -53,11 +81,19 @@ def _cap_scale(cap, scale, dim):
     return cap, scale
 
 
-def _workspace(q, kv_heads, seq_len, accumulate):
-    B, Sq, Hq, D = q.shape
-    n = _lib.query("oc_token_attention_workspace_bytes", _lib.dtype_code(q), B, Sq, Hq, kv_heads, D, seq_len,
-                   int(accumulate))
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device, *sizes):
+    return _lib.query("oc_token_attention_workspace_bytes", *sizes)
+
+
+def _workspace(q, dtype, kv_heads, seq_len, accumulate):
+    """Scratch of one call (what it needs depends on the sizes and the device alone)."""
+    n = _workspace_bytes(q.device, dtype, q.shape[0], q.shape[1], q.shape[2], kv_heads, q.shape[3], seq_len, accumulate)
     return torch.empty((n,), dtype=torch.uint8, device=q.device), n
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _check_heads(q, kv_heads):
@@ -83,12 +119,9 @@ def tree_attention(q, keys, values, draft_keys, draft_values, tree_mask, lengths
     cap * tanh(score / cap); ``scale`` defaults to 1 / sqrt(D).  A row that
     sees no token is zero.  Returns (B, T, Hq, D) in the cache's type.
     """
-    k = _lib.as_device(keys)
-    if k.dtype not in (torch.float32, torch.bfloat16):
-        k = k.float()
+    k, v = _cache(keys, values)
     dev, dt = k.device, k.dtype
-    v = _lib.as_device(values, device=dev, dtype=dt)
-    qq, dk, dv = (_lib.as_device(x, device=dev, dtype=dt) for x in (q, draft_keys, draft_values))
+    qq, dk, dv = _on(q, dev, dt), _on(draft_keys, dev, dt), _on(draft_values, dev, dt)
     batched = qq.dim() == 4
     if not batched:
         qq, dk, dv = qq.unsqueeze(0), dk.unsqueeze(0), dv.unsqueeze(0)
@@ -111,13 +144,13 @@ def tree_attention(q, keys, values, draft_keys, draft_values, tree_mask, lengths
     else:
         if k.shape[0] % PAGE or k.shape[0] == 0:
             raise ValueError(f"a pool of {k.shape[0]} tokens is not a whole number of {PAGE}-token pages")
-        table = _lib.as_device(block_table, device=dev)
+        table = _on(block_table, device=dev)
         if table.dim() == 1:
             table = table.unsqueeze(0)
         table = _int_rows(table, (B, table.shape[-1]), dev, "block_table")
         pages, stride = k.shape[0] // PAGE, table.shape[1]
         S = stride * PAGE
-    mask = _lib.as_device(tree_mask, device=dev)
+    mask = _on(tree_mask, device=dev)
     mask_batched = mask.dim() == 3
     if tuple(mask.shape) != ((B, T, T) if mask_batched else (T, T)):
         raise ValueError(f"tree_mask {tuple(mask.shape)}, expected ({T}, {T}) or ({B}, {T}, {T})")
@@ -125,18 +158,32 @@ def tree_attention(q, keys, values, draft_keys, draft_values, tree_mask, lengths
         raise TypeError(f"tree_mask must be bool, got {mask.dtype}")
     lens = _int_rows(lengths, (B,), dev, "lengths")
     cap, scale = _cap_scale(cap, scale, D)
-    with torch.cuda.device(dev):
-        out = torch.empty((B, T, Hq, D), dtype=dt, device=dev)
-        ws, ws_bytes = _workspace(qq, Hkv, S, False)
-        _lib.call("oc_tree_attention", _lib.ptr(qq), _lib.ptr(k), _lib.ptr(v), _lib.dtype_code(k), _lib.ptr(table),
-                  stride, pages, PAGE, _lib.ptr(lens), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(mask), int(mask_batched),
-                  B, T, Hq, Hkv, D, S, cap, scale, _lib.ptr(out), _lib.dtype_code(out), _lib.ptr(ws), ws_bytes,
+    code = _lib.dtype_code(k)
+    with _Device(dev):
+        out = torch.empty_like(qq)
+        ws, ws_bytes = _workspace(qq, code, Hkv, S, 0)
+        _lib.call("oc_tree_attention", _ptr(qq), _ptr(k), _ptr(v), code, _ptr(table),
+                  stride, pages, PAGE, _ptr(lens), _ptr(dk), _ptr(dv), _ptr(mask), int(mask_batched),
+                  B, T, Hq, Hkv, D, S, cap, scale, _ptr(out), code, _ptr(ws), ws_bytes,
                   _lib.stream_ptr(dev))
     return out if batched else out[0]
 
 
+def _cache(keys, values):
+    k = _on(keys)
+    if k.dtype not in (torch.float32, torch.bfloat16):
+        k = k.float()
+    return k, _on(values, k.device, k.dtype)
+
+
 def _chunk_inputs(q, keys, values, lengths):
-    qq, k, v, batched = _core.batched_qkv(q, keys, values)
+    k, v = _cache(keys, values)
+    qq = _on(q, k.device, k.dtype)
+    batched = k.dim() == 4
+    if not batched:
+        qq, k, v = qq.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)
+    if qq.dim() != 4 or k.dim() != 4 or k.shape != v.shape or qq.shape[0] != k.shape[0] or qq.shape[3] != k.shape[3]:
+        raise ValueError(f"incompatible shapes q {tuple(qq.shape)}, keys {tuple(k.shape)}, values {tuple(v.shape)}")
     _check_heads(qq, k.shape[2])
     return qq, k, v, batched, _int_rows(lengths, (k.shape[0],), k.device, "lengths")
 
@@ -167,19 +214,20 @@ def chunk_attention(q, keys, values, lengths=None, *, causal=True, prefix=None, 
     pre = _int_rows(prefix, (B,), dev, "prefix")
     docs = None
     if documents is not None:
-        docs = _lib.as_device(documents, device=dev)
+        docs = _on(documents, device=dev)
         docs = _int_rows(docs if batched or docs.dim() != 1 else docs.unsqueeze(0), (B, S), dev, "documents")
     sl = None
     if slopes is not None:
-        sl = _lib.as_device(slopes, device=dev, dtype=torch.float32)
+        sl = _on(slopes, device=dev, dtype=torch.float32)
         if tuple(sl.shape) != (Hq,):
             raise ValueError(f"slopes {tuple(sl.shape)}, expected ({Hq},)")
-    with torch.cuda.device(dev):
-        out = torch.empty((B, Sq, Hq, D), dtype=k.dtype, device=dev)
-        ws, ws_bytes = _workspace(qq, Hkv, S, False)
-        _lib.call("oc_chunk_attention", _lib.ptr(qq), _lib.ptr(k), _lib.ptr(v), _lib.dtype_code(k), _lib.ptr(lens),
-                  int(bool(causal)), _lib.ptr(pre), _lib.ptr(docs), _lib.ptr(sl), B, Sq, Hq, Hkv, D, S, cap, scale,
-                  _lib.ptr(out), _lib.dtype_code(out), _lib.ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+    code = _lib.dtype_code(k)
+    with _Device(dev):
+        out = torch.empty_like(qq)
+        ws, ws_bytes = _workspace(qq, code, Hkv, S, 0)
+        _lib.call("oc_chunk_attention", _ptr(qq), _ptr(k), _ptr(v), code, _ptr(lens),
+                  int(bool(causal)), _ptr(pre), _ptr(docs), _ptr(sl), B, Sq, Hq, Hkv, D, S, cap, scale,
+                  _ptr(out), code, _ptr(ws), ws_bytes, _lib.stream_ptr(dev))
     return out if batched else out[0]
 
 
@@ -200,7 +248,7 @@ def accumulate_attention(q, keys, values, weights=None, lengths=None, *, cap=0.0
     shape = (B, Hkv, S) if batched else (Hkv, S)
     w = None
     if weights is not None:
-        w = _lib.as_device(weights, device=dev, dtype=torch.float32)
+        w = _on(weights, device=dev, dtype=torch.float32)
         if tuple(w.shape) != shape:
             raise ValueError(f"weights {tuple(w.shape)}, expected {shape}")
     if out_weights is not None:
@@ -208,14 +256,15 @@ def accumulate_attention(q, keys, values, weights=None, lengths=None, *, cap=0.0
         if not (isinstance(o, torch.Tensor) and o.device == dev and o.dtype == torch.float32 and o.is_contiguous() and
                 tuple(o.shape) == shape):
             raise ValueError(f"out_weights must be a contiguous float32 tensor {shape} on {dev}")
-    with torch.cuda.device(dev):
+    code = _lib.dtype_code(k)
+    with _Device(dev):
         if out_weights is None:
             out_weights = torch.empty(shape, dtype=torch.float32, device=dev)
-        out = torch.empty((B, Sq, Hq, D), dtype=k.dtype, device=dev)
-        ws, ws_bytes = _workspace(qq, Hkv, S, True)
-        _lib.call("oc_accumulate_attention", _lib.ptr(qq), _lib.ptr(k), _lib.ptr(v), _lib.dtype_code(k),
-                  _lib.ptr(lens), _lib.ptr(w), _lib.ptr(out_weights), B, Sq, Hq, Hkv, D, S, cap, scale, _lib.ptr(out),
-                  _lib.dtype_code(out), _lib.ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+        out = torch.empty_like(qq)
+        ws, ws_bytes = _workspace(qq, code, Hkv, S, 1)
+        _lib.call("oc_accumulate_attention", _ptr(qq), _ptr(k), _ptr(v), code,
+                  _ptr(lens), _ptr(w), _ptr(out_weights), B, Sq, Hq, Hkv, D, S, cap, scale, _ptr(out),
+                  code, _ptr(ws), ws_bytes, _lib.stream_ptr(dev))
     return (out if batched else out[0]), out_weights
 
 
@@ -231,11 +280,8 @@ def evict_tokens(keys, values, weights, keep, recent=0, lengths=None):
     positions (B, Hkv, keep) int32 in ascending order, and min(n, keep) (B,)
     int32; behind the last kept token zeros and index -1.
     """
-    k = _lib.as_device(keys)
-    if k.dtype not in (torch.float32, torch.bfloat16):
-        k = k.float()
-    v = _lib.as_device(values, device=k.device, dtype=k.dtype)
-    w = _lib.as_device(weights, device=k.device, dtype=torch.float32)
+    k, v = _cache(keys, values)
+    w = _on(weights, device=k.device, dtype=torch.float32)
     batched = k.dim() == 4
     if not batched:
         k, v, w = k.unsqueeze(0), v.unsqueeze(0), w.unsqueeze(0)
@@ -248,15 +294,15 @@ def evict_tokens(keys, values, weights, keep, recent=0, lengths=None):
         raise ValueError(f"keep {keep} of {S} tokens")
     if not 0 <= recent <= keep:
         raise ValueError(f"recent {recent}, keep {keep}")
-    dev = k.device
+    dev, code = k.device, _lib.dtype_code(k)
     lens = _int_rows(lengths, (B,), dev, "lengths")
-    with torch.cuda.device(dev):
+    with _Device(dev):
         ko = torch.empty((B, keep, H, D), dtype=k.dtype, device=dev)
         vo = torch.empty_like(ko)
         wo = torch.empty((B, H, keep), dtype=torch.float32, device=dev)
         index = torch.empty((B, H, keep), dtype=torch.int32, device=dev)
         left = torch.empty((B,), dtype=torch.int32, device=dev)
-        _lib.call("oc_evict_tokens", _lib.ptr(k), _lib.ptr(v), _lib.dtype_code(k), _lib.ptr(w), _lib.ptr(lens), B, S,
-                  H, D, keep, recent, _lib.ptr(ko), _lib.ptr(vo), _lib.ptr(wo), _lib.ptr(index), _lib.ptr(left),
+        _lib.call("oc_evict_tokens", _ptr(k), _ptr(v), code, _ptr(w), _ptr(lens), B, S,
+                  H, D, keep, recent, _ptr(ko), _ptr(vo), _ptr(wo), _ptr(index), _ptr(left),
                   _lib.stream_ptr(dev))
     return (ko, vo, wo, index, left) if batched else (ko[0], vo[0], wo[0], index[0], left[0])
