@@ -15,21 +15,21 @@
 //   * warp 8 loads by TMA (128-byte swizzle): the two query tiles, then K and V
 //     tiles of 128 tokens into a ring; from the cache, its pages, or the drafted
 //     tokens;
-//   * one thread of warp 9 issues the tcgen05.mma: S_t = Q_t K^T into tensor
-//     memory, O_t += P_t V with P_t from tensor memory; per key tile j in the
-//     order PV_0(j-1), S_0(j), PV_1(j-1), S_1(j), so that one tile's softmax runs
-//     under the other tile's products, and the next unit's first S under the
-//     output of the last;
+//   * a thread of warp 17 issues the tcgen05.mma of tile 0, one of warp 18 those of
+//     tile 1: per key tile j PV_t(j-1), then S_t(j) (S_t = Q_t K^T into tensor
+//     memory, O_t += P_t V with P_t from tensor memory), so that one tile's
+//     softmax runs under the other's products, and the next unit's first S under
+//     the output of the last.  One thread for both tiles left the tensor cores
+//     idle at each of its waits (about 170 cycles apiece; period of a pair of
+//     tiles 4,300 cycles at head_dim 128 against 2,048 of products);
 //   * V of tokens that nobody may see (behind the sequence, padding) is
 //     overwritten with zeros before the tile is multiplied: their weights are
 //     zero, but zero times whatever memory holds may not be;
-//   * warps 0-3 / 4-7 are the softmax of tile 0 / 1, a thread per row with all
-//     128 scores in registers (setmaxnreg moves registers to them from the
-//     other warps): one tensor-memory read per score.  The running maximum is
-//     left stale until a row's maximum has grown by 2^8 (exact: numerator and
-//     denominator use the same one), so O is rarely rescaled.  P is rounded to
-//     bfloat16 (half a step, 2^-8 of each weight); row sums are float32, taken
-//     before the rounding.
+//   * warps 0-3 / 4-7 are the softmax of tile 0 / 1, a thread per row (setmaxnreg
+//     moves registers to them from the other warps); most tiles go through 32
+//     scores at a time: load, scale, 2^x, sum, pack.  No maximum is sought there
+//     (kRefMax below).  P is rounded to bfloat16 (half a step, 2^-8 of each
+//     weight); row sums are float32, taken before the rounding.
 //   * only key tiles that some row's limit or a document border cuts are masked
 //     element by element; tiles without a visible key are never loaded (causal
 //     limits; with documents, the span of tiles that hold a unit's documents,
@@ -55,7 +55,7 @@ namespace {
 constexpr int kRows = 128;  // rows of a tile (UMMA M)
 constexpr int kTok = 128;   // keys of a tile
 constexpr int kThreads = 384;
-constexpr int kProducerWarp = 8, kMmaWarp = 9;
+constexpr int kProducerWarp = 8, kMmaWarp = 9, kCleanWarp = 10;
 constexpr int kTmemCols = 512;
 
 template <int D> struct TcCfg {
@@ -70,6 +70,7 @@ struct TcSmem {
   unsigned char kv[TcCfg<D>::kSlots][TcCfg<D>::kTileBytes];
   uint64_t kv_full[TcCfg<D>::kSlots], kv_empty[TcCfg<D>::kSlots];
   uint64_t q_full, q_empty;
+  uint64_t v_clean[TcCfg<D>::kSlots];
   uint64_t s_full[2], p_full[2], o_full[2], o_free[2];
   uint64_t drain;
   uint32_t tmem_base;
@@ -154,16 +155,30 @@ __device__ __forceinline__ TcUnit tc_unit(const TcArgs& x, int u) {
 // First key row of cache tile jt in the (rows, Hkv, D) view; -1: no such page.
 __device__ __forceinline__ int tc_key_row(const TokArgs& a, int b, int jt) { return (int)tok_kv_row(a, b, jt * kTok); }
 
-template <int D>
-__device__ __forceinline__ bool tc_wait(TcSmem<D>& sm, uint64_t* bar, uint32_t parity) {
-  if (*(volatile int*)&sm.abort == 0 && mbar_wait(bar, parity)) return true;
-  if (atomicExch(&sm.abort, 1) == 0) atomicExch(&g_token_status, 1);
-  return false;
+// Bounded wait.  The hardware suspends a failed try for a while by itself, so the
+// clock is read, and the abort flag of a role that gave up looked at, only every
+// 32 tries: a timer read costs as much as several hand-overs.
+__device__ __forceinline__ bool bar_wait(int* abort, uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  uint64_t t0 = 0;
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*(volatile int*)abort != 0) return false;
+    const uint64_t now = globaltimer_ns();
+    if (t0 == 0) {
+      t0 = now;
+    } else if (now - t0 > g_wait_limit_ns) {
+      atomicExch(abort, 1);
+      atomicExch(&g_token_status, 1);
+      return false;
+    }
+  }
 }
 // The same for a whole warp, with one answer for all its lanes.
-template <int D>
-__device__ __forceinline__ bool tc_wait_warp(TcSmem<D>& sm, uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, tc_wait<D>(sm, bar, parity));
+__device__ __forceinline__ bool bar_wait_warp(int* abort, uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, bar_wait(abort, bar, parity));
 }
 
 __device__ __forceinline__ uint64_t pk2(float a, float b) {
@@ -206,46 +221,59 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // The cap in log2 units: cap' tanh(k s) with cap' = cap log2(e), k = scale / cap.
+// tanh(z) / z by least-squares polynomials in z^2 with equalised error of tanh:
+// degree 2 for |z| <= 0.3 (1.7e-7), degree 3 for |z| <= 0.5 (1.3e-7); beyond, 1 - 2
+// / (1 + e^(2 z)).
+constexpr float kCapPoly2 = 0.3f, kCapPoly3 = 0.5f;
 struct CapFn {
-  float k, cap2;             // k_in, cap * log2(e)
-  float a0, a1, a2, a3, a4;  // the polynomial's coefficients in s^2, times cap' k
+  float k, cap2;         // k_in, cap * log2(e)
+  float b0, b1, b2;      // degree 2 in s^2, times cap' k
+  float a0, a1, a2, a3;  // degree 3
   __device__ __forceinline__ CapFn(const TcArgs& x) {
     k = x.k_in;
     cap2 = x.t.cap * kLog2e;
     const float k2 = k * k, c = cap2 * k;
-    a0 = c * 0.9999996423721313f;
-    a1 = c * k2 * -0.33331209421157837f;
-    a2 = c * k2 * k2 * 0.13299210369586945f;
-    a3 = c * k2 * k2 * k2 * -0.051696740090847015f;
-    a4 = c * k2 * k2 * k2 * k2 * 0.014976956881582737f;
+    b0 = c * 0.9999960064888f;
+    b1 = c * k2 * -0.33297479152679443f;
+    b2 = c * k2 * k2 * 0.12522591650485992f;
+    a0 = c * 0.9999976754188538f;
+    a1 = c * k2 * -0.33320656418800354f;
+    a2 = c * k2 * k2 * 0.13145145773887634f;
+    a3 = c * k2 * k2 * k2 * -0.04337248206138611f;
   }
   __device__ __forceinline__ float exact(float s) const {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(2.f * kLog2e * k * s)));
     return fmaf(-2.f * cap2, r, cap2);
   }
+  template <int DEG>
   __device__ __forceinline__ uint64_t poly2(uint64_t s, uint64_t off) const {  // cap' tanh(k s) + off
     const uint64_t u = mul2(s, s);
-    uint64_t p = fma2(pk2(a4, a4), u, pk2(a3, a3));
-    p = fma2(p, u, pk2(a2, a2));
-    p = fma2(p, u, pk2(a1, a1));
-    p = fma2(p, u, pk2(a0, a0));
+    uint64_t p;
+    if (DEG == 2) {
+      p = fma2(pk2(b2, b2), u, pk2(b1, b1));
+      p = fma2(p, u, pk2(b0, b0));
+    } else {
+      p = fma2(pk2(a3, a3), u, pk2(a2, a2));
+      p = fma2(p, u, pk2(a1, a1));
+      p = fma2(p, u, pk2(a0, a0));
+    }
     return fma2(p, s, off);
   }
 };
 
-// Is any of the warp's 128 x 32 scores beyond the polynomial?  (NaN: yes.)
+// Is any of the warp's 32 x N scores beyond the polynomial?  (NaN may pass: it
+// stays NaN in the polynomial.)
+template <int N>
 __device__ __forceinline__ bool cap_far(const float* s, float k_in) {
   float top[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) top[k] = absmax3(s[k], s[4 + k], s[8 + k]);
+  for (int k = 0; k < 4; ++k) top[k] = absmax3(s[k], s[4 + k], 0.f);
 #pragma unroll
-  for (int i = 12; i < 124; i += 8)
+  for (int i = 8; i < N; i += 8)
 #pragma unroll
     for (int k = 0; k < 4; ++k) top[k] = absmax3(top[k], s[i + k], s[i + 4 + k]);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) top[k] = absmax3(top[k], s[124 + k], 0.f);
-  return __any_sync(0xffffffffu, !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * k_in <= 0.6f));
+  return __any_sync(0xffffffffu, !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * k_in <= kCapPoly3));
 }
 
 __device__ __forceinline__ float row_max(const float* s) {
@@ -261,22 +289,46 @@ __device__ __forceinline__ float row_max(const float* s) {
   return fmaxf(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], max3(m8[5], m8[6], m8[7])));
 }
 
-// P = 2^(score - m) of 128 scores as bfloat16 pairs over the scores in tensor
-// memory; returns their sum.  FORM 0: scores in log2 units already; 1: raw
-// products, times c; 2: raw products, capped (m = 0).
-template <int FORM>
-__device__ __forceinline__ float exp_pack(const float* s, uint32_t t_s, float c, float m, const CapFn& cap) {
+// 2^x of a pair on the FMA pipe, for x >= -126 or clamped there: x = n + f, n =
+// floor(x) by adding 1.5 * 2^23 with rounding toward -inf (its low bits are then
+// n), 2^f on [0, 1) a least-squares polynomial of degree 4 with equalised
+// relative error (2.6e-6), times 2^n built in the exponent field.  NaN stays NaN.
+template <bool CLAMP>
+__device__ __forceinline__ uint64_t poly_ex2(uint64_t x) {
+  if (CLAMP) {
+    float a, b;
+    up2(x, a, b);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+    x = pk2(a, b);
+  }
+  uint64_t t, n, f;
+  const uint64_t magic = pk2(12582912.f, 12582912.f);
+  asm("add.rm.f32x2 %0, %1, %2;" : "=l"(t) : "l"(x), "l"(magic));
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(n) : "l"(t), "l"(magic));
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(f) : "l"(x), "l"(n));
+  uint64_t p = fma2(pk2(0.013534166850149632f, 0.013534166850149632f), f, pk2(0.052011460065841675f, 0.052011460065841675f));
+  p = fma2(p, f, pk2(0.2414427548646927f, 0.2414427548646927f));
+  p = fma2(p, f, pk2(0.6930038332939148f, 0.6930038332939148f));
+  p = fma2(p, f, pk2(1.0000026226043701f, 1.0000026226043701f));
+  float t0, t1;
+  up2(t, t0, t1);
+  return mul2(p, pk2(__uint_as_float(__float_as_uint(t0) * (1u << 23) + 0x3f800000u),
+                     __uint_as_float(__float_as_uint(t1) * (1u << 23) + 0x3f800000u)));
+}
+
+// P = 2^(score - m) of 128 masked scores in log2 units as bfloat16 pairs over the
+// scores in tensor memory; returns their sum.
+__device__ __forceinline__ float exp_pack(const float* s, uint32_t t_s, float m) {
   uint64_t r2[4] = {0, 0, 0, 0};
-  const uint64_t nm2 = pk2(-m, -m), c2 = pk2(c, c);
+  const uint64_t nm2 = pk2(-m, -m);
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     uint32_t pk[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const uint64_t v = pk2(s[64 * half + 2 * i], s[64 * half + 2 * i + 1]);
-      const uint64_t e = FORM == 0 ? add2(v, nm2) : FORM == 1 ? fma2(v, c2, nm2) : cap.poly2(v, 0);
       float e0, e1;
-      up2(e, e0, e1);
+      up2(add2(pk2(s[64 * half + 2 * i], s[64 * half + 2 * i + 1]), nm2), e0, e1);
       e0 = ex2(e0);
       e1 = ex2(e1);
       r2[i & 3] = add2(r2[i & 3], pk2(e0, e1));
@@ -288,6 +340,35 @@ __device__ __forceinline__ float exp_pack(const float* s, uint32_t t_s, float c,
 #pragma unroll
   for (int i = 0; i < 4; ++i) up2(r2[i], q[2 * i], q[2 * i + 1]);
   return ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+}
+
+// 2^(score - m) of 32 scores (columns 32 c ..) as bfloat16 pairs, and their sums;
+// At head_dim 64 an eighth of the exponentials run on the FMA pipe (the products
+// are half as long there; a 2048-token chunk on 32K: 884 -> 795 us; at 128, and
+// with a cap's polynomial on that pipe already, it costs 0.3 to 8 %).
+// DEG > 0: capped by the polynomial of that degree, with the largest |product| in
+// top.
+template <int D, int DEG, bool BIAS>
+__device__ __forceinline__ void chunk_exp(const float* s, int c, uint32_t* pk, uint64_t (&r2)[4], float& top,
+                                          float c_scale, uint64_t nm2, uint64_t sl2, float b0, const CapFn& cap) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint64_t v = pk2(s[2 * i], s[2 * i + 1]);
+    uint64_t off = nm2;
+    if (BIAS) off = fma2(pk2((float)(32 * c + 2 * i), (float)(32 * c + 2 * i + 1)), sl2, pk2(b0, b0));
+    if (DEG) top = absmax3(top, s[2 * i], s[2 * i + 1]);
+    const uint64_t e = DEG ? cap.poly2<DEG ? DEG : 2>(v, off) : fma2(v, pk2(c_scale, c_scale), off);
+    float e0, e1;
+    if (D == 64 && !DEG && i % 8 == 0) {
+      up2(poly_ex2<true>(e), e0, e1);
+    } else {
+      up2(e, e0, e1);
+      e0 = ex2(e0);
+      e1 = ex2(e1);
+    }
+    r2[i & 3] = add2(r2[i & 3], pk2(e0, e1));
+    pk[16 * c + i] = pack_bf16x2(e0, e1);
+  }
 }
 
 // Does tile j of the unit hold tokens that no query may see?
@@ -302,44 +383,19 @@ __device__ __forceinline__ bool tc_dirty(const TcArgs& x, const TcUnit& w, int j
          (a.docs && x.key_docs[(size_t)w.b * x.nkt + jt].x < 0);
 }
 
-// Zeros over the values of such tokens, by the 128 threads of the first tile's
-// softmax before they publish P of tile j (no PV of the tile is issued earlier).
-// V of the tile is load `load`; its slot's earlier loads were used up by products
-// that S(j) waited for, and the slot is not refilled before PV(j), so the parity
-// is unambiguous.
-template <int D>
-__device__ __forceinline__ bool tc_clean(TcSmem<D>& sm, const TcArgs& x, const TcUnit& w, int j, uint32_t load) {
-  using C = TcCfg<D>;
-  const TokArgs& a = x.t;
-  const uint32_t slot = load % C::kSlots;
-  if (!tc_wait_warp<D>(sm, &sm.kv_full[slot], (load / C::kSlots) & 1)) return false;
-  const int rr = threadIdx.x & 127;  // a token per thread
-  bool keep;
-  if (j >= w.ncache) {
-    const int s = (j - w.ncache) * kTok + rr;
-    const uint32_t* seen = reinterpret_cast<const uint32_t*>(x.tree_bits) + ((size_t)w.b * (a.Sq + 1) + a.Sq) * 8;
-    keep = seen[s >> 5] >> (s & 31) & 1;
-  } else {
-    const int jj = (w.jt0 + j) * kTok + rr;
-    keep = jj < w.len && !(a.table && tc_key_row(a, w.b, w.jt0 + j) < 0) &&
-           (!a.docs || a.docs[(size_t)w.b * a.S + jj] >= 0);
-  }
-  if (!keep)
-#pragma unroll
-    for (int c = 0; c < D / 64; ++c)
-#pragma unroll
-      for (int y = 0; y < 8; ++y)
-        *reinterpret_cast<uint4*>(sm.kv[slot] + c * C::kBox + rr * 128 + y * 16) = make_uint4(0, 0, 0, 0);
-  fence_proxy_async();  // the tensor cores read through the async proxy
-  return true;
-}
-
 // CAP 0: no cap.  CAP 1 (cap <= kCapFixed, no bias): a capped score lies within
 // cap log2(e) <= 90 of zero in log2 units, so neither 2^score nor its sums leave
 // float32: the reference point of the softmax is 0 for every row, with no
 // maximum to find and nothing to rescale.  CAP 2: larger caps, or with a bias; a
 // running maximum.
 constexpr float kCapFixed = 62.f;
+
+// The reference point m of a row's softmax is exact whatever it is, as long as
+// 2^(score - m) and its sums stay in range, and bfloat16 has the range of
+// float32.  So a row takes the maximum of its first visible tile, and the tiles
+// after it are exponentiated without looking for one; a tile whose sum comes to
+// kRefMax or more is done over, with the rescaling.
+constexpr float kRefMax = 1.152921504606846976e18f;  // 2^60
 
 template <int D, int CAP, bool BIAS>
 __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem) {
@@ -349,7 +405,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
   const uint32_t t_o = t_s + 128;
   const float c_scale = a.scale * kLog2e;
   const CapFn cap(x);
-  uint32_t s_ph = 0, o_ph = 0, L = 0;  // L: K and V tiles loaded before this unit
+  uint32_t s_ph = 0, o_ph = 0;
   for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
     const int u = tc_deal(k);
     if (u >= x.units) continue;
@@ -362,7 +418,8 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
     const TokRow row = tok_row(a, w.b, w.h, real ? r : a.R, w.len);
     int4 qd = make_int4(0, 0, 0, 0);
     if (a.docs) qd = x.query_docs[(size_t)w.b * x.npt + p0 / x.P];
-    float m_used = CAP == 1 ? 0.f : -INFINITY, l = 0.f;
+    float m_used = CAP == 1 || !real ? 0.f : -INFINITY, l = 0.f;
+    int level = 0;  // which of the cap's polynomials is in use
     for (int j = 0; j < w.n; ++j) {
       // is every key of the tile visible to every row of it?
       const bool draft = j >= w.ncache;
@@ -370,42 +427,66 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
       bool part = draft || j0 + kTok > min_hi || (a.table && tc_key_row(a, w.b, jt) < 0);
       if (a.docs && !draft) {
         const int2 kd = x.key_docs[(size_t)w.b * x.nkt + jt];
-        part = part || kd.x != kd.y || qd.x != kd.x || qd.y != kd.x;
+        part = part || kd.x < 0 || kd.x != kd.y || qd.x != kd.x || qd.y != kd.x;
       }
-      if (!tc_wait_warp<D>(sm, &sm.s_full[t], s_ph)) return;
+      if (!bar_wait_warp(&sm.abort, &sm.s_full[t], s_ph)) return;
       s_ph ^= 1;
       tc_fence_after();
-      float s[128];
-      tmem_ld128_wait(t_s, s);
-      const bool far = CAP && cap_far(s, x.k_in);
-      const bool raw = CAP != 2 && !BIAS && !part && !far;  // the exponent straight from the products
-      if (!raw) {
+      // Fast: every key visible, every row with a reference point.
+      bool done = false;
+      const float d0 = (float)(row.pos - j0);
+      const bool behind = !BIAS || (a.causal && !a.prefix);
+      if (!part && behind && level < 2 && !__any_sync(0xffffffffu, m_used == -INFINITY)) {
+        uint32_t pk[64];
+        const uint64_t nm2 = pk2(-m_used, -m_used);
+        const uint64_t sl2 = pk2(row.slope2, row.slope2);
+        // |d| = d behind the query: bias and reference point are linear along the tile
+        const float b0 = fmaf(-row.slope2, d0, -m_used);
+        uint64_t r2[4] = {0, 0, 0, 0};
+        float s[128], top = 0.f;
+        tmem_ld128_wait(t_s, s);
+        if (!CAP || level == 0) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            chunk_exp<D, CAP ? 2 : 0, BIAS>(s + 32 * c, c, pk, r2, top, c_scale, nm2, sl2, b0, cap);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) chunk_exp<D, 3, BIAS>(s + 32 * c, c, pk, r2, top, c_scale, nm2, sl2, b0, cap);
+        }
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) up2(r2[i], q[2 * i], q[2 * i + 1]);
+        const float sum = ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+        // a score beyond the polynomial, or a sum that has grown too large?
+        const bool far = CAP && __any_sync(0xffffffffu, !(top * x.k_in <= (level ? kCapPoly3 : kCapPoly2)));
+        if (far) ++level;  // for the rest of the unit; 2: not this way
+        const bool over = far || (CAP != 1 && real && !(sum < kRefMax));
+        if (!__any_sync(0xffffffffu, over)) {
+          tmem_st32u(t_s, pk);
+          tmem_st32u(t_s + 32, pk + 32);
+          l += sum;
+          done = true;
+        }
+      }
+      if (!done) {
+        float s[128];
+        tmem_ld128_wait(t_s, s);
         // scores in log2 units, biased and masked, in place
-        if (CAP && far) {
+        if (CAP) {
+          if (cap_far<128>(s, x.k_in)) {
 #pragma unroll
-          for (int i = 0; i < 128; ++i) s[i] = cap.exact(s[i]);
-        } else if (CAP) {
+            for (int i = 0; i < 128; ++i) s[i] = cap.exact(s[i]);
+          } else {
 #pragma unroll
-          for (int i = 0; i < 128; i += 2) up2(cap.poly2(pk2(s[i], s[i + 1]), 0), s[i], s[i + 1]);
-        } else if (!BIAS) {
+            for (int i = 0; i < 128; i += 2) up2(cap.poly2<3>(pk2(s[i], s[i + 1]), 0), s[i], s[i + 1]);
+          }
+        } else {
 #pragma unroll
           for (int i = 0; i < 128; ++i) s[i] *= c_scale;
         }
         if (BIAS) {
-          const uint64_t c2 = CAP ? pk2(1.f, 1.f) : pk2(c_scale, c_scale);
-          const float d0 = (float)(row.pos - j0);
-          if (a.causal && !a.prefix) {  // what a row sees lies behind it: |d| = d, linear along the tile
-            const uint64_t sl2 = pk2(row.slope2, row.slope2), b0 = pk2(-row.slope2 * d0, -row.slope2 * d0);
 #pragma unroll
-            for (int i = 0; i < 128; i += 2)
-              up2(fma2(pk2(s[i], s[i + 1]), c2, fma2(pk2((float)i, (float)(i + 1)), sl2, b0)), s[i], s[i + 1]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 128; ++i) {
-              if (!CAP) s[i] *= c_scale;
-              s[i] = fmaf(-row.slope2, fabsf(d0 - (float)i), s[i]);
-            }
-          }
+          for (int i = 0; i < 128; ++i) s[i] = fmaf(-row.slope2, fabsf(d0 - (float)i), s[i]);
         }
         if (part) {
           if (draft) {
@@ -432,41 +513,34 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
             }
           }
         }
-      }
-      if (CAP != 1) {
-        const float mx = raw ? row_max(s) * c_scale : row_max(s);
-        const bool need = mx > m_used + 8.f;
-        if (__any_sync(0xffffffffu, need)) {
-          const float alpha = need ? ex2(m_used - mx) : 1.f;  // 0 on a row's first visible tile
-          if (j > 0) {
+        if (CAP != 1) {
+          const float mx = row_max(s);
+          const bool need = mx > m_used + 8.f;
+          if (__any_sync(0xffffffffu, need)) {
+            const float alpha = need ? ex2(m_used - mx) : 1.f;  // 0 on a row's first visible tile
+            if (j > 0) {
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              float o[32];
-              tmem_ld32_wait(t_o + 32 * c, o);
+              for (int c = 0; c < D / 32; ++c) {
+                float o[32];
+                tmem_ld32_wait(t_o + 32 * c, o);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] *= alpha;
-              tmem_st32(t_o + 32 * c, o);
+                for (int i = 0; i < 32; ++i) o[i] *= alpha;
+                tmem_st32(t_o + 32 * c, o);
+              }
             }
+            l *= alpha;
+            if (need) m_used = mx;
           }
-          l *= alpha;
-          if (need) m_used = mx;
         }
+        l += exp_pack(s, t_s, m_used == -INFINITY ? 0.f : m_used);
       }
-      const float base = m_used == -INFINITY ? 0.f : m_used;
-      if (!raw)
-        l += exp_pack<0>(s, t_s, c_scale, base, cap);
-      else if (CAP)
-        l += exp_pack<2>(s, t_s, c_scale, base, cap);
-      else
-        l += exp_pack<1>(s, t_s, c_scale, base, cap);
-      if (t == 0 && tc_dirty(x, w, j) && !tc_clean<D>(sm, x, w, j, L + 2 * j + 1)) return;
       tc_wait_st();
       tc_fence_before();
-      mbar_arrive(&sm.p_full[t]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.p_full[t]);
     }
-    L += 2 * w.n;
     if (w.n > 0) {
-      if (!tc_wait_warp<D>(sm, &sm.o_full[t], o_ph)) return;
+      if (!bar_wait_warp(&sm.abort, &sm.o_full[t], o_ph)) return;
       o_ph ^= 1;
       tc_fence_after();
     }
@@ -513,7 +587,8 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
     }
     if (w.n > 0) {
       tc_fence_before();
-      mbar_arrive(&sm.o_free[t]);  // the next unit may overwrite O
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.o_free[t]);  // the next unit may overwrite O
     }
   }
 }
@@ -536,7 +611,7 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
     if (u >= x.units) continue;
     const TcUnit w = tc_unit(x, u);
     if (w.n == 0) continue;
-    if (!tc_wait<D>(sm, &sm.q_empty, q_ph ^ 1)) return drain();
+    if (!bar_wait(&sm.abort, &sm.q_empty, q_ph ^ 1)) return drain();
     q_ph ^= 1;
     mbar_expect_tx(&sm.q_full, (uint32_t)(w.ntile * C::kTileBytes));
 #pragma unroll
@@ -552,7 +627,7 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv, ++L) {
         const uint32_t slot = L % C::kSlots;
-        if (!tc_wait<D>(sm, &sm.kv_empty[slot], ((L / C::kSlots) & 1) ^ 1)) return drain();
+        if (!bar_wait(&sm.abort, &sm.kv_empty[slot], ((L / C::kSlots) & 1) ^ 1)) return drain();
         mbar_expect_tx(&sm.kv_full[slot], C::kTileBytes);
         const CUtensorMap* m = kv ? (draft ? mdv : mv) : (draft ? mdk : mk);
 #pragma unroll
@@ -563,68 +638,158 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
   }
 }
 
+// Zeros over the values of tokens that nobody may see, before the tensor cores
+// read the tile.  The warp looks at every load in order and takes part in the
+// release of its slot, so that it neither lags nor runs ahead of the ring.
 template <int D>
-__device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
+__device__ void tc_cleaner(TcSmem<D>& sm, const TcArgs& x) {
   using C = TcCfg<D>;
-  constexpr uint32_t kIdQK = tc_idesc_bf16(kRows, kTok, 0), kIdPV = tc_idesc_bf16(kRows, D, 1);
-  uint32_t q_ph = 0, p_ph = 0, o_ph = 0, L = 0;  // phases: bit t
+  const TokArgs& a = x.t;
+  const int lane = threadIdx.x & 31;
+  uint32_t L = 0;
   for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
     const int u = tc_deal(k);
     if (u >= x.units) continue;
     const TcUnit w = tc_unit(x, u);
-    if (w.n == 0) continue;
-    if (!tc_wait<D>(sm, &sm.q_full, q_ph)) return;
+    for (int j = 0; j < w.n; ++j, L += 2) {
+      const uint32_t kslot = L % C::kSlots, slot = (L + 1) % C::kSlots;
+      if (!bar_wait_warp(&sm.abort, &sm.kv_full[kslot], (L / C::kSlots) & 1)) return;
+      if (lane == 0) mbar_arrive(&sm.kv_empty[kslot]);
+      if (!bar_wait_warp(&sm.abort, &sm.kv_full[slot], ((L + 1) / C::kSlots) & 1)) return;
+      if (tc_dirty(x, w, j)) {
+        const bool draft = j >= w.ncache;
+        const int jt = draft ? j - w.ncache : w.jt0 + j, j0 = jt * kTok;
+        const uint32_t* seen = reinterpret_cast<const uint32_t*>(x.tree_bits) + ((size_t)w.b * (a.Sq + 1) + a.Sq) * 8;
+        const bool no_page = !draft && a.table && tc_key_row(a, w.b, jt) < 0;
+        for (int it = 0; it < kTok / 4; ++it) {
+          const int rr = it * 4 + (lane >> 3), jj = j0 + rr;
+          const bool keep = draft ? (seen[jj >> 5] >> (jj & 31) & 1) != 0
+                                  : jj < w.len && !no_page && (!a.docs || a.docs[(size_t)w.b * a.S + jj] >= 0);
+          if (!keep)
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              *reinterpret_cast<uint4*>(sm.kv[slot] + c * C::kBox + rr * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async();  // the tensor cores read through the async proxy
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.v_clean[slot]);
+      }
+      if (lane == 0) mbar_arrive(&sm.kv_empty[slot]);
+    }
+  }
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// A place in the K / V ring.
+template <int D>
+struct RingPos {
+  uint32_t slot = 0, ph = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == TcCfg<D>::kSlots) {
+      slot = 0;
+      ph ^= 1;
+    }
+  }
+};
+
+// The issuing warp.  All its lanes run the loop, so that the compiler keeps the
+// operands of the products in uniform registers; one elected lane issues.  Every
+// instruction here delays the tensor cores (the warp shares its scheduler with
+// four that keep it busy), so the loop does what it can before the tile's P is
+// awaited.
+template <int D>
+__device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
+  using C = TcCfg<D>;
+  constexpr uint32_t kIdQK = tc_idesc_bf16(kRows, kTok, 0), kIdPV = tc_idesc_bf16(kRows, D, 1);
+  const uint64_t qd0 = sdesc(__shfl_sync(0xffffffffu, smem_u32(sm.q[0]), 0), 16, 1024);
+  const uint64_t kd0 = sdesc(__shfl_sync(0xffffffffu, smem_u32(sm.kv[0]), 0), 16, 1024);
+  const uint64_t vd0 = sdesc(__shfl_sync(0xffffffffu, smem_u32(sm.kv[0]), 0), C::kBox, 1024);
+  tmem = __shfl_sync(0xffffffffu, tmem, 0);
+  uint32_t q_ph = 0, p_ph[2] = {0, 0}, o_ph[2] = {1, 1}, clean_ph = 0;  // clean_ph: a bit per slot
+  RingPos<D> kp;
+  for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
+    const int u = tc_deal(k);
+    if (u >= x.units) continue;
+    const TcUnit w = tc_unit(x, u);
+    const int n = __shfl_sync(0xffffffffu, w.n, 0), ntile = __shfl_sync(0xffffffffu, w.ntile, 0);
+    if (n == 0) continue;
+    // first tile that may hold tokens nobody sees
+    const int dirty0 = x.t.docs || x.t.table || x.t.dk ? 0 : w.len / kTok - w.jt0;
+    if (!bar_wait_warp(&sm.abort, &sm.q_full, q_ph)) return;
     q_ph ^= 1;
+    if (!bar_wait_warp(&sm.abort, &sm.kv_full[kp.slot], kp.ph)) return;
     tc_fence_after();
-    uint32_t vslot = 0;
-    for (int j = 0; j <= w.n; ++j) {
-      uint32_t kslot = 0;
-      if (j < w.n) {
-        kslot = L % C::kSlots;
-        if (!tc_wait<D>(sm, &sm.kv_full[kslot], (L / C::kSlots) & 1)) return;
-        tc_fence_after();
+    // S of the first key tile
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (t < ntile && elect_one()) {
+        const uint64_t kd = kd0 + kp.slot * (C::kTileBytes >> 4);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * C::kBox + (kk & 3) * 32) >> 4;
+          umma_bf16(tmem + t * 256, qd0 + t * (C::kTileBytes >> 4) + off, kd + off, kIdQK, kk > 0 ? 1 : 0);
+        }
+        umma_commit(&sm.s_full[t]);
+        if (t == ntile - 1) {
+          umma_commit(&sm.kv_empty[kp.slot]);
+          if (n == 1) umma_commit(&sm.q_empty);
+        }
       }
-      if (j > 0) {  // V of tile j - 1 is load L - 1
-        if (!tc_wait<D>(sm, &sm.kv_full[vslot], ((L - 1) / C::kSlots) & 1)) return;
-        tc_fence_after();
+      __syncwarp();
+    }
+    for (int j = 1; j <= n; ++j) {
+      RingPos<D> vp = kp;
+      vp.next();  // V of tile j - 1; K of tile j after it
+      kp = vp;
+      kp.next();
+      const uint64_t vd = vd0 + vp.slot * (C::kTileBytes >> 4), kd = kd0 + kp.slot * (C::kTileBytes >> 4);
+      if (!bar_wait_warp(&sm.abort, &sm.kv_full[vp.slot], vp.ph)) return;
+      if (j > dirty0 && tc_dirty(x, w, j - 1)) {
+        if (!bar_wait_warp(&sm.abort, &sm.v_clean[vp.slot], (clean_ph >> vp.slot) & 1)) return;
+        clean_ph ^= 1u << vp.slot;
       }
+      if (j < n && !bar_wait_warp(&sm.abort, &sm.kv_full[kp.slot], kp.ph)) return;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        if (t >= w.ntile) break;
+        if (t >= ntile) break;
         const uint32_t d_s = tmem + t * 256, d_o = d_s + 128;
         if (j == 1) {  // the softmax has read the previous unit's O_t
-          if (!tc_wait<D>(sm, &sm.o_free[t], ((o_ph >> t) & 1) ^ 1)) return;
-          o_ph ^= 1u << t;
+          if (!bar_wait_warp(&sm.abort, &sm.o_free[t], o_ph[t])) return;
+          o_ph[t] ^= 1;
         }
-        if (j > 0) {
-          if (!tc_wait<D>(sm, &sm.p_full[t], (p_ph >> t) & 1)) return;
-          p_ph ^= 1u << t;
-          tc_fence_after();
-          const uint32_t vb = smem_u32(sm.kv[vslot]);
+        if (!bar_wait_warp(&sm.abort, &sm.p_full[t], p_ph[t])) return;
+        p_ph[t] ^= 1;
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kTok / 16; ++kk)
-            umma_bf16_ts(d_o, d_s + kk * 8, sdesc(vb + kk * 2048, C::kBox, 1024), kIdPV, (j > 1 || kk > 0) ? 1 : 0);
-          if (t == w.ntile - 1) umma_commit(&sm.kv_empty[vslot]);
-        }
-        if (j < w.n) {
-          const uint32_t qa = smem_u32(sm.q[t]), kb = smem_u32(sm.kv[kslot]);
+            umma_bf16_ts(d_o, d_s + kk * 8, vd + kk * 128, kIdPV, (j > 1 || kk > 0) ? 1 : 0);
+          if (j < n) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * C::kBox + (kk & 3) * 32;
-            umma_bf16(d_s, sdesc(qa + off, 16, 1024), sdesc(kb + off, 16, 1024), kIdQK, kk > 0 ? 1 : 0);
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = ((kk >> 2) * C::kBox + (kk & 3) * 32) >> 4;
+              umma_bf16(d_s, qd0 + t * (C::kTileBytes >> 4) + off, kd + off, kIdQK, kk > 0 ? 1 : 0);
+            }
+            umma_commit(&sm.s_full[t]);  // covers PV of tile j - 1 too: O_t may be rescaled
+          } else {
+            umma_commit(&sm.o_full[t]);
           }
-          umma_commit(&sm.s_full[t]);  // covers PV of tile j - 1 too: O_t may be rescaled
-          if (t == w.ntile - 1) {
-            umma_commit(&sm.kv_empty[kslot]);
-            if (j == w.n - 1) umma_commit(&sm.q_empty);
+          if (t == ntile - 1) {
+            umma_commit(&sm.kv_empty[vp.slot]);
+            if (j < n) umma_commit(&sm.kv_empty[kp.slot]);
+            if (j == n - 1) umma_commit(&sm.q_empty);
           }
-        } else {
-          umma_commit(&sm.o_full[t]);
         }
-      }
-      if (j < w.n) {
-        vslot = (L + 1) % C::kSlots;
-        L += 2;
+        __syncwarp();
       }
     }
   }
@@ -641,15 +806,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < TcCfg<D>::kSlots; ++i) {
       mbar_init(&sm.kv_full[i], 1);
-      mbar_init(&sm.kv_empty[i], 1);
+      mbar_init(&sm.kv_empty[i], 2);  // the products and the cleaner
+      mbar_init(&sm.v_clean[i], 1);
     }
     mbar_init(&sm.q_full, 1);
     mbar_init(&sm.q_empty, 1);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&sm.s_full[t], 1);
-      mbar_init(&sm.p_full[t], 128);
+      mbar_init(&sm.p_full[t], 4);
       mbar_init(&sm.o_full[t], 1);
-      mbar_init(&sm.o_free[t], 128);
+      mbar_init(&sm.o_free[t], 4);
     }
     mbar_init(&sm.drain, 1);
     sm.abort = 0;
@@ -676,9 +842,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kProducerWarp) {
       if ((threadIdx.x & 31) == 0) tc_producer<D>(sm, x, &mq, &mk, &mv, &mdk, &mdv);
       __syncwarp();
+    } else if (warp == kCleanWarp) {
+      tc_cleaner<D>(sm, x);
     } else if (warp == kMmaWarp) {
-      if ((threadIdx.x & 31) == 0) {
-        tc_mma<D>(sm, x, tmem);
+      tc_mma<D>(sm, x, tmem);
+      __syncwarp();
+      if (elect_one()) {
         umma_commit(&sm.drain);  // every MMA in flight, before the memory is freed
         if (!mbar_wait(&sm.drain, 0)) atomicExch(&g_token_status, 1);
       }
@@ -740,13 +909,6 @@ __device__ __forceinline__ TwUnit tw_unit(const TcArgs& x, int u) {
 }
 
 template <int D>
-__device__ __forceinline__ bool tw_wait(TwSmem<D>& sm, uint64_t* bar, uint32_t parity) {
-  const bool ok = *(volatile int*)&sm.abort == 0 && mbar_wait(bar, parity);
-  if (!ok && atomicExch(&sm.abort, 1) == 0) atomicExch(&g_token_status, 1);
-  return __all_sync(0xffffffffu, ok);
-}
-
-template <int D>
 __device__ void tw_producer(TwSmem<D>& sm, const TcArgs& x, const CUtensorMap* mq, const CUtensorMap* mk) {
   using C = TcCfg<D>;
   const TokArgs& a = x.t;
@@ -761,7 +923,7 @@ __device__ void tw_producer(TwSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
     if (u >= x.units) continue;
     const TwUnit w = tw_unit(x, u);
     if (w.n == 0) continue;
-    if (!tw_wait<D>(sm, &sm.k_empty, k_ph ^ 1)) return drain();
+    if (!bar_wait_warp(&sm.abort, &sm.k_empty, k_ph ^ 1)) return drain();
     k_ph ^= 1;
     if (lane == 0) {
       mbar_expect_tx(&sm.k_full, (uint32_t)(w.ntile * C::kTileBytes));
@@ -779,7 +941,7 @@ __device__ void tw_producer(TwSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
         lse[k] = pos < a.Sq ? a.lse[(int64_t)w.bh * a.R + (int64_t)pos * a.G + hs * x.Gp + col % x.Gp] : INFINITY;
       }
       const uint32_t slot = L % kWqSlots;
-      if (!tw_wait<D>(sm, &sm.q_empty[slot], ((L / kWqSlots) & 1) ^ 1)) return drain();
+      if (!bar_wait_warp(&sm.abort, &sm.q_empty[slot], ((L / kWqSlots) & 1) ^ 1)) return drain();
 #pragma unroll
       for (int k = 0; k < 4; ++k) sm.lse[slot][32 * k + lane] = lse[k];
       if (lane == 0) {
@@ -805,17 +967,17 @@ __device__ void tw_mma(TwSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
     if (u >= x.units) continue;
     const TwUnit w = tw_unit(x, u);
     if (w.n == 0) continue;
-    if (!tw_wait<D>(sm, &sm.k_full, k_ph)) return;
+    if (!bar_wait_warp(&sm.abort, &sm.k_full, k_ph)) return;
     k_ph ^= 1;
     for (int i = 0; i < w.n; ++i, ++L) {
       const uint32_t slot = L % kWqSlots;
-      if (!tw_wait<D>(sm, &sm.q_full[slot], (L / kWqSlots) & 1)) return;
+      if (!bar_wait_warp(&sm.abort, &sm.q_full[slot], (L / kWqSlots) & 1)) return;
       tc_fence_after();
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (t >= w.ntile) break;
         const uint32_t buf = use[t] & 1;
-        if (!tw_wait<D>(sm, &sm.s_empty[t][buf], ((use[t] >> 1) & 1) ^ 1)) return;
+        if (!bar_wait_warp(&sm.abort, &sm.s_empty[t][buf], ((use[t] >> 1) & 1) ^ 1)) return;
         ++use[t];
         tc_fence_after();
         if (lead) {
@@ -855,10 +1017,10 @@ __device__ void tw_sum(TwSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem, con
     float edge = 0.f;
     for (int i = 0; i < w.n; ++i, ++L) {
       const uint32_t slot = L % kWqSlots;
-      if (!tw_wait<D>(sm, &sm.q_full[slot], (L / kWqSlots) & 1)) return;  // the denominators
+      if (!bar_wait_warp(&sm.abort, &sm.q_full[slot], (L / kWqSlots) & 1)) return;  // the denominators
       if (t < w.ntile) {
         const uint32_t buf = use & 1;
-        if (!tw_wait<D>(sm, &sm.s_full[t][buf], (use >> 1) & 1)) return;
+        if (!bar_wait_warp(&sm.abort, &sm.s_full[t][buf], (use >> 1) & 1)) return;
         ++use;
         tc_fence_after();
         float s[128];
@@ -869,7 +1031,7 @@ __device__ void tw_sum(TwSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem, con
         const float4* lse = reinterpret_cast<const float4*>(sm.lse[slot]);
         // rows [lo, hi) of the tile see this thread's key
         const bool part = w.j0 + t * kTok + kTok - 1 > pos0 || p0 + x.P > a.Sq;
-        const bool far = CAP && cap_far(s, x.k_in);
+        const bool far = CAP && cap_far<128>(s, x.k_in);
         if (!part && !far) {
           const uint64_t sc2 = pk2(c_scale, c_scale);
 #pragma unroll
@@ -878,8 +1040,8 @@ __device__ void tw_sum(TwSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem, con
             const uint64_t n0 = pk2(-z.x, -z.y), n1 = pk2(-z.z, -z.w);
             uint64_t e0, e1;
             if (CAP) {
-              e0 = cap.poly2(pk2(s[k], s[k + 1]), n0);
-              e1 = cap.poly2(pk2(s[k + 2], s[k + 3]), n1);
+              e0 = cap.poly2<3>(pk2(s[k], s[k + 1]), n0);
+              e1 = cap.poly2<3>(pk2(s[k + 2], s[k + 3]), n1);
             } else {
               e0 = fma2(pk2(s[k], s[k + 1]), sc2, n0);
               e1 = fma2(pk2(s[k + 2], s[k + 3]), sc2, n1);
