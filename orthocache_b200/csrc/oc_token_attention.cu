@@ -440,8 +440,11 @@ inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 //
 // Split of the keys: the CTAs of all (row tile, batch row, KV head, chunk) run
 // in waves of one (tcgen05) or two per SM; of the possible numbers of chunks
-// the one with the least waves x (keys of a chunk + what a CTA's set-up and its
-// partial cost, in keys) is taken.
+// the one with the least waves x (keys of a chunk + what a CTA's set-up costs, in
+// keys) plus the traffic of the partials is taken.  Row tiles of a causal chunk
+// as long as a good part of its sequence differ in work and fill the SMs evenly
+// by themselves; documents shorten the spans to a length the host does not
+// know: then keys are split only while there are fewer row tiles than SMs.
 constexpr int kTcRows = 64;
 
 // The accumulating form needs every score again once the denominators are
@@ -451,7 +454,7 @@ constexpr int kTcRows = 64;
 constexpr int kLogitRows = 16;
 
 TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int head_dim, int seq_len, float scale,
-                 bool lse) {
+                 bool uneven, bool lse) {
   TokPlan p;
   const int G = q_heads / kv_heads;
   const int64_t R = (int64_t)q_len * G;
@@ -474,12 +477,17 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
   }
   int64_t most = seq_len / (2 * step);
   if (most > 2 * slots / units + 4) most = 2 * slots / units + 4;
-  int64_t best = 0;
+  if (uneven && units >= slots) most = 1;
+  // partials: rows x head_dim floats written and read at about 6 TB/s, in keys of
+  // one CTA (the tcgen05 kernel takes 67 keys a microsecond, the others less)
+  const double part_keys = p.tc ? 256.0 * head_dim * 8 / 6e6 * 67 : 0.0;
+  double best = 0;
   p.nchunk = 1;
   p.chunk = seq_len < step ? step : (seq_len + step - 1) / step * step;
   for (int64_t n = 1; n <= most; ++n) {
     const int64_t keys = ((seq_len + n - 1) / n + step - 1) / step * step;
-    const int64_t cost = (units * n + slots - 1) / slots * (keys + (n > 1 ? setup : 0));
+    const double cost =
+        (double)((units * n + slots - 1) / slots) * (keys + (n > 1 ? setup : 0)) + (n > 1 ? units * n * part_keys : 0);
     if (n == 1 || cost < best) {
       best = cost;
       p.chunk = (int)keys;
@@ -592,7 +600,8 @@ int tok_common(const char* fn, TokArgs& a, const void* q, const void* k, const v
 
 int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void* workspace, size_t workspace_bytes,
             cudaStream_t st, const float* w_in = nullptr, float* w_out = nullptr) {
-  const TokPlan p = tok_plan(dtype, a.B, a.Sq, a.Hq, a.Hkv, head_dim, a.S, a.scale, lse);
+  const bool uneven = a.docs || (a.causal && a.Sq > a.S / 4);
+  const TokPlan p = tok_plan(dtype, a.B, a.Sq, a.Hq, a.Hkv, head_dim, a.S, a.scale, uneven, lse);
   OC_REQUIRE((int64_t)a.B * a.Hkv * p.nchunk * (p.tc ? tok_tc_shape(a.Sq, a.G).npairs : p.nrt) < INT32_MAX &&
                  p.nchunk <= 65535,
              OC_ERR_SHAPE, "%s: too many work units", fn);
@@ -639,10 +648,14 @@ extern "C" size_t oc_token_attention_workspace_bytes(int dtype, int batch, int q
   if (batch < 1 || q_len < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || seq_len < 0 ||
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return 0;
-  // the larger of what a positive scale and any other need
-  const size_t pos = tok_plan(dtype, batch, q_len, q_heads, kv_heads, head_dim, seq_len, 1.f, accumulate != 0).bytes;
-  const size_t any = tok_plan(dtype, batch, q_len, q_heads, kv_heads, head_dim, seq_len, 0.f, accumulate != 0).bytes;
-  return pos > any ? pos : any;
+  // the most that any call of these sizes needs
+  size_t most = 0;
+  for (int i = 0; i < 4; ++i) {
+    const size_t n = tok_plan(dtype, batch, q_len, q_heads, kv_heads, head_dim, seq_len, i & 1 ? 1.f : 0.f, (i & 2) != 0,
+                              accumulate != 0).bytes;
+    if (n > most) most = n;
+  }
+  return most;
 }
 
 extern "C" int oc_tree_attention(const void* q, const void* k, const void* v, int dtype, const int32_t* block_table,

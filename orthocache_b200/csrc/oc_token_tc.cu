@@ -351,11 +351,21 @@ __device__ __forceinline__ float exp_pack(const float* s, uint32_t t_s, float m)
 template <int D, int DEG, bool BIAS>
 __device__ __forceinline__ void chunk_exp(const float* s, int c, uint32_t* pk, uint64_t (&r2)[4], float& top,
                                           float c_scale, uint64_t nm2, uint64_t sl2, float b0, const CapFn& cap) {
+  uint64_t off4[4];
+  if (BIAS) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      off4[i] = fma2(pk2((float)(32 * c + 2 * i), (float)(32 * c + 2 * i + 1)), sl2, pk2(b0, b0));
+  }
+  const uint64_t step = BIAS ? mul2(pk2(8.f, 8.f), sl2) : 0;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const uint64_t v = pk2(s[2 * i], s[2 * i + 1]);
     uint64_t off = nm2;
-    if (BIAS) off = fma2(pk2((float)(32 * c + 2 * i), (float)(32 * c + 2 * i + 1)), sl2, pk2(b0, b0));
+    if (BIAS) {
+      off = off4[i & 3];
+      off4[i & 3] = add2(off, step);
+    }
     if (DEG) top = absmax3(top, s[2 * i], s[2 * i + 1]);
     const uint64_t e = DEG ? cap.poly2<DEG ? DEG : 2>(v, off) : fma2(v, pk2(c_scale, c_scale), off);
     float e0, e1;
@@ -489,29 +499,41 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
           for (int i = 0; i < 128; ++i) s[i] = fmaf(-row.slope2, fabsf(d0 - (float)i), s[i]);
         }
         if (part) {
+          // which of the 128 keys the row sees, a bit each
+          uint32_t vis[4];
           if (draft) {
             const uint4 bits = real ? x.tree_bits[((size_t)w.b * (a.Sq + 1) + pos_i) * 2 + jt] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 128; ++i) {
-              const uint32_t word = i < 32 ? bits.x : i < 64 ? bits.y : i < 96 ? bits.z : bits.w;
-              if (!(word >> (i & 31) & 1)) s[i] = -INFINITY;
-            }
+            vis[0] = bits.x;
+            vis[1] = bits.y;
+            vis[2] = bits.z;
+            vis[3] = bits.w;
           } else {
             const int lim = a.table && tc_key_row(a, w.b, jt) < 0 ? 0 : row.hi - j0;
 #pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (i >= lim) s[i] = -INFINITY;
+            for (int y = 0; y < 4; ++y) vis[y] = lim >= 32 * y + 32 ? ~0u : lim <= 32 * y ? 0u : (1u << (lim - 32 * y)) - 1u;
             if (a.docs) {
+              // one round per document among the warp's rows
+              int d[4];
 #pragma unroll
               for (int y = 0; y < 4; ++y) {
                 const int jj = j0 + 32 * y + lane;
-                const int d = jj < a.S ? a.docs[(size_t)w.b * a.S + jj] : -1;
+                d[y] = jj < a.S ? a.docs[(size_t)w.b * a.S + jj] : -1;
+              }
+              uint32_t todo = ~0u;
+              while (todo) {
+                const int doc = __shfl_sync(0xffffffffu, row.doc, __ffs(todo) - 1);
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (__shfl_sync(0xffffffffu, d, i) != row.doc) s[32 * y + i] = -INFINITY;
+                for (int y = 0; y < 4; ++y) {
+                  const uint32_t same = __ballot_sync(0xffffffffu, d[y] == doc);
+                  if (row.doc == doc) vis[y] &= same;
+                }
+                todo &= ~__ballot_sync(0xffffffffu, row.doc == doc);
               }
             }
           }
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (!(vis[i >> 5] >> (i & 31) & 1)) s[i] = -INFINITY;
         }
         if (CAP != 1) {
           const float mx = row_max(s);
