@@ -35,9 +35,13 @@ struct TokArgs {
   float scale, cap;
   void* out;
   int out_dtype;
-  // split over the keys: chunk c covers tokens [c * chunk, (c + 1) * chunk)
-  int chunk, nchunk, nrt;        // nrt row tiles per (b, h)
-  float *pm, *pl, *po;           // partials: [(bh * nrt + rt) * nchunk + c][row tile][(D)]
+  // A unit is a row tile of one (b, h): units of batch row b are numbered h *
+  // nrt + rt.  Either every unit is one CTA's (even = 0), or the key tiles of
+  // all units, laid end to end, are cut into equal runs, ncta in all (even = 1).
+  int nrt, even, ncta, tile;  // row tiles per (b, h); keys of a tile
+  int hg;                     // heads that are cut alike; divides Hkv and ncta
+  int unit_rows;              // rows of a unit's partial
+  float *pm, *pl, *po;        // partials: [part][unit_rows][(D)], parts 2 * cta and 2 * cta + 1
   float* logits;                 // (B * Hkv, R, logit_stride) scores in log2 units, -inf where masked; nullable
   int64_t logit_stride;
   float* lse;                    // (B * Hkv, R) log2 of the softmax denominator, +inf for empty rows; nullable
@@ -87,6 +91,79 @@ __device__ __forceinline__ TokRow tok_row(const TokArgs& a, int b, int h, int r,
   return w;
 }
 
+// ---- the even cut ---------------------------------------------------------
+// The lengths are on the device, so the cut is made there: every CTA adds up
+// the rows' tiles (at most kMaxEvenBatch of them) and finds its run.  A run
+// begins and ends inside a unit at most; those two pieces are partials, which
+// tok_merge_kernel joins.  hg neighbouring heads, whose keys lie side by side in
+// memory, are cut alike and go to hg neighbouring CTAs, which read the same
+// tokens at about the same time: DRAM pages are then opened for hg heads' bytes
+// instead of one's.
+constexpr int kMaxEvenBatch = 256;
+
+__device__ __forceinline__ int tok_tiles(const TokArgs& a, int b) {
+  const int n = (tok_len(a, b) + a.tile - 1) / a.tile + (a.dk ? (a.Sq + a.tile - 1) / a.tile : 0);
+  return n > 0 ? n : 1;  // a unit without keys still has rows to write
+}
+
+// pre[b] = tiles of a unit of the rows before b (one warp).
+__device__ __forceinline__ void tok_prefix(const TokArgs& a, int* pre) {
+  const int lane = threadIdx.x & 31;
+  int run = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    int n = b0 + lane < a.B ? tok_tiles(a, b0 + lane) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, n, o);
+      if (lane >= o) n += y;
+    }
+    if (b0 + lane < a.B) pre[b0 + lane + 1] = run + n;
+    run += __shfl_sync(0xffffffffu, n, 31);
+  }
+  if (lane == 0) pre[0] = 0;
+}
+
+struct TokSeg {
+  int b, unit, t0, t1;  // tiles [t0, t1) of the unit
+  int part;             // -1: the whole unit
+};
+
+// Runs of one head of a group: no more than there are tiles, so that none is
+// empty.
+__device__ __forceinline__ int tok_runs(const TokArgs& a, int64_t total) {
+  const int n = a.ncta / a.hg;
+  return total < n ? (total > 0 ? (int)total : 1) : n;
+}
+
+struct TokWalk {
+  int64_t x, lo, hi;
+  int b;
+  __device__ __forceinline__ TokWalk(const TokArgs& a, const int* pre, int cta) {
+    const int64_t total = a.even ? (int64_t)(a.Hkv / a.hg) * a.nrt * pre[a.B] : 0;
+    const int n = tok_runs(a, total), i = cta / a.hg;
+    lo = i < n ? total * i / n : 0;
+    hi = i < n ? total * (i + 1) / n : 0;
+    x = lo;
+    b = 0;
+  }
+  __device__ __forceinline__ bool next(const TokArgs& a, const int* pre, int cta, TokSeg& s) {
+    if (x >= hi) return false;
+    const int64_t upb = (int64_t)(a.Hkv / a.hg) * a.nrt;
+    while (x >= upb * pre[b + 1]) ++b;
+    const int64_t rel = x - upb * pre[b];
+    const int nt = pre[b + 1] - pre[b];
+    const int u = (int)(rel / nt);  // head group * nrt + row tile
+    s.b = b;
+    s.unit = (u / a.nrt * a.hg + cta % a.hg) * a.nrt + u % a.nrt;
+    s.t0 = (int)(rel % nt);
+    const int64_t left = hi - x;
+    s.t1 = left < nt - s.t0 ? s.t0 + (int)left : nt;
+    s.part = s.t0 == 0 && s.t1 == nt ? -1 : 2 * cta + (x == lo ? 0 : 1);
+    x += s.t1 - s.t0;
+    return true;
+  }
+};
+
 // Row (of the (rows, Hkv, D) view of k / v) of token j of batch row b; -1 for
 // a token whose page lies outside the pool.
 __device__ __forceinline__ int64_t tok_kv_row(const TokArgs& a, int b, int j) {
@@ -110,11 +187,11 @@ __device__ __forceinline__ float tok_score(const TokArgs& a, float dot, float sl
 
 // The bfloat16 kernel for few rows (oc_token_mma.cu); row_tile 16, 32 or 64.
 int tok_mma(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st);
+int tok_mma_tile(int head_dim);  // keys of its tiles
 
 // The bfloat16 kernel on the tcgen05 tensor cores (oc_token_tc.cu) for
-// head_dim 64 and 128 and a positive scale.  chunk is a multiple of 128;
-// partials are indexed [(bh * nchunk + c) * R + r].  prep: tok_tc_prep_bytes
-// of scratch.
+// head_dim 64 and 128 and a positive scale; a unit is a pair of row tiles.
+// prep: tok_tc_prep_bytes of scratch.
 struct TokTcShape {
   int Gp, nhs, P, npt, npairs;  // heads and positions of a row tile; head groups, position tiles, pairs of row tiles
 };
@@ -126,7 +203,7 @@ int tok_tc(const char* fn, const TokArgs& a, int head_dim, void* prep, cudaStrea
 // (bfloat16, head_dim 64 or 128, contiguous keys, positive scale).
 int tok_tc_weights(const char* fn, const TokArgs& a, int head_dim, const float* w_in, float* w_out, cudaStream_t st);
 
-// Merge of the partials of all chunks (oc_token_attention.cu).
-int tok_merge(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st);
+// Merge of the partials of the even cut (oc_token_attention.cu).
+int tok_merge(const TokArgs& a, int head_dim, bool tc, cudaStream_t st);
 
 }  // namespace oc

@@ -12,6 +12,7 @@
 // (src/orthocache/indirect_attention.py:29-170).
 #include <math.h>
 
+#include "oc_mma.cuh"
 #include "oc_token.cuh"
 
 namespace oc {
@@ -29,7 +30,8 @@ struct SimtSmem {
   TokRow row[16 * RPT];
   int doc[kSimtTok];
   int seen[kSimtTok];
-  int hi, lo;
+  int hi;
+  int pre[kMaxEvenBatch + 1];
 };
 
 // Load keys [j0, j0 + 64) of the cache (or of the drafted tokens) as float32.
@@ -57,18 +59,29 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
   extern __shared__ __align__(16) unsigned char raw[];
   SimtSmem<D, RPT>& sm = *reinterpret_cast<SimtSmem<D, RPT>*>(raw);
   constexpr int RT = 16 * RPT, kVec = Elem<T>::kVec, NC = D / 64;
-  const int bh = blockIdx.x % (a.B * a.Hkv);
-  const int rt = a.nrt - 1 - blockIdx.x / (a.B * a.Hkv);  // the rows with most keys first
-  const int b = bh / a.Hkv, h = bh % a.Hkv, c = blockIdx.y;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int len = tok_len(a, b);
   const T* kbase = static_cast<const T*>(a.k);
   const T* vbase = static_cast<const T*>(a.v);
-
-  if (tid == 0) {
-    sm.hi = 0;
-    sm.lo = INT32_MAX;
+  pdl_trigger();  // the merge may find its parts meanwhile
+  if (a.even) {
+    if (tid < 32) tok_prefix(a, sm.pre);
+    __syncthreads();
   }
+  TokWalk walk(a, sm.pre, blockIdx.x);
+  TokSeg seg;
+  for (bool more = true; more;) {
+  if (a.even) {
+    if (!walk.next(a, sm.pre, blockIdx.x, seg)) break;
+  } else {
+    // a CTA per unit, the rows with most keys first
+    const int bh = blockIdx.x % (a.B * a.Hkv);
+    seg = TokSeg{bh / a.Hkv, bh % a.Hkv * a.nrt + a.nrt - 1 - (int)(blockIdx.x / (a.B * a.Hkv)), 0, INT32_MAX, -1};
+    more = false;
+  }
+  const int b = seg.b, h = seg.unit / a.nrt, rt = seg.unit % a.nrt, bh = b * a.Hkv + h;
+  const int len = tok_len(a, b);
+  __syncthreads();  // the previous piece is done with shared memory
+  if (tid == 0) sm.hi = 0;
   __syncthreads();
   for (int r = tid; r < RT; r += kSimtThreads) {
     sm.row[r] = tok_row(a, b, h, rt * RT + r, len);
@@ -83,11 +96,11 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
       for (int y = 0; y < kVec; ++y) sm.q[r][x + y] = 0.f;
   }
   __syncthreads();
-  const int t0 = c * a.chunk;
-  int t1 = min(sm.hi, t0 + a.chunk);
-  if (t1 < t0) t1 = t0;
+  const int nct = (len + kSimtTok - 1) / kSimtTok;  // tiles of the cache; drafted tokens follow
+  const int t0 = min(seg.t0, nct) * kSimtTok, t1 = max(t0, min(sm.hi, min(seg.t1, nct) * kSimtTok));
   const int ncache = (t1 - t0 + kSimtTok - 1) / kSimtTok;
-  const int ndraft = a.dk && c == a.nchunk - 1 ? (a.Sq + kSimtTok - 1) / kSimtTok : 0;
+  const int d0 = max(seg.t0 - nct, 0);
+  const int ndraft = a.dk && seg.t1 > nct ? min(seg.t1 - nct, (a.Sq + kSimtTok - 1) / kSimtTok) - d0 : 0;
 
   TokRow row[RPT];
   float m[RPT], l[RPT], o[RPT][NC * 4];
@@ -102,7 +115,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
 
   for (int tile = 0; tile < ncache + ndraft; ++tile) {
     const bool draft = tile >= ncache;
-    const int j0 = draft ? (tile - ncache) * kSimtTok : t0 + tile * kSimtTok;
+    const int j0 = draft ? (d0 + tile - ncache) * kSimtTok : t0 + tile * kSimtTok;
     __syncthreads();  // the previous tile's keys and values are read
     if (tid < kSimtTok) {
       const int j = j0 + tid;
@@ -217,8 +230,8 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
   for (int i = 0; i < RPT; ++i) {
     const int rl = ty + 16 * i, r = rt * RT + rl;
     if (r >= a.R) continue;
-    if (a.nchunk > 1) {
-      const int64_t part = ((int64_t)(bh * a.nrt + rt) * a.nchunk + c) * RT + rl;
+    if (seg.part >= 0) {
+      const int64_t part = (int64_t)seg.part * RT + rl;
       if (tx == 0) {
         a.pm[part] = m[i];
         a.pl[part] = l[i];
@@ -244,57 +257,161 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
           static_cast<float*>(a.out)[at + 4 * tx + 64 * cc + y] = val;
       }
   }
+  }
 }
 
-// One warp per query row: out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c.
-template <int D>
-__global__ void __launch_bounds__(128) tok_merge_kernel(const TokArgs a, int row_tile) {
+// out = sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p over the parts p of a row's
+// unit.  A block takes rows of one unit (a unit without parts was written by its
+// CTA): the parts are found once for all of them.  WPR warps share a row: eight
+// when there are few rows with many parts, whose loads then run side by side,
+// one when there are many rows.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeMaxParts = 2 * 256;  // CTAs of the even cut, at most two per SM
+
+template <int D, int WPR>
+__global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs a, const TokTcShape tc, int blocks_per_unit) {
+  __shared__ int s_part[kMergeMaxParts];
+  __shared__ int s_tiles[3];  // tiles of a unit: of the rows before b, of all rows, of row b
+  __shared__ int s_c[2];
+  __shared__ float s_l[8], s_o[WPR > 1 ? 8 : 1][D];
+  const int unit = blockIdx.x / blocks_per_unit, block = blockIdx.x % blocks_per_unit;
+  const int upb = a.Hkv * a.nrt, b = unit / upb, h = unit % upb / a.nrt, rt = unit % a.nrt;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid < 32) {
+    int before = 0, all = 0, mine = 0;
+    for (int y = lane; y < a.B; y += 32) {
+      const int n = tok_tiles(a, y);
+      all += n;
+      if (y < b) before += n;
+      if (y == b) mine = n;
+    }
+    all = __reduce_add_sync(0xffffffffu, all);
+    before = __reduce_add_sync(0xffffffffu, before);
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if (lane == 0) {
+      s_tiles[0] = before;
+      s_tiles[1] = all;
+      s_tiles[2] = mine;
+    }
+  }
+  __syncthreads();
+  const int64_t upg = (int64_t)(a.Hkv / a.hg) * a.nrt, total = upg * s_tiles[1];
+  const int64_t start = upg * s_tiles[0] + (int64_t)(h / a.hg * a.nrt + rt) * s_tiles[2], end = start + s_tiles[2];
+  const int n = tok_runs(a, total);
+  if (tid < 2)  // the runs [total i / n, total (i + 1) / n) that hold its first and last tile
+    s_c[tid] = (int)(((tid ? end : start + 1) * n - 1) / total);
+  __syncthreads();
+  const int c0 = s_c[0], parts = s_c[1] - c0 + 1;
+  if (parts <= 1) return;
+  for (int c = tid; c < parts; c += kMergeThreads) 
+    s_part[c] = 2 * ((c0 + c) * a.hg + h % a.hg) + (total * (c0 + c) / n >= start ? 0 : 1);
+  __syncthreads();
   pdl_wait();
-  const int64_t gr = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (gr >= (int64_t)a.B * a.Hkv * a.R) return;
-  const int bh = (int)(gr / a.R), r = (int)(gr % a.R);
-  const int rt = r / row_tile, rl = r % row_tile;
-  const int64_t base = (int64_t)(bh * a.nrt + rt) * a.nchunk;
-  float M = -INFINITY;
-  for (int c = lane; c < a.nchunk; c += 32) M = fmaxf(M, a.pm[(base + c) * row_tile + rl]);
-  M = warp_max(M);
-  float o[D / 32], L = 0.f;
+
+  constexpr int kV = D < 128 ? 2 : 4, kN = D / 32 / kV, kRows = 8 / WPR;  // rows of a block at a time
+  const int rows = a.unit_rows;
+  for (int r0 = block * kRows; r0 < rows; r0 += blocks_per_unit * kRows) {
+    const int rl = r0 + (WPR > 1 ? 0 : warp);
+    // query row of local row rl of the unit
+    int r;
+    bool real = rl < rows;
+    if (tc.Gp) {
+      const int t = 2 * rt + rl / 128, i = t / tc.nhs * tc.P + rl % 128 / tc.Gp;
+      real = real && t < tc.npt * tc.nhs && i < a.Sq;
+      r = i * a.G + t % tc.nhs * tc.Gp + rl % 128 % tc.Gp;
+    } else {
+      r = rt * rows + rl;
+      real = real && r < a.R;
+    }
+    if (!real) continue;  // with WPR > 1 the same for the whole block
+    float M = -INFINITY;
+    for (int c = lane; c < parts; c += 32) M = fmaxf(M, a.pm[(int64_t)s_part[c] * rows + rl]);
+    M = warp_max(M);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float o[D / 32], L = 0.f;
 #pragma unroll
-  for (int x = 0; x < D / 32; ++x) o[x] = 0.f;
-  const float ref = M == -INFINITY ? 0.f : M;
-  for (int c = 0; c < a.nchunk; ++c) {
-    const int64_t part = (base + c) * row_tile + rl;
-    const float mc = a.pm[part];
-    if (mc == -INFINITY) {
-      L += a.pl[part];  // 0, or NaN when every visible score was NaN
+    for (int x = 0; x < D / 32; ++x) o[x] = 0.f;
+#pragma unroll 4
+    for (int c = WPR > 1 ? warp : 0; c < parts; c += WPR) {
+      const int64_t part = (int64_t)s_part[c] * rows + rl;
+      const float mc = a.pm[part], lc = a.pl[part];
+      const bool any = mc != -INFINITY;
+      const float w = any ? exp2f(mc - ref) : 1.f;
+      L += w * lc;  // of a part without keys 0, or NaN when every visible score was NaN
+      if (any) {
+#pragma unroll
+        for (int x = 0; x < kN; ++x) {
+          float v[kV];
+          const float* src = a.po + part * D + x * 32 * kV + lane * kV;
+          if (kV == 4)
+            *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+          else
+            *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+#pragma unroll
+          for (int y = 0; y < kV; ++y) o[x * kV + y] += w * v[y];
+        }
+      }
+    }
+    if (WPR > 1) {  // add up the eight warps
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < kN; ++x)
+#pragma unroll
+        for (int y = 0; y < kV; ++y) s_o[warp][x * 32 * kV + lane * kV + y] = o[x * kV + y];
+      if (lane == 0) s_l[warp] = L;
+      __syncthreads();
+      if (tid < D / 4) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        L = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          L += s_l[w];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) acc[y] += s_o[w][4 * tid + y];
+        }
+        if (a.lse && tid == 0) a.lse[(int64_t)(b * a.Hkv + h) * a.R + r] = L == 0.f ? INFINITY : M + log2f(L);
+        const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+        const int64_t at = tok_q_offset(a, b, h, r, D) + 4 * tid;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          if (a.out_dtype == OC_BF16)
+            static_cast<__nv_bfloat16*>(a.out)[at + y] = __float2bfloat16_rn(acc[y] * inv);
+          else
+            static_cast<float*>(a.out)[at + y] = acc[y] * inv;
+        }
+      }
       continue;
     }
-    const float w = exp2f(mc - ref);
-    L += w * a.pl[part];
+    if (a.lse && lane == 0) a.lse[(int64_t)(b * a.Hkv + h) * a.R + r] = L == 0.f ? INFINITY : M + log2f(L);
+    const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+    const int64_t at = tok_q_offset(a, b, h, r, D);
 #pragma unroll
-    for (int x = 0; x < D / 128 + (D < 128); ++x) {
-      constexpr int kV = D < 128 ? 2 : 4;
+    for (int x = 0; x < kN; ++x) {
+      const int64_t e = at + x * 32 * kV + lane * kV;
+      if (a.out_dtype == OC_BF16) {
 #pragma unroll
-      for (int y = 0; y < kV; ++y) o[x * kV + y] += w * a.po[part * D + x * 32 * kV + lane * kV + y];
+        for (int y = 0; y < kV; y += 2)
+          *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + e + y) =
+              pack_bf16x2(o[x * kV + y] * inv, o[x * kV + y + 1] * inv);
+      } else {
+#pragma unroll
+        for (int y = 0; y < kV; ++y) static_cast<float*>(a.out)[e + y] = o[x * kV + y] * inv;
+      }
     }
   }
-  if (a.lse && lane == 0) a.lse[gr] = L == 0.f ? INFINITY : M + log2f(L);
-  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-  const int64_t at = tok_q_offset(a, bh / a.Hkv, bh % a.Hkv, r, D);
-#pragma unroll
-  for (int x = 0; x < D / 128 + (D < 128); ++x) {
-    constexpr int kV = D < 128 ? 2 : 4;
-#pragma unroll
-    for (int y = 0; y < kV; ++y) {
-      const int64_t e = at + x * 32 * kV + lane * kV + y;
-      const float val = o[x * kV + y] * inv;
-      if (a.out_dtype == OC_BF16)
-        static_cast<__nv_bfloat16*>(a.out)[e] = __float2bfloat16_rn(val);
-      else
-        static_cast<float*>(a.out)[e] = val;
-    }
-  }
+}
+
+template <int D>
+int launch_merge(const TokArgs& a, const TokTcShape& tc, cudaStream_t st) {
+  const int units = a.B * a.Hkv * a.nrt;
+  // rows of a unit that exist at most, and whether all rows together are few
+  const int rows = a.R < a.unit_rows ? a.R : a.unit_rows;
+  const bool few = (int64_t)units * rows <= 4096;
+  const int bpu = few ? rows : (rows + 31) / 32;
+  cudaError_t e = few ? launch_pdl(tok_merge_kernel<D, 8>, dim3(units * bpu), dim3(kMergeThreads), 0, st, a, tc, bpu)
+                      : launch_pdl(tok_merge_kernel<D, 1>, dim3(units * bpu), dim3(kMergeThreads), 0, st, a, tc, bpu);
+  if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_merge_kernel: %s", cudaGetErrorString(e));
+  return OC_OK;
 }
 
 // Column sums of the softmax: for 64 keys of (b, h), the weights 2^(s - lse_r)
@@ -408,27 +525,20 @@ __global__ void __launch_bounds__(256) tok_sum_kernel(const TokArgs a, const flo
 
 }  // namespace
 
-int tok_merge(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st) {
-  const int64_t rows = (int64_t)a.B * a.Hkv * a.R;
-  const dim3 grid((unsigned)((rows + 3) / 4));
-  cudaError_t e;
-  if (head_dim == 64)
-    e = launch_pdl(tok_merge_kernel<64>, grid, dim3(128), 0, st, a, row_tile);
-  else if (head_dim == 128)
-    e = launch_pdl(tok_merge_kernel<128>, grid, dim3(128), 0, st, a, row_tile);
-  else
-    e = launch_pdl(tok_merge_kernel<256>, grid, dim3(128), 0, st, a, row_tile);
-  if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_merge_kernel: %s", cudaGetErrorString(e));
-  return OC_OK;
+int tok_merge(const TokArgs& a, int head_dim, bool tc, cudaStream_t st) {
+  const TokTcShape shape = tc ? tok_tc_shape(a.Sq, a.G) : TokTcShape{};
+  return head_dim == 64 ? launch_merge<64>(a, shape, st)
+                        : head_dim == 128 ? launch_merge<128>(a, shape, st) : launch_merge<256>(a, shape, st);
 }
 
 namespace {
 
 // How a call is cut.
 struct TokPlan {
-  bool tc;            // the tcgen05 kernel
-  int row_tile, nrt;  // rows per tile, row tiles per (b, h)
-  int chunk, nchunk;  // keys per chunk, chunks
+  bool tc, even;                          // the tcgen05 kernel; the even cut of the keys
+  int row_tile, nrt, unit_rows;           // rows per tile, units per (b, h), rows of a unit
+  int tile, ncta, hg;                     // keys per tile, CTAs of the even cut, heads cut alike
+  int64_t units;
   size_t lse_off, m_off, l_off, o_off, prep_off, logit_off, logit_stride, bytes;  // logit_stride 0: none
 };
 
@@ -438,14 +548,16 @@ inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // bfloat16 the m16n8k16 kernel (16, 32 or 64 rows, what the rows fill) or, for
 // more than kTcRows rows per KV head at head_dim 64 and 128, the tcgen05 one.
 //
-// Split of the keys: the CTAs of all (row tile, batch row, KV head, chunk) run
-// in waves of one (tcgen05) or two per SM; of the possible numbers of chunks
-// the one with the least waves x (keys of a chunk + what a CTA's set-up costs, in
-// keys) plus the traffic of the partials is taken.  Row tiles of a causal chunk
-// as long as a good part of its sequence differ in work and fill the SMs evenly
-// by themselves; documents shorten the spans to a length the host does not
-// know: then keys are split only while there are fewer row tiles than SMs.
+// Cut: with few units (row tile, batch row, KV head) for the GPU, all their key
+// tiles are dealt out evenly over one (tcgen05) or two CTAs per SM, so that
+// ragged lengths and odd numbers of units cost nothing but the partials: at most
+// two per CTA.  From four waves of units on, each is a CTA's own; from one wave on
+// too where the units differ in work anyway (a causal chunk as long as a good
+// part of its sequence; documents), since the dealing goes by length, and where
+// a unit has fewer than eight tiles.  A CTA takes at least kMinTiles tiles, below
+// which its set-up outweighs them.
 constexpr int kTcRows = 64;
+constexpr int kMinTiles = 2;
 
 // The accumulating form needs every score again once the denominators are
 // known.  Up to kLogitRows rows per KV head the bfloat16 kernel stores them
@@ -453,49 +565,37 @@ constexpr int kTcRows = 64;
 // rows and 128 channels 64 against 256); beyond, they are recomputed.
 constexpr int kLogitRows = 16;
 
-TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int head_dim, int seq_len, float scale,
-                 bool uneven, bool lse) {
+TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int head_dim, int seq_len, int draft_len,
+                 float scale, bool uneven, bool lse) {
   TokPlan p;
   const int G = q_heads / kv_heads;
   const int64_t R = (int64_t)q_len * G;
   p.tc = dtype == OC_BF16 && head_dim <= 128 && R > kTcRows && scale > 0.f;
-  int64_t units, slots = device_sm_count();
-  int step, setup;
+  int64_t slots = device_sm_count();
   if (p.tc) {
-    units = (int64_t)batch * kv_heads * tok_tc_shape(q_len, G).npairs;
-    p.row_tile = (int)R;
-    p.nrt = 1;
-    step = 128;
-    setup = 512;
+    p.row_tile = 128;
+    p.nrt = tok_tc_shape(q_len, G).npairs;
+    p.unit_rows = 256;
+    p.tile = 128;
   } else {
     p.row_tile = R <= 16 ? 16 : R <= 32 ? (dtype == OC_BF16 ? 32 : 16) : 64;
     p.nrt = (int)((R + p.row_tile - 1) / p.row_tile);
-    units = (int64_t)batch * kv_heads * p.nrt;
+    p.unit_rows = p.row_tile;
+    p.tile = dtype == OC_BF16 ? tok_mma_tile(head_dim) : kSimtTok;
     slots *= 2;
-    step = 64;
-    setup = dtype == OC_BF16 ? 160 : 32;
   }
-  int64_t most = seq_len / (2 * step);
-  if (most > 2 * slots / units + 4) most = 2 * slots / units + 4;
-  if (uneven && units >= slots) most = 1;
-  // partials: rows x head_dim floats written and read at about 6 TB/s, in keys of
-  // one CTA (the tcgen05 kernel takes 67 keys a microsecond, the others less)
-  const double part_keys = p.tc ? 256.0 * head_dim * 8 / 6e6 * 67 : 0.0;
-  double best = 0;
-  p.nchunk = 1;
-  p.chunk = seq_len < step ? step : (seq_len + step - 1) / step * step;
-  for (int64_t n = 1; n <= most; ++n) {
-    const int64_t keys = ((seq_len + n - 1) / n + step - 1) / step * step;
-    const double cost =
-        (double)((units * n + slots - 1) / slots) * (keys + (n > 1 ? setup : 0)) + (n > 1 ? units * n * part_keys : 0);
-    if (n == 1 || cost < best) {
-      best = cost;
-      p.chunk = (int)keys;
-      p.nchunk = (int)((seq_len + keys - 1) / keys);
-    }
-  }
-  if (p.nchunk < 1) p.nchunk = 1;
-  const size_t parts = p.nchunk > 1 ? (size_t)batch * kv_heads * p.nrt * p.nchunk * p.row_tile : 0;
+  p.units = (int64_t)batch * kv_heads * p.nrt;
+  const int64_t tiles = p.units * ((seq_len + p.tile - 1) / p.tile + (draft_len + p.tile - 1) / p.tile);
+  int64_t ncta = tiles / kMinTiles;
+  if (ncta > slots) ncta = slots;
+  if (ncta > kMergeMaxParts) ncta = kMergeMaxParts;
+  p.even = batch <= kMaxEvenBatch && (p.units < slots ? ncta > p.units
+                                      : !uneven && p.units < 4 * slots && tiles >= 8 * p.units);
+  p.hg = 1;
+  for (int g = 2; g <= 8; ++g)
+    if (kv_heads % g == 0 && g <= ncta) p.hg = g;
+  p.ncta = (int)(ncta < 1 ? 1 : ncta / p.hg * p.hg);
+  const size_t parts = p.even ? (size_t)2 * p.ncta * p.unit_rows : 0;
   size_t off = 0;
   p.lse_off = off;
   if (lse) off += up256((size_t)batch * kv_heads * R * sizeof(float));
@@ -526,7 +626,7 @@ int launch_simt(const TokArgs& a, cudaStream_t st) {
                                          (int)smem);
     if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_simt_kernel: %s", cudaGetErrorString(e));
   }
-  tok_simt_kernel<T, D, RPT><<<dim3((unsigned)(a.B * a.Hkv * a.nrt), (unsigned)a.nchunk), kSimtThreads, smem, st>>>(a);
+  tok_simt_kernel<T, D, RPT><<<a.even ? a.ncta : a.B * a.Hkv * a.nrt, kSimtThreads, smem, st>>>(a);
   return check_launch("tok_simt_kernel");
 }
 
@@ -601,18 +701,19 @@ int tok_common(const char* fn, TokArgs& a, const void* q, const void* k, const v
 int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void* workspace, size_t workspace_bytes,
             cudaStream_t st, const float* w_in = nullptr, float* w_out = nullptr) {
   const bool uneven = a.docs || (a.causal && a.Sq > a.S / 4);
-  const TokPlan p = tok_plan(dtype, a.B, a.Sq, a.Hq, a.Hkv, head_dim, a.S, a.scale, uneven, lse);
-  OC_REQUIRE((int64_t)a.B * a.Hkv * p.nchunk * (p.tc ? tok_tc_shape(a.Sq, a.G).npairs : p.nrt) < INT32_MAX &&
-                 p.nchunk <= 65535,
-             OC_ERR_SHAPE, "%s: too many work units", fn);
+  const TokPlan p = tok_plan(dtype, a.B, a.Sq, a.Hq, a.Hkv, head_dim, a.S, a.dk ? a.Sq : 0, a.scale, uneven, lse);
+  OC_REQUIRE(p.units < INT32_MAX, OC_ERR_SHAPE, "%s: too many work units", fn);
   OC_REQUIRE(workspace_bytes >= p.bytes, OC_ERR_CAPACITY, "%s: workspace %zu < %zu bytes", fn, workspace_bytes,
              p.bytes);
   OC_REQUIRE(p.bytes == 0 || (workspace && aligned16(workspace)), p.bytes && !workspace ? OC_ERR_NULL : OC_ERR_ALIGN,
              "%s: workspace must be a 16-byte aligned device pointer", fn);
   char* w = static_cast<char*>(workspace);
   a.nrt = p.nrt;
-  a.chunk = p.chunk;
-  a.nchunk = p.nchunk;
+  a.even = p.even;
+  a.ncta = p.ncta;
+  a.hg = p.hg;
+  a.tile = p.tile;
+  a.unit_rows = p.unit_rows;
   a.pm = reinterpret_cast<float*>(w + p.m_off);
   a.pl = reinterpret_cast<float*>(w + p.l_off);
   a.po = reinterpret_cast<float*>(w + p.o_off);
@@ -623,7 +724,7 @@ int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void*
            : dtype == OC_BF16 ? tok_mma(a, head_dim, p.row_tile, st)
                               : dispatch_simt<float>(a, head_dim, p.row_tile, st);
   if (rc) return rc;
-  if (p.nchunk > 1) rc = tok_merge(a, head_dim, p.row_tile, st);
+  if (p.even) rc = tok_merge(a, head_dim, p.tc, st);
   if (rc || !w_out || a.S == 0) return rc;
   // the column sums
   if (a.logits) {
@@ -650,9 +751,9 @@ extern "C" size_t oc_token_attention_workspace_bytes(int dtype, int batch, int q
     return 0;
   // the most that any call of these sizes needs
   size_t most = 0;
-  for (int i = 0; i < 4; ++i) {
-    const size_t n = tok_plan(dtype, batch, q_len, q_heads, kv_heads, head_dim, seq_len, i & 1 ? 1.f : 0.f, (i & 2) != 0,
-                              accumulate != 0).bytes;
+  for (int i = 0; i < 8; ++i) {
+    const size_t n = tok_plan(dtype, batch, q_len, q_heads, kv_heads, head_dim, seq_len, i & 4 ? q_len : 0,
+                              i & 1 ? 1.f : 0.f, (i & 2) != 0, accumulate != 0).bytes;
     if (n > most) most = n;
   }
   return most;

@@ -7,8 +7,8 @@
 // the warp-level m16n8k16 instructions; at 64 rows the two are about even, and
 // more rows go to the tcgen05 kernel (oc_token_tc.cu).
 //
-// Layout.  A CTA owns a tile of 16 WR rows of one (batch row, KV head) and one
-// chunk of the keys; its warps are WR row groups x WT token groups x WD
+// Layout.  A CTA works on a tile of 16 WR rows of one (batch row, KV head) and a
+// run of its keys at a time; its warps are WR row groups x WT token groups x WD
 // channel groups, so that every warp multiplies full 16-row fragments:
 //   * keys and values stream through shared memory in tiles of TOK tokens,
 //     STAGES deep, by 16-byte cp.async (it zero-fills the tokens nobody may
@@ -19,7 +19,7 @@
 //     bfloat16 (half a step, 2^-8 relative, of each weight; the row sums are
 //     taken before the rounding, in float32);
 //   * each warp keeps its own running maximum and sum; the WT token groups are
-//     joined once, at the end, in shared memory, and the chunks by
+//     joined once, at the end, in shared memory, and the runs by
 //     tok_merge_kernel.
 #include "oc_mma.cuh"
 #include "oc_token.cuh"
@@ -47,7 +47,7 @@ struct MmaShape {
   static constexpr int kJoin = WT * RT * D * 4;
   static constexpr int kQOff = kRing > kJoin ? kRing : kJoin;
   static constexpr int kTreeOff = kQOff + RT * D * 2;  // ancestor bits of the tile's rows, then the seen bits
-  static constexpr int kSmem = kTreeOff + (RT + 1) * (kMaxNodes / 32) * 4 + WT * RT * 2 * 4 + 64;
+  static constexpr int kSmem = kTreeOff + (RT + 1) * (kMaxNodes / 32) * 4 + WT * RT * 2 * 4 + 64 + (kMaxEvenBatch + 1) * 4;
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool real) {
@@ -73,11 +73,28 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int wd = warp % C::WD, wt = warp / C::WD % WT, wr = warp / C::WD / WT;
   const int g = lane >> 2, c2 = (lane & 3) * 2;
-  const int bh = blockIdx.x % (a.B * a.Hkv);
-  const int rt = a.nrt - 1 - blockIdx.x / (a.B * a.Hkv);  // the rows with most keys first
-  const int b = bh / a.Hkv, h = bh % a.Hkv, chunk = blockIdx.y;
+  int* pre = s_int + 16;
+  pdl_trigger();  // the merge may find its parts meanwhile
+  if (a.even) {
+    if (tid < 32) tok_prefix(a, pre);
+    __syncthreads();
+  }
+  TokWalk walk(a, pre, blockIdx.x);
+  TokSeg seg;
+  for (bool more = true; more;) {
+  if (a.even) {
+    if (!walk.next(a, pre, blockIdx.x, seg)) break;
+  } else {
+    // a CTA per unit, the rows with most keys first
+    const int u = blockIdx.x % (a.B * a.Hkv);
+    seg = TokSeg{u / a.Hkv, u % a.Hkv * a.nrt + a.nrt - 1 - (int)(blockIdx.x / (a.B * a.Hkv)), 0, INT32_MAX, -1};
+    more = false;
+  }
+  const int b = seg.b, h = seg.unit / a.nrt, rt = seg.unit % a.nrt, bh = b * a.Hkv + h;
   const int len = tok_len(a, b);
-  const bool has_draft = a.dk && chunk == a.nchunk - 1;
+  const int nct = (len + TOK - 1) / TOK;  // tiles of the cache; drafted tokens follow
+  const bool has_draft = a.dk && seg.t1 > nct;
+  __syncthreads();  // the previous piece is done with shared memory
 
   // queries of the tile (swizzled like the keys), first in the copy queue
   for (int e = tid; e < RT * CPR; e += THREADS) {
@@ -124,7 +141,7 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
     }
   }
   __syncthreads();
-  int t0 = chunk * a.chunk, t1 = min(s_int[0], t0 + a.chunk);
+  int t0 = min(seg.t0, nct) * TOK, t1 = min(s_int[0], min(seg.t1, nct) * TOK);
   const int min_hi = s_int[1];
   if (a.docs && t0 < t1) {  // the span of this chunk that holds any of the rows' documents
     const int d0 = s_int[2], d1 = s_int[3];
@@ -145,13 +162,14 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
     if (s_int[4] < t1) t0 = s_int[4] / TOK * TOK;
   }
   const int ncache = t1 > t0 ? (t1 - t0 + TOK - 1) / TOK : 0;
-  const int ntile = ncache + (has_draft ? (a.Sq + TOK - 1) / TOK : 0);
+  const int d0 = max(seg.t0 - nct, 0);  // first drafted tile
+  const int ntile = ncache + (has_draft ? min(seg.t1 - nct, (a.Sq + TOK - 1) / TOK) - d0 : 0);
 
   auto issue = [&](int t) {
     if (t < ntile) {
       const uint32_t slot = sbase + (t % ST) * 2 * C::kTileBytes;
       const bool draft = t >= ncache;
-      const int j0 = draft ? (t - ncache) * TOK : t0 + t * TOK;
+      const int j0 = draft ? (d0 + t - ncache) * TOK : t0 + t * TOK;
       const int64_t row0 = draft ? (int64_t)b * a.Sq + j0 : tok_kv_row(a, b, j0);  // a tile lies inside one page
       const __nv_bfloat16* kp = static_cast<const __nv_bfloat16*>(draft ? a.dk : a.k);
       const __nv_bfloat16* vp = static_cast<const __nv_bfloat16*>(draft ? a.dv : a.v);
@@ -195,7 +213,7 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
       for (int kk = 0; kk < KQ; ++kk) ldsm_x4(qf[kk], sbase + C::kQOff + swz<RT>(q_row, 2 * kk + q_c));
     }
     const bool draft = t >= ncache;
-    const int j0 = (draft ? (t - ncache) * TOK : t0 + t * TOK) + wt * C::TPW;
+    const int j0 = (draft ? (d0 + t - ncache) * TOK : t0 + t * TOK) + wt * C::TPW;
 
     // scores of this warp's tokens: B fragments are 8 tokens x 16 channels of
     // the keys as they lie
@@ -366,8 +384,8 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
       acc.z += f * ov.z;
       acc.w += f * ov.w;
     }
-    if (a.nchunk > 1) {
-      const int64_t part = ((int64_t)(bh * a.nrt + rt) * a.nchunk + chunk) * RT + rl;
+    if (seg.part >= 0) {
+      const int64_t part = (int64_t)seg.part * RT + rl;
       if (x == 0) {
         a.pm[part] = M;
         a.pl[part] = L;
@@ -385,6 +403,7 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
       *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) =
           make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
   }
+  }
 }
 
 template <int D, int WR>
@@ -395,7 +414,7 @@ int launch_mma(const TokArgs& a, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(tok_mma_kernel<D, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_mma_kernel: %s", cudaGetErrorString(e));
   }
-  tok_mma_kernel<D, WR><<<dim3((unsigned)(a.B * a.Hkv * a.nrt), (unsigned)a.nchunk), C::THREADS, C::kSmem, st>>>(a);
+  tok_mma_kernel<D, WR><<<a.even ? a.ncta : a.B * a.Hkv * a.nrt, C::THREADS, C::kSmem, st>>>(a);
   return check_launch("tok_mma_kernel");
 }
 
@@ -407,6 +426,8 @@ int launch_mma_rows(const TokArgs& a, int row_tile, cudaStream_t st) {
 }
 
 }  // namespace
+
+int tok_mma_tile(int head_dim) { return head_dim == 256 ? MmaTile<256>::kTok : MmaTile<128>::kTok; }
 
 int tok_mma(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st) {
   if (head_dim == 64) return launch_mma_rows<64>(a, row_tile, st);

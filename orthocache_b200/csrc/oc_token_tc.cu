@@ -75,12 +75,12 @@ struct TcSmem {
   uint64_t drain;
   uint32_t tmem_base;
   int abort;
+  int pre[kMaxEvenBatch + 1];
 };
 
 struct TcArgs {
   TokArgs t;
   int Gp, nhs, P, tiles, npairs, units;  // row tiles per (b, h): nhs head groups x position tiles of P
-  int chunk_tiles;
   const uint4* tree_bits;   // [(b, node)][2] ancestor bits; row T of each batch row: seen by any node
   const int2* key_docs;     // [(b, key tile)] least and largest document
   const int4* query_docs;   // [(b, position tile)] least, largest document; first key tile, last + 1
@@ -89,10 +89,12 @@ struct TcArgs {
 };
 
 struct TcUnit {
-  int b, h, bh, chunk, len;
+  int b, h, bh, len;
+  int part;            // -1: all of its keys
   int ntile;
   int p0[2], hs[2], min_hi[2];
   int jt0, ncache, n;  // first cache tile, cache tiles, all tiles
+  int d0;              // first drafted tile
 };
 
 // The k-th unit of this CTA.  Units are ordered by falling work and dealt out
@@ -101,15 +103,14 @@ __device__ __forceinline__ int tc_deal(int k) {
   return k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
-__device__ __forceinline__ TcUnit tc_unit(const TcArgs& x, int u) {
+__device__ __forceinline__ TcUnit tc_unit(const TcArgs& x, const TokSeg& seg) {
   const TokArgs& a = x.t;
   TcUnit w;
-  const int BH = a.B * a.Hkv;
-  w.bh = u % BH;
-  w.chunk = u / BH % a.nchunk;
-  const int pair = x.npairs - 1 - u / BH / a.nchunk;  // the rows with most keys first
-  w.b = w.bh / a.Hkv;
-  w.h = w.bh % a.Hkv;
+  const int pair = seg.unit % x.npairs;
+  w.b = seg.b;
+  w.h = seg.unit / x.npairs;
+  w.bh = w.b * a.Hkv + w.h;
+  w.part = seg.part;
   w.len = tok_len(a, w.b);
   w.ntile = 2 * pair + 1 < x.tiles ? 2 : 1;
   int first = INT32_MAX, last = 0, top = 0;
@@ -144,13 +145,37 @@ __device__ __forceinline__ TcUnit tc_unit(const TcArgs& x, int u) {
     }
     top = max(top, hi);
   }
-  const int c0 = w.chunk * x.chunk_tiles;
-  w.jt0 = max(first, c0);
-  w.ncache = max(0, min(last, c0 + x.chunk_tiles) - w.jt0);
-  if (first == INT32_MAX) w.ncache = 0;
-  w.n = w.ncache + (a.dk && w.chunk == a.nchunk - 1 ? (a.Sq + kTok - 1) / kTok : 0);
+  const int nct = (w.len + kTok - 1) / kTok;  // tiles of the cache; drafted tokens follow
+  if (first == INT32_MAX) first = last = 0;
+  w.jt0 = max(first, min(seg.t0, nct));
+  w.ncache = max(0, min(last, seg.t1) - w.jt0);
+  w.d0 = max(seg.t0 - nct, 0);
+  w.n = w.ncache + (a.dk && seg.t1 > nct ? min(seg.t1 - nct, (a.Sq + kTok - 1) / kTok) - w.d0 : 0);
   return w;
 }
+
+// This CTA's units in order: its run of the even cut, or whole units.
+struct TcWalk {
+  TokWalk even;
+  int k;
+  __device__ __forceinline__ TcWalk(const TcArgs& x, const int* pre) : even(x.t, pre, blockIdx.x), k(0) {}
+  __device__ __forceinline__ bool next(const TcArgs& x, const int* pre, TcUnit& w) {
+    TokSeg seg;
+    if (x.t.even) {
+      if (!even.next(x.t, pre, blockIdx.x, seg)) return false;
+    } else {
+      int u = x.units;
+      while (u >= x.units) {
+        if (k * (int)gridDim.x >= x.units) return false;
+        u = tc_deal(k++);
+      }
+      const int BH = x.t.B * x.t.Hkv, bh = u % BH;  // the rows with most keys first
+      seg = TokSeg{bh / x.t.Hkv, bh % x.t.Hkv * x.npairs + x.npairs - 1 - u / BH, 0, INT32_MAX, -1};
+    }
+    w = tc_unit(x, seg);
+    return true;
+  }
+};
 
 // First key row of cache tile jt in the (rows, Hkv, D) view; -1: no such page.
 __device__ __forceinline__ int tc_key_row(const TokArgs& a, int b, int jt) { return (int)tok_kv_row(a, b, jt * kTok); }
@@ -385,7 +410,7 @@ __device__ __forceinline__ void chunk_exp(const float* s, int c, uint32_t* pk, u
 __device__ __forceinline__ bool tc_dirty(const TcArgs& x, const TcUnit& w, int j) {
   const TokArgs& a = x.t;
   if (j >= w.ncache) {
-    const uint4 seen = x.tree_bits[((size_t)w.b * (a.Sq + 1) + a.Sq) * 2 + j - w.ncache];
+    const uint4 seen = x.tree_bits[((size_t)w.b * (a.Sq + 1) + a.Sq) * 2 + w.d0 + j - w.ncache];
     return (seen.x & seen.y & seen.z & seen.w) != ~0u;
   }
   const int jt = w.jt0 + j;
@@ -416,10 +441,9 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
   const float c_scale = a.scale * kLog2e;
   const CapFn cap(x);
   uint32_t s_ph = 0, o_ph = 0;
-  for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
-    const int u = tc_deal(k);
-    if (u >= x.units) continue;
-    const TcUnit w = tc_unit(x, u);
+  TcWalk walk(x, sm.pre);
+  TcUnit w;
+  while (walk.next(x, sm.pre, w)) {
     if (t >= w.ntile) continue;
     const int p0 = t ? w.p0[1] : w.p0[0], min_hi = t ? w.min_hi[1] : w.min_hi[0];
     const int pos_i = p0 + rl / x.Gp;  // query position of this row
@@ -430,15 +454,23 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
     if (a.docs) qd = x.query_docs[(size_t)w.b * x.npt + p0 / x.P];
     float m_used = CAP == 1 || !real ? 0.f : -INFINITY, l = 0.f;
     int level = 0;  // which of the cap's polynomials is in use
+    // what a tile's masking depends on, loaded a tile ahead
+    int2 kd = make_int2(0, 0);
+    bool no_page = false;
+    const auto look = [&](int j) {
+      if (j >= w.ncache) return;
+      if (a.docs) kd = x.key_docs[(size_t)w.b * x.nkt + w.jt0 + j];
+      if (a.table) no_page = tc_key_row(a, w.b, w.jt0 + j) < 0;
+    };
+    look(0);
     for (int j = 0; j < w.n; ++j) {
       // is every key of the tile visible to every row of it?
       const bool draft = j >= w.ncache;
-      const int jt = draft ? j - w.ncache : w.jt0 + j, j0 = jt * kTok;
-      bool part = draft || j0 + kTok > min_hi || (a.table && tc_key_row(a, w.b, jt) < 0);
-      if (a.docs && !draft) {
-        const int2 kd = x.key_docs[(size_t)w.b * x.nkt + jt];
-        part = part || kd.x < 0 || kd.x != kd.y || qd.x != kd.x || qd.y != kd.x;
-      }
+      const int jt = draft ? w.d0 + j - w.ncache : w.jt0 + j, j0 = jt * kTok;
+      const bool hole = no_page;
+      bool part = draft || j0 + kTok > min_hi || hole;
+      if (a.docs && !draft) part = part || kd.x < 0 || kd.x != kd.y || qd.x != kd.x || qd.y != kd.x;
+      look(j + 1);
       if (!bar_wait_warp(&sm.abort, &sm.s_full[t], s_ph)) return;
       s_ph ^= 1;
       tc_fence_after();
@@ -508,7 +540,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
             vis[2] = bits.z;
             vis[3] = bits.w;
           } else {
-            const int lim = a.table && tc_key_row(a, w.b, jt) < 0 ? 0 : row.hi - j0;
+            const int lim = hole ? 0 : row.hi - j0;
 #pragma unroll
             for (int y = 0; y < 4; ++y) vis[y] = lim >= 32 * y + 32 ? ~0u : lim <= 32 * y ? 0u : (1u << (lim - 32 * y)) - 1u;
             if (a.docs) {
@@ -567,10 +599,10 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
       tc_fence_after();
     }
     if (l == 0.f) m_used = -INFINITY;
-    const int64_t part = ((int64_t)w.bh * a.nchunk + w.chunk) * a.R + r;
+    const int64_t part = (int64_t)w.part * 256 + t * 128 + rl;
     const int64_t at = tok_q_offset(a, w.b, w.h, real ? r : 0, D);
     if (real) {
-      if (a.nchunk > 1) {
+      if (w.part >= 0) {
         a.pm[part] = m_used;
         a.pl[part] = l;
       } else if (a.lse) {
@@ -588,7 +620,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
         for (int i = 0; i < 32; ++i) o[i] = 0.f;
       }
       if (!real) continue;
-      if (a.nchunk > 1) {
+      if (w.part >= 0) {
         if (m_used != -INFINITY) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
@@ -628,10 +660,9 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
       mbar_wait(&sm.kv_full[s], ((L - s - 1) / C::kSlots) & 1);
     mbar_wait(&sm.q_full, q_ph ^ 1);
   };
-  for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
-    const int u = tc_deal(k);
-    if (u >= x.units) continue;
-    const TcUnit w = tc_unit(x, u);
+  TcWalk walk(x, sm.pre);
+  TcUnit w;
+  while (walk.next(x, sm.pre, w)) {
     if (w.n == 0) continue;
     if (!bar_wait(&sm.abort, &sm.q_empty, q_ph ^ 1)) return drain();
     q_ph ^= 1;
@@ -644,7 +675,7 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
           tma_load_3d(sm.q[t] + c * C::kBox, mq, &sm.q_full, 64 * c, w.h * a.G + w.hs[t] * x.Gp, w.b * a.Sq + w.p0[t]);
     for (int j = 0; j < w.n; ++j) {
       const bool draft = j >= w.ncache;
-      int key = draft ? w.b * a.Sq + (j - w.ncache) * kTok : tc_key_row(a, w.b, w.jt0 + j);
+      int key = draft ? w.b * a.Sq + (w.d0 + j - w.ncache) * kTok : tc_key_row(a, w.b, w.jt0 + j);
       if (key < 0) key = 0;  // a page outside the pool: loaded from page 0, masked and zeroed
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv, ++L) {
@@ -660,6 +691,11 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
   }
 }
 
+// Where padding, pages or drafted tokens make it a matter of memory reads whether
+// a tile is dirty, the cleaner passes every tile, and the issuing warp need not
+// know.
+__device__ __forceinline__ bool tc_look_always(const TokArgs& a) { return a.docs || a.table || a.dk; }
+
 // Zeros over the values of tokens that nobody may see, before the tensor cores
 // read the tile.  The warp looks at every load in order and takes part in the
 // release of its slot, so that it neither lags nor runs ahead of the ring.
@@ -669,18 +705,18 @@ __device__ void tc_cleaner(TcSmem<D>& sm, const TcArgs& x) {
   const TokArgs& a = x.t;
   const int lane = threadIdx.x & 31;
   uint32_t L = 0;
-  for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
-    const int u = tc_deal(k);
-    if (u >= x.units) continue;
-    const TcUnit w = tc_unit(x, u);
+  TcWalk walk(x, sm.pre);
+  TcUnit w;
+  while (walk.next(x, sm.pre, w)) {
     for (int j = 0; j < w.n; ++j, L += 2) {
       const uint32_t kslot = L % C::kSlots, slot = (L + 1) % C::kSlots;
       if (!bar_wait_warp(&sm.abort, &sm.kv_full[kslot], (L / C::kSlots) & 1)) return;
       if (lane == 0) mbar_arrive(&sm.kv_empty[kslot]);
       if (!bar_wait_warp(&sm.abort, &sm.kv_full[slot], ((L + 1) / C::kSlots) & 1)) return;
-      if (tc_dirty(x, w, j)) {
+      const bool dirty = tc_dirty(x, w, j);
+      if (dirty) {
         const bool draft = j >= w.ncache;
-        const int jt = draft ? j - w.ncache : w.jt0 + j, j0 = jt * kTok;
+        const int jt = draft ? w.d0 + j - w.ncache : w.jt0 + j, j0 = jt * kTok;
         const uint32_t* seen = reinterpret_cast<const uint32_t*>(x.tree_bits) + ((size_t)w.b * (a.Sq + 1) + a.Sq) * 8;
         const bool no_page = !draft && a.table && tc_key_row(a, w.b, jt) < 0;
         for (int it = 0; it < kTok / 4; ++it) {
@@ -694,9 +730,11 @@ __device__ void tc_cleaner(TcSmem<D>& sm, const TcArgs& x) {
         }
         fence_proxy_async();  // the tensor cores read through the async proxy
         __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.v_clean[slot]);
       }
-      if (lane == 0) mbar_arrive(&sm.kv_empty[slot]);
+      if (lane == 0) {
+        if (dirty || tc_look_always(a)) mbar_arrive(&sm.v_clean[slot]);
+        mbar_arrive(&sm.kv_empty[slot]);
+      }
     }
   }
 }
@@ -738,14 +776,13 @@ __device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
   tmem = __shfl_sync(0xffffffffu, tmem, 0);
   uint32_t q_ph = 0, p_ph[2] = {0, 0}, o_ph[2] = {1, 1}, clean_ph = 0;  // clean_ph: a bit per slot
   RingPos<D> kp;
-  for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
-    const int u = tc_deal(k);
-    if (u >= x.units) continue;
-    const TcUnit w = tc_unit(x, u);
+  TcWalk walk(x, sm.pre);
+  TcUnit w;
+  while (walk.next(x, sm.pre, w)) {
     const int n = __shfl_sync(0xffffffffu, w.n, 0), ntile = __shfl_sync(0xffffffffu, w.ntile, 0);
     if (n == 0) continue;
-    // first tile that may hold tokens nobody sees
-    const int dirty0 = x.t.docs || x.t.table || x.t.dk ? 0 : w.len / kTok - w.jt0;
+    // first tile whose values pass the cleaner
+    const int dirty0 = tc_look_always(x.t) ? 0 : w.len / kTok - w.jt0;
     if (!bar_wait_warp(&sm.abort, &sm.q_full, q_ph)) return;
     q_ph ^= 1;
     if (!bar_wait_warp(&sm.abort, &sm.kv_full[kp.slot], kp.ph)) return;
@@ -775,7 +812,7 @@ __device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
       kp.next();
       const uint64_t vd = vd0 + vp.slot * (C::kTileBytes >> 4), kd = kd0 + kp.slot * (C::kTileBytes >> 4);
       if (!bar_wait_warp(&sm.abort, &sm.kv_full[vp.slot], vp.ph)) return;
-      if (j > dirty0 && tc_dirty(x, w, j - 1)) {
+      if (j > dirty0) {
         if (!bar_wait_warp(&sm.abort, &sm.v_clean[vp.slot], (clean_ph >> vp.slot) & 1)) return;
         clean_ph ^= 1u << vp.slot;
       }
@@ -849,7 +886,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (x.t.even && warp == 0) tok_prefix(x.t, sm.pre);
   pdl_wait();
+  pdl_trigger();  // the merge may find its parts meanwhile
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -1256,7 +1295,7 @@ int launch_tc(const CUtensorMap (&m)[5], const TcArgs& x, cudaStream_t st) {
     if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_tc_kernel: %s", cudaGetErrorString(e));
   }
   const int sms = device_sm_count();
-  const dim3 grid((unsigned)(x.units < sms ? x.units : sms));
+  const dim3 grid((unsigned)(x.t.even ? x.t.ncta : x.units < sms ? x.units : sms));
   cudaError_t e;
   if (x.tree_bits || x.query_docs) {
     e = launch_pdl(kern, grid, dim3(kThreads), smem, st, m[0], m[1], m[2], m[3], m[4], x);
@@ -1306,8 +1345,7 @@ int tok_tc(const char* fn, const TokArgs& a, int head_dim, void* prep, cudaStrea
   x.P = s.P;
   x.tiles = s.npt * s.nhs;
   x.npairs = s.npairs;
-  x.units = a.B * a.Hkv * s.npairs * a.nchunk;
-  x.chunk_tiles = a.chunk / kTok;
+  x.units = a.B * a.Hkv * s.npairs;
   x.nkt = (a.S + kTok - 1) / kTok;
   x.npt = s.npt;
   x.k_in = a.cap > 0.f ? a.scale / a.cap : 0.f;
