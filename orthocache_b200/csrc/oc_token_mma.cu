@@ -165,25 +165,44 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
   const int d0 = max(seg.t0 - nct, 0);  // first drafted tile
   const int ntile = ncache + (has_draft ? min(seg.t1 - nct, (a.Sq + TOK - 1) / TOK) - d0 : 0);
 
+  // this thread's 16-byte column and rows r0, r0 + kStep, ... of a tile
+  constexpr int kStep = THREADS / CPR;
+  const int c_mine = tid % CPR, r0 = tid / CPR;
+  const int64_t row_bytes = (int64_t)a.Hkv * D * 2;
   auto issue = [&](int t) {
     if (t < ntile) {
       const uint32_t slot = sbase + (t % ST) * 2 * C::kTileBytes;
       const bool draft = t >= ncache;
       const int j0 = draft ? (d0 + t - ncache) * TOK : t0 + t * TOK;
       const int64_t row0 = draft ? (int64_t)b * a.Sq + j0 : tok_kv_row(a, b, j0);  // a tile lies inside one page
-      const __nv_bfloat16* kp = static_cast<const __nv_bfloat16*>(draft ? a.dk : a.k);
-      const __nv_bfloat16* vp = static_cast<const __nv_bfloat16*>(draft ? a.dv : a.v);
-      for (int e = tid; e < TOK * CPR; e += THREADS) {
-        const int r = e / CPR, c = e % CPR, j = j0 + r;
-        bool real;
-        if (draft)
-          real = j < a.Sq && (seen_bits[j >> 5] >> (j & 31) & 1);
-        else
-          real = j < len && row0 >= 0 && (!a.docs || a.docs[(size_t)b * a.S + j] >= 0);
-        const int64_t at = real ? ((row0 + r) * a.Hkv + h) * D + c * 8 : 0;
-        const uint32_t off = swz<TOK>(r, c);
-        cp16(slot + off, (real ? kp : static_cast<const __nv_bfloat16*>(a.q)) + at, real);
-        cp16(slot + C::kTileBytes + off, (real ? vp : static_cast<const __nv_bfloat16*>(a.q)) + at, real);
+      const char* kp = static_cast<const char*>(draft ? a.dk : a.k);
+      const char* vp = static_cast<const char*>(draft ? a.dv : a.v);
+      const int64_t off0 = (row0 + r0) * row_bytes + (h * D + c_mine * 8) * 2;
+      if (!draft && !a.docs && row0 >= 0 && j0 + TOK <= len) {
+        kp += off0;
+        vp += off0;
+#pragma unroll
+        for (int i = 0; i < TOK / kStep; ++i) {
+          const uint32_t dst = slot + swz<TOK>(r0 + i * kStep, c_mine);
+          cp16(dst, kp, true);
+          cp16(dst + C::kTileBytes, vp, true);
+          kp += kStep * row_bytes;
+          vp += kStep * row_bytes;
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < TOK / kStep; ++i) {
+          const int r = r0 + i * kStep, j = j0 + r;
+          bool real;
+          if (draft)
+            real = j < a.Sq && (seen_bits[j >> 5] >> (j & 31) & 1);
+          else
+            real = j < len && row0 >= 0 && (!a.docs || a.docs[(size_t)b * a.S + j] >= 0);
+          const int64_t at = off0 + i * kStep * row_bytes;
+          const uint32_t dst = slot + swz<TOK>(r, c_mine);
+          cp16(dst, real ? kp + at : static_cast<const char*>(a.q), real);
+          cp16(dst + C::kTileBytes, real ? vp + at : static_cast<const char*>(a.q), real);
+        }
       }
     }
     cp_commit();

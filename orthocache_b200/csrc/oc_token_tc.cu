@@ -609,34 +609,53 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
         a.lse[(int64_t)w.bh * a.R + r] = l == 0.f ? INFINITY : m_used + log2f(l);
       }
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    if (w.part >= 0) {
+      // float32 rows leave in the accumulator layout: four lanes write 32 bytes of
+      // a row (a thread writing its own row 16 bytes at a time takes 32 sectors an
+      // instruction)
+      const int64_t base = (int64_t)w.part * 256 + t * 128 + (threadIdx.x & 96);
 #pragma unroll 1
-    for (int c = 0; c < D / 32; ++c) {
-      float o[32];
-      if (w.n > 0) {
-        tmem_ld32_wait(t_o + 32 * c, o);
-      } else {
+      for (int half = 0; half < 2; ++half) {
+        const int g = half * 16 + (lane >> 2);
+        const bool put0 = __shfl_sync(0xffffffffu, real && m_used != -INFINITY, g);
+        const bool put1 = __shfl_sync(0xffffffffu, real && m_used != -INFINITY, g + 8);
+        if (w.n == 0) continue;
+#pragma unroll 1
+        for (int c = 0; c < D / 64; ++c) {
+          float o[32];
+          tmem_frag64_wait(t_o + ((uint32_t)(half * 16) << 16) + 64 * c, o);
+          float* dst = a.po + (base + g) * D + 64 * c + 2 * (lane & 3);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0.f;
+          for (int n = 0; n < 8; ++n) {
+            if (put0) *reinterpret_cast<float2*>(dst + 8 * n) = make_float2(o[4 * n], o[4 * n + 1]);
+            if (put1) *reinterpret_cast<float2*>(dst + 8 * D + 8 * n) = make_float2(o[4 * n + 2], o[4 * n + 3]);
+          }
+        }
       }
-      if (!real) continue;
-      if (w.part >= 0) {
-        if (m_used != -INFINITY) {
+    } else {
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        float o[32];
+        if (w.n > 0) {
+          tmem_ld32_wait(t_o + 32 * c, o);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        }
+        if (!real) continue;
+        if (a.out_dtype == OC_BF16) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + at + 32 * c + i) =
+                make_uint4(pack_bf16x2(o[i] * inv, o[i + 1] * inv), pack_bf16x2(o[i + 2] * inv, o[i + 3] * inv),
+                           pack_bf16x2(o[i + 4] * inv, o[i + 5] * inv), pack_bf16x2(o[i + 6] * inv, o[i + 7] * inv));
+        } else {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(a.po + part * D + 32 * c + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at + 32 * c + i) =
+                make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
         }
-      } else if (a.out_dtype == OC_BF16) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 8)
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + at + 32 * c + i) =
-              make_uint4(pack_bf16x2(o[i] * inv, o[i + 1] * inv), pack_bf16x2(o[i + 2] * inv, o[i + 3] * inv),
-                         pack_bf16x2(o[i + 4] * inv, o[i + 5] * inv), pack_bf16x2(o[i + 6] * inv, o[i + 7] * inv));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; i += 4)
-          *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at + 32 * c + i) =
-              make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
       }
     }
     if (w.n > 0) {
