@@ -143,6 +143,14 @@ __device__ __forceinline__ void tmem_wait32(float* v) {
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
 // 64 fp32 columns of 16 lanes (rows) in the layout of an m16n8 accumulator:
 // v[4 n + 2 i + e] is row lane / 4 + 8 i, column 8 n + 2 (lane % 4) + e, n < 8.
 // The lane field of taddr is 32 (warp % 4) or 16 more.  Loaded and waited for

@@ -128,36 +128,45 @@ struct TokSeg {
   int part;             // -1: the whole unit
 };
 
-// Runs of one head of a group: no more than there are tiles, so that none is
-// empty.
-__device__ __forceinline__ int tok_runs(const TokArgs& a, int64_t total) {
-  const int n = a.ncta / a.hg;
-  return total < n ? (total > 0 ? (int)total : 1) : n;
-}
+// The cut of `total` tiles into n runs: the first `rem` have one tile more.  (All
+// in 32 bits: a 64-bit division costs a CTA's set-up a microsecond.)
+struct TokCut {
+  int n, q, rem;
+  __device__ __forceinline__ TokCut(const TokArgs& a, int total) {
+    n = a.ncta / a.hg;
+    if (n > total) n = total > 0 ? total : 1;  // none is empty
+    q = (int)((unsigned)total / (unsigned)n);
+    rem = total - q * n;
+  }
+  __device__ __forceinline__ int first(int i) const { return i * q + min(i, rem); }  // first tile of run i
+  __device__ __forceinline__ int run(int t) const {                                  // run of tile t
+    const int big = rem * (q + 1);
+    return t < big ? (int)((unsigned)t / (unsigned)(q + 1)) : rem + (int)((unsigned)(t - big) / (unsigned)q);
+  }
+};
 
 struct TokWalk {
-  int64_t x, lo, hi;
-  int b;
+  int x, lo, hi, b;
   __device__ __forceinline__ TokWalk(const TokArgs& a, const int* pre, int cta) {
-    const int64_t total = a.even ? (int64_t)(a.Hkv / a.hg) * a.nrt * pre[a.B] : 0;
-    const int n = tok_runs(a, total), i = cta / a.hg;
-    lo = i < n ? total * i / n : 0;
-    hi = i < n ? total * (i + 1) / n : 0;
+    const int total = a.even ? a.Hkv / a.hg * a.nrt * pre[a.B] : 0;
+    const TokCut cut(a, total);
+    const int i = cta / a.hg;
+    lo = i < cut.n ? cut.first(i) : 0;
+    hi = i < cut.n && total ? cut.first(i + 1) : 0;
     x = lo;
     b = 0;
   }
   __device__ __forceinline__ bool next(const TokArgs& a, const int* pre, int cta, TokSeg& s) {
     if (x >= hi) return false;
-    const int64_t upb = (int64_t)(a.Hkv / a.hg) * a.nrt;
+    const int upb = a.Hkv / a.hg * a.nrt;
     while (x >= upb * pre[b + 1]) ++b;
-    const int64_t rel = x - upb * pre[b];
-    const int nt = pre[b + 1] - pre[b];
-    const int u = (int)(rel / nt);  // head group * nrt + row tile
+    const int rel = x - upb * pre[b], nt = pre[b + 1] - pre[b];
+    const int u = (int)((unsigned)rel / (unsigned)nt);  // head group * nrt + row tile
+    const int hgroup = a.nrt == 1 ? u : u / a.nrt;
     s.b = b;
-    s.unit = (u / a.nrt * a.hg + cta % a.hg) * a.nrt + u % a.nrt;
-    s.t0 = (int)(rel % nt);
-    const int64_t left = hi - x;
-    s.t1 = left < nt - s.t0 ? s.t0 + (int)left : nt;
+    s.unit = (hgroup * a.hg + cta % a.hg) * a.nrt + u - hgroup * a.nrt;
+    s.t0 = rel - u * nt;
+    s.t1 = min(nt, s.t0 + hi - x);
     s.part = s.t0 == 0 && s.t1 == nt ? -1 : 2 * cta + (x == lo ? 0 : 1);
     x += s.t1 - s.t0;
     return true;

@@ -272,8 +272,7 @@ template <int D, int WPR>
 __global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs a, const TokTcShape tc, int blocks_per_unit) {
   __shared__ int s_part[kMergeMaxParts];
   __shared__ int s_tiles[3];  // tiles of a unit: of the rows before b, of all rows, of row b
-  __shared__ int s_c[2];
-  __shared__ float s_l[8], s_o[WPR > 1 ? 8 : 1][D];
+  __shared__ float s_m[8], s_l[8], s_o[WPR > 1 ? 8 : 1][D];
   const int unit = blockIdx.x / blocks_per_unit, block = blockIdx.x % blocks_per_unit;
   const int upb = a.Hkv * a.nrt, b = unit / upb, h = unit % upb / a.nrt, rt = unit % a.nrt;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -295,16 +294,13 @@ __global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs 
     }
   }
   __syncthreads();
-  const int64_t upg = (int64_t)(a.Hkv / a.hg) * a.nrt, total = upg * s_tiles[1];
-  const int64_t start = upg * s_tiles[0] + (int64_t)(h / a.hg * a.nrt + rt) * s_tiles[2], end = start + s_tiles[2];
-  const int n = tok_runs(a, total);
-  if (tid < 2)  // the runs [total i / n, total (i + 1) / n) that hold its first and last tile
-    s_c[tid] = (int)(((tid ? end : start + 1) * n - 1) / total);
-  __syncthreads();
-  const int c0 = s_c[0], parts = s_c[1] - c0 + 1;
+  const int upg = a.Hkv / a.hg * a.nrt;
+  const int start = upg * s_tiles[0] + (h / a.hg * a.nrt + rt) * s_tiles[2];
+  const TokCut cut(a, upg * s_tiles[1]);
+  const int c0 = cut.run(start), parts = cut.run(start + s_tiles[2] - 1) - c0 + 1;
   if (parts <= 1) return;
-  for (int c = tid; c < parts; c += kMergeThreads) 
-    s_part[c] = 2 * ((c0 + c) * a.hg + h % a.hg) + (total * (c0 + c) / n >= start ? 0 : 1);
+  for (int c = tid; c < parts; c += kMergeThreads)
+    s_part[c] = 2 * ((c0 + c) * a.hg + h % a.hg) + (cut.first(c0 + c) >= start ? 0 : 1);
   __syncthreads();
   pdl_wait();
 
@@ -324,32 +320,44 @@ __global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs 
       real = real && r < a.R;
     }
     if (!real) continue;  // with WPR > 1 the same for the whole block
-    float M = -INFINITY;
-    for (int c = lane; c < parts; c += 32) M = fmaxf(M, a.pm[(int64_t)s_part[c] * rows + rl]);
-    M = warp_max(M);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float o[D / 32], L = 0.f;
+    float M = -INFINITY, o[D / 32], L = 0.f;
 #pragma unroll
     for (int x = 0; x < D / 32; ++x) o[x] = 0.f;
-#pragma unroll 4
-    for (int c = WPR > 1 ? warp : 0; c < parts; c += WPR) {
-      const int64_t part = (int64_t)s_part[c] * rows + rl;
-      const float mc = a.pm[part], lc = a.pl[part];
-      const bool any = mc != -INFINITY;
-      const float w = any ? exp2f(mc - ref) : 1.f;
-      L += w * lc;  // of a part without keys 0, or NaN when every visible score was NaN
-      if (any) {
+    // four parts at a time, everything of them requested at once
+    for (int c = WPR > 1 ? warp : 0; c < parts; c += 4 * WPR) {
+      float mc[4], lc[4], v[4][D / 32];
 #pragma unroll
-        for (int x = 0; x < kN; ++x) {
-          float v[kV];
-          const float* src = a.po + part * D + x * 32 * kV + lane * kV;
-          if (kV == 4)
-            *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-          else
-            *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+      for (int z = 0; z < 4; ++z) {
+        mc[z] = -INFINITY;
+        lc[z] = 0.f;
+        if (c + z * WPR < parts) {
+          const int64_t part = (int64_t)s_part[c + z * WPR] * rows + rl;
+          mc[z] = a.pm[part];
+          lc[z] = a.pl[part];
 #pragma unroll
-          for (int y = 0; y < kV; ++y) o[x * kV + y] += w * v[y];
+          for (int x = 0; x < kN; ++x) {
+            const float* src = a.po + part * D + x * 32 * kV + lane * kV;
+            if (kV == 4)
+              *reinterpret_cast<float4*>(&v[z][x * kV]) = *reinterpret_cast<const float4*>(src);
+            else
+              *reinterpret_cast<float2*>(&v[z][x * kV]) = *reinterpret_cast<const float2*>(src);
+          }
         }
+      }
+      const float m_new = fmaxf(M, fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])));
+      const float ref = m_new == -INFINITY ? 0.f : m_new, old = exp2f(M - ref);
+      L *= old;
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) o[x] *= old;
+      M = m_new;
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        const bool any = mc[z] != -INFINITY;  // else nothing was written but l: 0, or NaN when all its scores were
+        const float w = any ? exp2f(mc[z] - ref) : 1.f;
+        L += w * lc[z];
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+          if (any) o[x] = fmaf(w, v[z][x], o[x]);
       }
     }
     if (WPR > 1) {  // add up the eight warps
@@ -358,16 +366,23 @@ __global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs 
       for (int x = 0; x < kN; ++x)
 #pragma unroll
         for (int y = 0; y < kV; ++y) s_o[warp][x * 32 * kV + lane * kV + y] = o[x * kV + y];
-      if (lane == 0) s_l[warp] = L;
+      if (lane == 0) {
+        s_m[warp] = M;
+        s_l[warp] = L;
+      }
       __syncthreads();
       if (tid < D / 4) {
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
         L = 0.f;
+        M = s_m[0];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) M = fmaxf(M, s_m[w]);
 #pragma unroll
         for (int w = 0; w < 8; ++w) {
-          L += s_l[w];
+          const float f = s_m[w] == -INFINITY ? 1.f : exp2f(s_m[w] - M);
+          L += f * s_l[w];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) acc[y] += s_o[w][4 * tid + y];
+          for (int y = 0; y < 4; ++y) acc[y] += f * s_o[w][4 * tid + y];
         }
         if (a.lse && tid == 0) a.lse[(int64_t)(b * a.Hkv + h) * a.R + r] = L == 0.f ? INFINITY : M + log2f(L);
         const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
@@ -406,8 +421,12 @@ int launch_merge(const TokArgs& a, const TokTcShape& tc, cudaStream_t st) {
   const int units = a.B * a.Hkv * a.nrt;
   // rows of a unit that exist at most, and whether all rows together are few
   const int rows = a.R < a.unit_rows ? a.R : a.unit_rows;
-  const bool few = (int64_t)units * rows <= 4096;
-  const int bpu = few ? rows : (rows + 31) / 32;
+  const bool few = (int64_t)units * rows <= 1184;
+  int bpu = rows;
+  if (!few) {  // about eight blocks per SM, at least a row per warp
+    bpu = (1184 + units - 1) / units;
+    if (bpu > (a.unit_rows + 7) / 8) bpu = (a.unit_rows + 7) / 8;
+  }
   cudaError_t e = few ? launch_pdl(tok_merge_kernel<D, 8>, dim3(units * bpu), dim3(kMergeThreads), 0, st, a, tc, bpu)
                       : launch_pdl(tok_merge_kernel<D, 1>, dim3(units * bpu), dim3(kMergeThreads), 0, st, a, tc, bpu);
   if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_merge_kernel: %s", cudaGetErrorString(e));
@@ -589,7 +608,7 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
   int64_t ncta = tiles / kMinTiles;
   if (ncta > slots) ncta = slots;
   if (ncta > kMergeMaxParts) ncta = kMergeMaxParts;
-  p.even = batch <= kMaxEvenBatch && (p.units < slots ? ncta > p.units
+  p.even = batch <= kMaxEvenBatch && tiles < (1 << 30) && (p.units < slots ? ncta > p.units
                                       : !uneven && p.units < 4 * slots && tiles >= 8 * p.units);
   p.hg = 1;
   for (int g = 2; g <= 8; ++g)

@@ -301,19 +301,6 @@ __device__ __forceinline__ bool cap_far(const float* s, float k_in) {
   return __any_sync(0xffffffffu, !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * k_in <= kCapPoly3));
 }
 
-__device__ __forceinline__ float row_max(const float* s) {
-  float m8[8];  // independent chains
-#pragma unroll
-  for (int k = 0; k < 8; ++k) m8[k] = s[k];
-#pragma unroll
-  for (int i = 8; i < 120; i += 16)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) m8[k] = max3(m8[k], s[i + k], s[i + 8 + k]);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) m8[k] = fmaxf(m8[k], s[120 + k]);
-  return fmaxf(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], max3(m8[5], m8[6], m8[7])));
-}
-
 // 2^x of a pair on the FMA pipe, for x >= -126 or clamped there: x = n + f, n =
 // floor(x) by adding 1.5 * 2^23 with rounding toward -inf (its low bits are then
 // n), 2^f on [0, 1) a least-squares polynomial of degree 4 with equalised
@@ -340,31 +327,6 @@ __device__ __forceinline__ uint64_t poly_ex2(uint64_t x) {
   up2(t, t0, t1);
   return mul2(p, pk2(__uint_as_float(__float_as_uint(t0) * (1u << 23) + 0x3f800000u),
                      __uint_as_float(__float_as_uint(t1) * (1u << 23) + 0x3f800000u)));
-}
-
-// P = 2^(score - m) of 128 masked scores in log2 units as bfloat16 pairs over the
-// scores in tensor memory; returns their sum.
-__device__ __forceinline__ float exp_pack(const float* s, uint32_t t_s, float m) {
-  uint64_t r2[4] = {0, 0, 0, 0};
-  const uint64_t nm2 = pk2(-m, -m);
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    uint32_t pk[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      float e0, e1;
-      up2(add2(pk2(s[64 * half + 2 * i], s[64 * half + 2 * i + 1]), nm2), e0, e1);
-      e0 = ex2(e0);
-      e1 = ex2(e1);
-      r2[i & 3] = add2(r2[i & 3], pk2(e0, e1));
-      pk[i] = pack_bf16x2(e0, e1);
-    }
-    tmem_st32u(t_s + 32 * half, pk);
-  }
-  float q[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) up2(r2[i], q[2 * i], q[2 * i + 1]);
-  return ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
 }
 
 // 2^(score - m) of 32 scores (columns 32 c ..) as bfloat16 pairs, and their sums;
@@ -511,64 +473,79 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
         }
       }
       if (!done) {
-        float s[128];
-        tmem_ld128_wait(t_s, s);
-        // scores in log2 units, biased and masked, in place
-        if (CAP) {
-          if (cap_far<128>(s, x.k_in)) {
+        // which of the 128 keys the row sees, a bit each
+        uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+        if (part && draft) {
+          const uint4 bits = real ? x.tree_bits[((size_t)w.b * (a.Sq + 1) + pos_i) * 2 + jt] : make_uint4(0, 0, 0, 0);
+          vis[0] = bits.x;
+          vis[1] = bits.y;
+          vis[2] = bits.z;
+          vis[3] = bits.w;
+        } else if (part) {
+          const int lim = hole ? 0 : row.hi - j0;
 #pragma unroll
-            for (int i = 0; i < 128; ++i) s[i] = cap.exact(s[i]);
-          } else {
+          for (int y = 0; y < 4; ++y) vis[y] = lim >= 32 * y + 32 ? ~0u : lim <= 32 * y ? 0u : (1u << (lim - 32 * y)) - 1u;
+          if (a.docs) {
+            // one round per document among the warp's rows
+            int d[4];
 #pragma unroll
-            for (int i = 0; i < 128; i += 2) up2(cap.poly2<3>(pk2(s[i], s[i + 1]), 0), s[i], s[i + 1]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 128; ++i) s[i] *= c_scale;
-        }
-        if (BIAS) {
-#pragma unroll
-          for (int i = 0; i < 128; ++i) s[i] = fmaf(-row.slope2, fabsf(d0 - (float)i), s[i]);
-        }
-        if (part) {
-          // which of the 128 keys the row sees, a bit each
-          uint32_t vis[4];
-          if (draft) {
-            const uint4 bits = real ? x.tree_bits[((size_t)w.b * (a.Sq + 1) + pos_i) * 2 + jt] : make_uint4(0, 0, 0, 0);
-            vis[0] = bits.x;
-            vis[1] = bits.y;
-            vis[2] = bits.z;
-            vis[3] = bits.w;
-          } else {
-            const int lim = hole ? 0 : row.hi - j0;
-#pragma unroll
-            for (int y = 0; y < 4; ++y) vis[y] = lim >= 32 * y + 32 ? ~0u : lim <= 32 * y ? 0u : (1u << (lim - 32 * y)) - 1u;
-            if (a.docs) {
-              // one round per document among the warp's rows
-              int d[4];
+            for (int y = 0; y < 4; ++y) {
+              const int jj = j0 + 32 * y + lane;
+              d[y] = jj < a.S ? a.docs[(size_t)w.b * a.S + jj] : -1;
+            }
+            uint32_t todo = ~0u;
+            while (todo) {
+              const int doc = __shfl_sync(0xffffffffu, row.doc, __ffs(todo) - 1);
 #pragma unroll
               for (int y = 0; y < 4; ++y) {
-                const int jj = j0 + 32 * y + lane;
-                d[y] = jj < a.S ? a.docs[(size_t)w.b * a.S + jj] : -1;
+                const uint32_t same = __ballot_sync(0xffffffffu, d[y] == doc);
+                if (row.doc == doc) vis[y] &= same;
               }
-              uint32_t todo = ~0u;
-              while (todo) {
-                const int doc = __shfl_sync(0xffffffffu, row.doc, __ffs(todo) - 1);
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                  const uint32_t same = __ballot_sync(0xffffffffu, d[y] == doc);
-                  if (row.doc == doc) vis[y] &= same;
-                }
-                todo &= ~__ballot_sync(0xffffffffu, row.doc == doc);
-              }
+              todo &= ~__ballot_sync(0xffffffffu, row.doc == doc);
             }
           }
-#pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (!(vis[i >> 5] >> (i & 31) & 1)) s[i] = -INFINITY;
         }
+        // 32 scores in log2 units, biased and masked.  They are read from tensor
+        // memory once for the maximum and once for the exponentials: the code stays
+        // a quarter as long (a CTA's first tile comes this way, with cold
+        // instruction caches)
+        const auto scores = [&](int c, float (&s)[32]) {
+          tmem_ld32_wait(t_s + 32 * c, s);
+          if (CAP) {
+            if (cap_far<32>(s, x.k_in)) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s[i] = cap.exact(s[i]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) up2(cap.poly2<3>(pk2(s[i], s[i + 1]), 0), s[i], s[i + 1]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[i] *= c_scale;
+          }
+          if (BIAS) {
+            const float dc = d0 - (float)(32 * c);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[i] = fmaf(-row.slope2, fabsf(dc - (float)i), s[i]);
+          }
+          const uint32_t word = c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(word >> i & 1)) s[i] = -INFINITY;
+        };
         if (CAP != 1) {
-          const float mx = row_max(s);
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float s[32];
+            scores(c, s);
+            float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+#pragma unroll
+              for (int y = 0; y < 4; ++y) m4[y] = max3(m4[y], s[i + y], s[i + 4 + y]);
+            mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
+          }
           const bool need = mx > m_used + 8.f;
           if (__any_sync(0xffffffffu, need)) {
             const float alpha = need ? ex2(m_used - mx) : 1.f;  // 0 on a row's first visible tile
@@ -586,7 +563,22 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
             if (need) m_used = mx;
           }
         }
-        l += exp_pack(s, t_s, m_used == -INFINITY ? 0.f : m_used);
+        const float base = m_used == -INFINITY ? 0.f : m_used;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {  // P of 32 keys takes 16 columns, behind the scores still to be read
+          float s[32];
+          uint32_t pk[16];
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          scores(c, s);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float e0 = ex2(s[2 * i] - base), e1 = ex2(s[2 * i + 1] - base);
+            sum[i & 3] += e0 + e1;
+            pk[i] = pack_bf16x2(e0, e1);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st16u(t_s + 16 * c, pk);
+        }
       }
       tc_wait_st();
       tc_fence_before();
