@@ -299,13 +299,18 @@ __global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs 
   const TokCut cut(a, upg * s_tiles[1]);
   const int c0 = cut.run(start), parts = cut.run(start + s_tiles[2] - 1) - c0 + 1;
   if (parts <= 1) return;
-  for (int c = tid; c < parts; c += kMergeThreads)
-    s_part[c] = 2 * ((c0 + c) * a.hg + h % a.hg) + (cut.first(c0 + c) >= start ? 0 : 1);
+  // a unit of one row tile has two partials of 128 rows a piece (both halves of its
+  // CTA worked on it)
+  const int sub = tc.Gp && tc.npt * tc.nhs == 1 ? 2 : 1, nparts = parts * sub;
+  for (int e = tid; e < nparts; e += kMergeThreads) {
+    const int c = c0 + e / sub;
+    s_part[e] = (2 * (c * a.hg + h % a.hg) + (cut.first(c) >= start ? 0 : 1)) * sub + e % sub;
+  }
   __syncthreads();
   pdl_wait();
 
   constexpr int kV = D < 128 ? 2 : 4, kN = D / 32 / kV, kRows = 8 / WPR;  // rows of a block at a time
-  const int rows = a.unit_rows;
+  const int rows = a.unit_rows / sub;
   for (int r0 = block * kRows; r0 < rows; r0 += blocks_per_unit * kRows) {
     const int rl = r0 + (WPR > 1 ? 0 : warp);
     // query row of local row rl of the unit
@@ -324,13 +329,13 @@ __global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs 
 #pragma unroll
     for (int x = 0; x < D / 32; ++x) o[x] = 0.f;
     // four parts at a time, everything of them requested at once
-    for (int c = WPR > 1 ? warp : 0; c < parts; c += 4 * WPR) {
+    for (int c = WPR > 1 ? warp : 0; c < nparts; c += 4 * WPR) {
       float mc[4], lc[4], v[4][D / 32];
 #pragma unroll
       for (int z = 0; z < 4; ++z) {
         mc[z] = -INFINITY;
         lc[z] = 0.f;
-        if (c + z * WPR < parts) {
+        if (c + z * WPR < nparts) {
           const int64_t part = (int64_t)s_part[c + z * WPR] * rows + rl;
           mc[z] = a.pm[part];
           lc[z] = a.pl[part];
@@ -564,8 +569,10 @@ struct TokPlan {
 inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 // Kernel: float32 takes the float32-arithmetic kernel (row tiles of 16 or 64);
-// bfloat16 the m16n8k16 kernel (16, 32 or 64 rows, what the rows fill) or, for
-// more than kTcRows rows per KV head at head_dim 64 and 128, the tcgen05 one.
+// bfloat16 the m16n8k16 kernel (16, 32 or 64 rows, what the rows fill) or the
+// tcgen05 one, from the rows on where it is the faster (a tree over 64K tokens, 8
+// KV heads: at 128 channels 32 rows take 69 and 77 us, 64 rows 108 and 77; at 64
+// channels 48 rows 54 and 56, 96 rows 75 and 58).
 //
 // Cut: with few units (row tile, batch row, KV head) for the GPU, all their key
 // tiles are dealt out evenly over one (tcgen05) or two CTAs per SM, so that
@@ -575,7 +582,6 @@ inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // part of its sequence; documents), since the dealing goes by length, and where
 // a unit has fewer than eight tiles.  A CTA takes at least kMinTiles tiles, below
 // which its set-up outweighs them.
-constexpr int kTcRows = 64;
 constexpr int kMinTiles = 2;
 
 // The accumulating form needs every score again once the denominators are
@@ -589,7 +595,7 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
   TokPlan p;
   const int G = q_heads / kv_heads;
   const int64_t R = (int64_t)q_len * G;
-  p.tc = dtype == OC_BF16 && head_dim <= 128 && R > kTcRows && scale > 0.f;
+  p.tc = dtype == OC_BF16 && head_dim <= 128 && R > (head_dim == 128 ? 32 : 64) && scale > 0.f;
   int64_t slots = device_sm_count();
   if (p.tc) {
     p.row_tile = 128;
@@ -628,7 +634,7 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
   if (p.tc) off += up256(tok_tc_prep_bytes(batch, q_len, G, seq_len));
   p.logit_off = off;
   p.logit_stride = 0;
-  if (lse && dtype == OC_BF16 && R <= kLogitRows) {
+  if (lse && dtype == OC_BF16 && !p.tc && R <= kLogitRows) {
     p.logit_stride = (seq_len + 63) / 64 * 64;  // whole tiles
     off += up256((size_t)batch * kv_heads * R * p.logit_stride * sizeof(float));
   }

@@ -68,9 +68,9 @@ template <int D>
 struct TcSmem {
   unsigned char q[2][TcCfg<D>::kTileBytes];
   unsigned char kv[TcCfg<D>::kSlots][TcCfg<D>::kTileBytes];
-  uint64_t kv_full[TcCfg<D>::kSlots], kv_empty[TcCfg<D>::kSlots];
+  uint64_t kv_full[TcCfg<D>::kSlots + 1], kv_empty[TcCfg<D>::kSlots + 1];
   uint64_t q_full, q_empty;
-  uint64_t v_clean[TcCfg<D>::kSlots];
+  uint64_t v_clean[TcCfg<D>::kSlots + 1];
   uint64_t s_full[2], p_full[2], o_full[2], o_free[2];
   uint64_t drain;
   uint32_t tmem_base;
@@ -95,6 +95,7 @@ struct TcUnit {
   int p0[2], hs[2], min_hi[2];
   int jt0, ncache, n;  // first cache tile, cache tiles, all tiles
   int d0;              // first drafted tile
+  bool dual;           // both halves of the CTA on one row tile, key tiles in turn
 };
 
 // The k-th unit of this CTA.  Units are ordered by falling work and dealt out
@@ -106,9 +107,9 @@ __device__ __forceinline__ int tc_deal(int k) {
 __device__ __forceinline__ TcUnit tc_unit(const TcArgs& x, const TokSeg& seg) {
   const TokArgs& a = x.t;
   TcUnit w;
-  const int pair = seg.unit % x.npairs;
+  const int pair = x.npairs == 1 ? 0 : seg.unit % x.npairs;
   w.b = seg.b;
-  w.h = seg.unit / x.npairs;
+  w.h = x.npairs == 1 ? seg.unit : seg.unit / x.npairs;
   w.bh = w.b * a.Hkv + w.h;
   w.part = seg.part;
   w.len = tok_len(a, w.b);
@@ -116,8 +117,8 @@ __device__ __forceinline__ TcUnit tc_unit(const TcArgs& x, const TokSeg& seg) {
   int first = INT32_MAX, last = 0, top = 0;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int r = 2 * pair + t, pt = r / x.nhs;
-    w.hs[t] = r % x.nhs;
+    const int r = 2 * pair + t, pt = x.nhs == 1 ? r : r / x.nhs;
+    w.hs[t] = r - pt * x.nhs;
     w.p0[t] = pt * x.P;
     w.min_hi[t] = 0;
     if (t >= w.ntile) continue;
@@ -151,7 +152,14 @@ __device__ __forceinline__ TcUnit tc_unit(const TcArgs& x, const TokSeg& seg) {
   w.ncache = max(0, min(last, seg.t1) - w.jt0);
   w.d0 = max(seg.t0 - nct, 0);
   w.n = w.ncache + (a.dk && seg.t1 > nct ? min(seg.t1 - nct, (a.Sq + kTok - 1) / kTok) - w.d0 : 0);
+  w.dual = x.tiles == 1 && seg.part >= 0;
   return w;
+}
+
+// Tile j of a unit: cache tiles from the last to the first, so that a row's
+// reference point comes from its nearest keys, then drafted tiles.
+__device__ __forceinline__ int tc_tile(const TcUnit& w, int j) {
+  return j < w.ncache ? w.jt0 + w.ncache - 1 - j : w.d0 + j - w.ncache;
 }
 
 // This CTA's units in order: its run of the even cut, or whole units.
@@ -371,11 +379,11 @@ __device__ __forceinline__ void chunk_exp(const float* s, int c, uint32_t* pk, u
 // Does tile j of the unit hold tokens that no query may see?
 __device__ __forceinline__ bool tc_dirty(const TcArgs& x, const TcUnit& w, int j) {
   const TokArgs& a = x.t;
+  const int jt = tc_tile(w, j);
   if (j >= w.ncache) {
-    const uint4 seen = x.tree_bits[((size_t)w.b * (a.Sq + 1) + a.Sq) * 2 + w.d0 + j - w.ncache];
+    const uint4 seen = x.tree_bits[((size_t)w.b * (a.Sq + 1) + a.Sq) * 2 + jt];
     return (seen.x & seen.y & seen.z & seen.w) != ~0u;
   }
-  const int jt = w.jt0 + j;
   return jt * kTok + kTok > w.len || (a.table && tc_key_row(a, w.b, jt) < 0) ||
          (a.docs && x.key_docs[(size_t)w.b * x.nkt + jt].x < 0);
 }
@@ -406,10 +414,13 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
   TcWalk walk(x, sm.pre);
   TcUnit w;
   while (walk.next(x, sm.pre, w)) {
-    if (t >= w.ntile) continue;
-    const int p0 = t ? w.p0[1] : w.p0[0], min_hi = t ? w.min_hi[1] : w.min_hi[0];
+    if (t >= w.ntile && !w.dual) continue;
+    const int rt = w.dual ? 0 : t;  // row tile
+    const int p0 = rt ? w.p0[1] : w.p0[0], min_hi = rt ? w.min_hi[1] : w.min_hi[0];
     const int pos_i = p0 + rl / x.Gp;  // query position of this row
-    const int r = pos_i * a.G + (t ? w.hs[1] : w.hs[0]) * x.Gp + rl % x.Gp;
+    const int r = pos_i * a.G + (rt ? w.hs[1] : w.hs[0]) * x.Gp + rl % x.Gp;
+    const int j_first = w.dual ? t : 0, j_step = w.dual ? 2 : 1;
+    const bool any = j_first < w.n;  // is there a tile for this half?
     const bool real = pos_i < a.Sq;
     const TokRow row = tok_row(a, w.b, w.h, real ? r : a.R, w.len);
     int4 qd = make_int4(0, 0, 0, 0);
@@ -421,18 +432,18 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
     bool no_page = false;
     const auto look = [&](int j) {
       if (j >= w.ncache) return;
-      if (a.docs) kd = x.key_docs[(size_t)w.b * x.nkt + w.jt0 + j];
-      if (a.table) no_page = tc_key_row(a, w.b, w.jt0 + j) < 0;
+      if (a.docs) kd = x.key_docs[(size_t)w.b * x.nkt + tc_tile(w, j)];
+      if (a.table) no_page = tc_key_row(a, w.b, tc_tile(w, j)) < 0;
     };
-    look(0);
-    for (int j = 0; j < w.n; ++j) {
+    look(j_first);
+    for (int j = j_first; j < w.n; j += j_step) {
       // is every key of the tile visible to every row of it?
       const bool draft = j >= w.ncache;
-      const int jt = draft ? w.d0 + j - w.ncache : w.jt0 + j, j0 = jt * kTok;
-      const bool hole = no_page;
+      const int jt = tc_tile(w, j), j0 = jt * kTok;
+      const bool hole = no_page && !draft;
       bool part = draft || j0 + kTok > min_hi || hole;
       if (a.docs && !draft) part = part || kd.x < 0 || kd.x != kd.y || qd.x != kd.x || qd.y != kd.x;
-      look(j + 1);
+      look(j + j_step);
       if (!bar_wait_warp(&sm.abort, &sm.s_full[t], s_ph)) return;
       s_ph ^= 1;
       tc_fence_after();
@@ -549,7 +560,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
           const bool need = mx > m_used + 8.f;
           if (__any_sync(0xffffffffu, need)) {
             const float alpha = need ? ex2(m_used - mx) : 1.f;  // 0 on a row's first visible tile
-            if (j > 0) {
+            if (j > j_first) {
 #pragma unroll 1
               for (int c = 0; c < D / 32; ++c) {
                 float o[32];
@@ -585,7 +596,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.p_full[t]);
     }
-    if (w.n > 0) {
+    if (any) {
       if (!bar_wait_warp(&sm.abort, &sm.o_full[t], o_ph)) return;
       o_ph ^= 1;
       tc_fence_after();
@@ -611,7 +622,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
         const int g = half * 16 + (lane >> 2);
         const bool put0 = __shfl_sync(0xffffffffu, real && m_used != -INFINITY, g);
         const bool put1 = __shfl_sync(0xffffffffu, real && m_used != -INFINITY, g + 8);
-        if (w.n == 0) continue;
+        if (!any) continue;
 #pragma unroll 1
         for (int c = 0; c < D / 64; ++c) {
           float o[32];
@@ -629,7 +640,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         float o[32];
-        if (w.n > 0) {
+        if (any) {
           tmem_ld32_wait(t_o + 32 * c, o);
         } else {
 #pragma unroll
@@ -650,12 +661,24 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
         }
       }
     }
-    if (w.n > 0) {
+    if (any) {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.o_free[t]);  // the next unit may overwrite O
     }
   }
+}
+
+// The K / V ring.  With one row tile per unit (dual) the second query buffer,
+// which lies right before it, is a slot more: two streams of key tiles are in
+// flight.
+template <int D>
+__device__ __forceinline__ unsigned char* tc_ring(TcSmem<D>& sm, const TcArgs& x) {
+  return x.tiles == 1 ? sm.q[1] : sm.kv[0];
+}
+template <int D>
+__device__ __forceinline__ uint32_t tc_slots(const TcArgs& x) {
+  return TcCfg<D>::kSlots + (x.tiles == 1 ? 1 : 0);
 }
 
 template <int D>
@@ -664,11 +687,12 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
   using C = TcCfg<D>;
   const TokArgs& a = x.t;
   uint32_t q_ph = 0, L = 0;
+  unsigned char* ring = tc_ring<D>(sm, x);
+  const uint32_t slots = tc_slots<D>(x);
   // after a wait that gave up: let the copies in flight land (bounded) before
   // the CTA ends
   auto drain = [&]() {
-    for (uint32_t s = 0; s < C::kSlots && s < L; ++s)
-      mbar_wait(&sm.kv_full[s], ((L - s - 1) / C::kSlots) & 1);
+    for (uint32_t s = 0; s < slots && s < L; ++s) mbar_wait(&sm.kv_full[s], ((L - s - 1) / slots) & 1);
     mbar_wait(&sm.q_full, q_ph ^ 1);
   };
   TcWalk walk(x, sm.pre);
@@ -686,17 +710,17 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
           tma_load_3d(sm.q[t] + c * C::kBox, mq, &sm.q_full, 64 * c, w.h * a.G + w.hs[t] * x.Gp, w.b * a.Sq + w.p0[t]);
     for (int j = 0; j < w.n; ++j) {
       const bool draft = j >= w.ncache;
-      int key = draft ? w.b * a.Sq + (w.d0 + j - w.ncache) * kTok : tc_key_row(a, w.b, w.jt0 + j);
+      int key = draft ? w.b * a.Sq + tc_tile(w, j) * kTok : tc_key_row(a, w.b, tc_tile(w, j));
       if (key < 0) key = 0;  // a page outside the pool: loaded from page 0, masked and zeroed
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv, ++L) {
-        const uint32_t slot = L % C::kSlots;
-        if (!bar_wait(&sm.abort, &sm.kv_empty[slot], ((L / C::kSlots) & 1) ^ 1)) return drain();
+        const uint32_t slot = L % slots;
+        if (!bar_wait(&sm.abort, &sm.kv_empty[slot], ((L / slots) & 1) ^ 1)) return drain();
         mbar_expect_tx(&sm.kv_full[slot], C::kTileBytes);
         const CUtensorMap* m = kv ? (draft ? mdv : mv) : (draft ? mdk : mk);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_3d(sm.kv[slot] + c * C::kBox, m, &sm.kv_full[slot], 64 * c, w.h, key);
+          tma_load_3d(ring + slot * C::kTileBytes + c * C::kBox, m, &sm.kv_full[slot], 64 * c, w.h, key);
       }
     }
   }
@@ -715,19 +739,21 @@ __device__ void tc_cleaner(TcSmem<D>& sm, const TcArgs& x) {
   using C = TcCfg<D>;
   const TokArgs& a = x.t;
   const int lane = threadIdx.x & 31;
+  unsigned char* ring = tc_ring<D>(sm, x);
+  const uint32_t slots = tc_slots<D>(x);
   uint32_t L = 0;
   TcWalk walk(x, sm.pre);
   TcUnit w;
   while (walk.next(x, sm.pre, w)) {
     for (int j = 0; j < w.n; ++j, L += 2) {
-      const uint32_t kslot = L % C::kSlots, slot = (L + 1) % C::kSlots;
-      if (!bar_wait_warp(&sm.abort, &sm.kv_full[kslot], (L / C::kSlots) & 1)) return;
+      const uint32_t kslot = L % slots, slot = (L + 1) % slots;
+      if (!bar_wait_warp(&sm.abort, &sm.kv_full[kslot], (L / slots) & 1)) return;
       if (lane == 0) mbar_arrive(&sm.kv_empty[kslot]);
-      if (!bar_wait_warp(&sm.abort, &sm.kv_full[slot], ((L + 1) / C::kSlots) & 1)) return;
+      if (!bar_wait_warp(&sm.abort, &sm.kv_full[slot], ((L + 1) / slots) & 1)) return;
       const bool dirty = tc_dirty(x, w, j);
       if (dirty) {
         const bool draft = j >= w.ncache;
-        const int jt = draft ? w.d0 + j - w.ncache : w.jt0 + j, j0 = jt * kTok;
+        const int jt = tc_tile(w, j), j0 = jt * kTok;
         const uint32_t* seen = reinterpret_cast<const uint32_t*>(x.tree_bits) + ((size_t)w.b * (a.Sq + 1) + a.Sq) * 8;
         const bool no_page = !draft && a.table && tc_key_row(a, w.b, jt) < 0;
         for (int it = 0; it < kTok / 4; ++it) {
@@ -737,7 +763,8 @@ __device__ void tc_cleaner(TcSmem<D>& sm, const TcArgs& x) {
           if (!keep)
 #pragma unroll
             for (int c = 0; c < D / 64; ++c)
-              *reinterpret_cast<uint4*>(sm.kv[slot] + c * C::kBox + rr * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(ring + slot * C::kTileBytes + c * C::kBox + rr * 128 + (lane & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async();  // the tensor cores read through the async proxy
         __syncwarp();
@@ -761,14 +788,16 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // A place in the K / V ring.
-template <int D>
 struct RingPos {
-  uint32_t slot = 0, ph = 0;
-  __device__ __forceinline__ void next() {
-    if (++slot == TcCfg<D>::kSlots) {
-      slot = 0;
-      ph ^= 1;
+  uint32_t slot, ph, slots;
+  __device__ __forceinline__ RingPos ahead(uint32_t n) const {  // n <= slots
+    RingPos r = *this;
+    r.slot += n;
+    if (r.slot >= slots) {
+      r.slot -= slots;
+      r.ph ^= 1;
     }
+    return r;
   }
 };
 
@@ -782,32 +811,98 @@ __device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
   using C = TcCfg<D>;
   constexpr uint32_t kIdQK = tc_idesc_bf16(kRows, kTok, 0), kIdPV = tc_idesc_bf16(kRows, D, 1);
   const uint64_t qd0 = sdesc(__shfl_sync(0xffffffffu, smem_u32(sm.q[0]), 0), 16, 1024);
-  const uint64_t kd0 = sdesc(__shfl_sync(0xffffffffu, smem_u32(sm.kv[0]), 0), 16, 1024);
-  const uint64_t vd0 = sdesc(__shfl_sync(0xffffffffu, smem_u32(sm.kv[0]), 0), C::kBox, 1024);
+  const uint32_t kv = __shfl_sync(0xffffffffu, smem_u32(tc_ring<D>(sm, x)), 0);
+  const uint64_t kd0 = sdesc(kv, 16, 1024), vd0 = sdesc(kv, C::kBox, 1024);
   tmem = __shfl_sync(0xffffffffu, tmem, 0);
   uint32_t q_ph = 0, p_ph[2] = {0, 0}, o_ph[2] = {1, 1}, clean_ph = 0;  // clean_ph: a bit per slot
-  RingPos<D> kp;
+  RingPos kp{0, 0, tc_slots<D>(x)};
+  const bool always = tc_look_always(x.t);
+  const auto wait_full = [&](const RingPos& r) { return bar_wait_warp(&sm.abort, &sm.kv_full[r.slot], r.ph); };
+  const auto wait_clean = [&](const RingPos& r) {
+    if (!bar_wait_warp(&sm.abort, &sm.v_clean[r.slot], (clean_ph >> r.slot) & 1)) return false;
+    clean_ph ^= 1u << r.slot;
+    return true;
+  };
+  // by the elected lane: S_t = Q K^T of the tile at kd; O_t (+)= P_t V
+  const auto scores = [&](int t, uint64_t qd, const RingPos& r) {
+    const uint64_t kd = kd0 + r.slot * (C::kTileBytes >> 4);
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      const uint32_t off = ((kk >> 2) * C::kBox + (kk & 3) * 32) >> 4;
+      umma_bf16(tmem + t * 256, qd + off, kd + off, kIdQK, kk > 0 ? 1 : 0);
+    }
+  };
+  const auto values = [&](int t, const RingPos& r, bool first) {
+    const uint64_t vd = vd0 + r.slot * (C::kTileBytes >> 4);
+#pragma unroll
+    for (int kk = 0; kk < kTok / 16; ++kk)
+      umma_bf16_ts(tmem + t * 256 + 128, tmem + t * 256 + kk * 8, vd + kk * 128, kIdPV, !first || kk > 0 ? 1 : 0);
+  };
   TcWalk walk(x, sm.pre);
   TcUnit w;
   while (walk.next(x, sm.pre, w)) {
     const int n = __shfl_sync(0xffffffffu, w.n, 0), ntile = __shfl_sync(0xffffffffu, w.ntile, 0);
+    const bool dual = __shfl_sync(0xffffffffu, (int)w.dual, 0) != 0;
     if (n == 0) continue;
-    // first tile whose values pass the cleaner
-    const int dirty0 = tc_look_always(x.t) ? 0 : w.len / kTok - w.jt0;
+    // is the first tile cut by the end of the sequence?
+    const bool cut = (w.jt0 + w.ncache) * kTok > w.len && w.ncache > 0;
     if (!bar_wait_warp(&sm.abort, &sm.q_full, q_ph)) return;
     q_ph ^= 1;
-    if (!bar_wait_warp(&sm.abort, &sm.kv_full[kp.slot], kp.ph)) return;
+    if (dual) {
+      // half t takes the key tiles t, t + 2, ...: K of tile j is load 2 j of the
+      // unit, V load 2 j + 1
+      for (int j = 0; j < n + 2; ++j) {
+        const int t = j & 1;
+        const RingPos kn = kp.ahead(4);  // of tile j + 2 (there are at least six slots)
+        if (j >= 2) {                    // PV of tile j - 2
+          const RingPos vp = kp.ahead(1);
+          if (!wait_full(vp)) return;
+          if ((always || (cut && j == 2)) && !wait_clean(vp)) return;
+          if (j < 4) {  // the softmax has read the previous unit's O_t
+            if (!bar_wait_warp(&sm.abort, &sm.o_free[t], o_ph[t])) return;
+            o_ph[t] ^= 1;
+          }
+          if (j < n && !wait_full(kn)) return;
+          if (!bar_wait_warp(&sm.abort, &sm.p_full[t], p_ph[t])) return;
+          p_ph[t] ^= 1;
+          tc_fence_after();
+          if (elect_one()) {
+            values(t, vp, j < 4);
+            umma_commit(&sm.kv_empty[vp.slot]);
+            if (j < n) {
+              scores(t, qd0, kn);
+              umma_commit(&sm.s_full[t]);
+              umma_commit(&sm.kv_empty[kn.slot]);
+              if (j == n - 1) umma_commit(&sm.q_empty);
+            } else {
+              umma_commit(&sm.o_full[t]);
+            }
+          }
+          kp = kp.ahead(2);
+        } else if (j < n) {  // the first S of each half
+          const RingPos r = kp.ahead(2 * j);
+          if (!wait_full(r)) return;
+          tc_fence_after();
+          if (elect_one()) {
+            scores(t, qd0, r);
+            umma_commit(&sm.s_full[t]);
+            umma_commit(&sm.kv_empty[r.slot]);
+            if (j == n - 1) umma_commit(&sm.q_empty);
+          }
+        } else {
+          continue;
+        }
+        __syncwarp();
+      }
+      continue;
+    }
+    if (!wait_full(kp)) return;
     tc_fence_after();
     // S of the first key tile
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       if (t < ntile && elect_one()) {
-        const uint64_t kd = kd0 + kp.slot * (C::kTileBytes >> 4);
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = ((kk >> 2) * C::kBox + (kk & 3) * 32) >> 4;
-          umma_bf16(tmem + t * 256, qd0 + t * (C::kTileBytes >> 4) + off, kd + off, kIdQK, kk > 0 ? 1 : 0);
-        }
+        scores(t, qd0 + t * (C::kTileBytes >> 4), kp);
         umma_commit(&sm.s_full[t]);
         if (t == ntile - 1) {
           umma_commit(&sm.kv_empty[kp.slot]);
@@ -817,21 +912,14 @@ __device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
       __syncwarp();
     }
     for (int j = 1; j <= n; ++j) {
-      RingPos<D> vp = kp;
-      vp.next();  // V of tile j - 1; K of tile j after it
-      kp = vp;
-      kp.next();
-      const uint64_t vd = vd0 + vp.slot * (C::kTileBytes >> 4), kd = kd0 + kp.slot * (C::kTileBytes >> 4);
-      if (!bar_wait_warp(&sm.abort, &sm.kv_full[vp.slot], vp.ph)) return;
-      if (j > dirty0) {
-        if (!bar_wait_warp(&sm.abort, &sm.v_clean[vp.slot], (clean_ph >> vp.slot) & 1)) return;
-        clean_ph ^= 1u << vp.slot;
-      }
-      if (j < n && !bar_wait_warp(&sm.abort, &sm.kv_full[kp.slot], kp.ph)) return;
+      const RingPos vp = kp.ahead(1);  // V of tile j - 1; K of tile j after it
+      kp = kp.ahead(2);
+      if (!wait_full(vp)) return;
+      if ((always || (cut && j == 1)) && !wait_clean(vp)) return;
+      if (j < n && !wait_full(kp)) return;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (t >= ntile) break;
-        const uint32_t d_s = tmem + t * 256, d_o = d_s + 128;
         if (j == 1) {  // the softmax has read the previous unit's O_t
           if (!bar_wait_warp(&sm.abort, &sm.o_free[t], o_ph[t])) return;
           o_ph[t] ^= 1;
@@ -840,15 +928,9 @@ __device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
         p_ph[t] ^= 1;
         tc_fence_after();
         if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < kTok / 16; ++kk)
-            umma_bf16_ts(d_o, d_s + kk * 8, vd + kk * 128, kIdPV, (j > 1 || kk > 0) ? 1 : 0);
+          values(t, vp, j == 1);
           if (j < n) {
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = ((kk >> 2) * C::kBox + (kk & 3) * 32) >> 4;
-              umma_bf16(d_s, qd0 + t * (C::kTileBytes >> 4) + off, kd + off, kIdQK, kk > 0 ? 1 : 0);
-            }
+            scores(t, qd0 + t * (C::kTileBytes >> 4), kp);
             umma_commit(&sm.s_full[t]);  // covers PV of tile j - 1 too: O_t may be rescaled
           } else {
             umma_commit(&sm.o_full[t]);
@@ -874,7 +956,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   TcSmem<D>& sm = *reinterpret_cast<TcSmem<D>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < TcCfg<D>::kSlots; ++i) {
+    for (int i = 0; i <= TcCfg<D>::kSlots; ++i) {
       mbar_init(&sm.kv_full[i], 1);
       mbar_init(&sm.kv_empty[i], 2);  // the products and the cleaner
       mbar_init(&sm.v_clean[i], 1);
