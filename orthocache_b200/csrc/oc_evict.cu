@@ -8,12 +8,26 @@
 // position of each.  The reference evicts whole 512-token blocks by their
 // spectrum (src/orthocache/compaction.py:28-100); this is the token-level
 // counterpart by attention weight.
+//
+// Selection is bound by latency, not bytes (a head's weights are 4 bytes a token,
+// its kept keys and values 4 D): a head's weights are read once into the shared
+// memory of a cluster of CTAs, and the threshold found by three histograms of 11,
+// 11 and 10 bits of the order-preserving key, added up over the cluster through
+// distributed shared memory, an eighth of the bins by each CTA (every CTA reading
+// all histograms took 8,000 cycles a pass, this 2,500).  The gather is bound by memory: every kept row read
+// and written once.
+#include <cooperative_groups.h>
+
 #include "oc_common.cuh"
 
 namespace oc {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kSelThreads = 1024;
+constexpr int kBins = 2048;
+constexpr int kSelCached = 48 * 1024;  // weights of one CTA that fit its shared memory
 
 // Order-preserving 32-bit key of a weight: larger weight, larger key; -0 = +0;
 // NaN above everything.
@@ -23,48 +37,63 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exclusive scan of one value per thread over the block; returns the total too.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int& total) {
+// Exclusive scan of two values per thread over the block, with the totals.
+__device__ __forceinline__ int2 block_scan2(int2 v, int2* warp_sums, int2& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
+  int2 x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+    const int a = __shfl_up_sync(0xffffffffu, x.x, o), b = __shfl_up_sync(0xffffffffu, x.y, o);
+    if (lane >= o) {
+      x.x += a;
+      x.y += b;
+    }
   }
   __syncthreads();  // the previous scan's sums are read
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
-  int before = 0, all = 0;
+  int2 s = warp_sums[lane];  // 32 warps: every warp scans the sums
 #pragma unroll
-  for (int w = 0; w < kSelThreads / 32; ++w) {
-    const int s = warp_sums[w];
-    if (w < warp) before += s;
-    all += s;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, s.x, o), b = __shfl_up_sync(0xffffffffu, s.y, o);
+    if (lane >= o) {
+      s.x += a;
+      s.y += b;
+    }
   }
-  total = all;
-  return before + x - v;
+  total = make_int2(__shfl_sync(0xffffffffu, s.x, 31), __shfl_sync(0xffffffffu, s.y, 31));
+  const int2 before = make_int2(__shfl_sync(0xffffffffu, s.x, warp ? warp - 1 : 0),
+                                __shfl_sync(0xffffffffu, s.y, warp ? warp - 1 : 0));
+  return make_int2(x.x - v.x + (warp ? before.x : 0), x.y - v.y + (warp ? before.y : 0));
 }
 
-// One CTA per (b, h): radix selection of the (keep - recent)-th largest key, 8
-// bits a pass, then one pass in order of position that writes the kept
-// positions.
+struct SelSmem {
+  int hist[kBins];
+  int all[kBins];  // the cluster's
+  int2 warp_sums[kSelThreads / 32];
+  int2 sums;  // this CTA's kept by value, equal to the threshold
+  uint32_t digit;
+  int need;
+};
+
+// One cluster of CS CTAs per (b, h); CTA r holds the r-th segment of the tokens.
+// CACHED: its weights lie in shared memory behind SelSmem.
+template <int CS, bool CACHED>
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const float* weights, const int32_t* lengths,
                                                                    int S, int H, int keep, int recent, int32_t* index,
                                                                    float* weights_out, int32_t* new_lengths) {
-  __shared__ int hist[256];
-  __shared__ int warp_sums[kSelThreads / 32];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
-  const int bh = blockIdx.x, b = bh / H, tid = threadIdx.x;
+  extern __shared__ __align__(16) unsigned char raw[];
+  SelSmem& sm = *reinterpret_cast<SelSmem*>(raw);
+  float* cache = reinterpret_cast<float*>(raw + sizeof(SelSmem));
+  const int bh = blockIdx.x / CS, rank = blockIdx.x % CS, b = bh / H, tid = threadIdx.x;
   int n = lengths ? lengths[b] : S;
   n = n < 0 ? 0 : (n > S ? S : n);
   const float* w = weights + (int64_t)bh * S;
   int32_t* idx = index + (int64_t)bh * keep;
   float* wo = weights_out + (int64_t)bh * keep;
-  if (bh % H == 0 && tid == 0) new_lengths[b] = min(n, keep);
-  if (n <= keep) {
-    for (int i = tid; i < keep; i += kSelThreads) {
+  if (bh % H == 0 && rank == 0 && tid == 0) new_lengths[b] = min(n, keep);
+  if (n <= keep) {  // the same for the whole cluster
+    for (int i = rank * kSelThreads + tid; i < keep; i += CS * kSelThreads) {
       idx[i] = i < n ? i : -1;
       wo[i] = i < n ? w[i] : 0.f;
     }
@@ -72,56 +101,137 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const float* 
   }
   const int cand = n - recent;  // tokens that compete
   const int want = keep - recent;
+  const int seg = (n + CS - 1) / CS, s0 = min(n, rank * seg), cnt = min(n, s0 + seg) - s0;
+  const int comp = max(0, min(cnt, cand - s0));  // of them, those that compete
+  if (CACHED) {
+#pragma unroll 8
+    for (int i = tid; i < cnt; i += kSelThreads) cache[i] = w[s0 + i];
+  }
+  const float* mine = CACHED ? cache : w + s0;
+
+  // threshold key: the want-th largest; need: how many equal to it are taken
   uint32_t prefix = 0;
-  int need = want;  // of the tokens equal to the prefix so far, how many are still to be taken
+  int need = want;
   if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+      for (int i = tid; i < kBins; i += kSelThreads) sm.hist[i] = 0;
       __syncthreads();
-      for (int i = tid; i < cand; i += kSelThreads) {
-        const uint32_t key = weight_key(w[i]);
-        if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
+#pragma unroll 4
+      for (int j0 = 0; j0 < comp; j0 += kSelThreads) {
+        const bool valid = j0 + tid < comp;
+        const uint32_t key = valid ? weight_key(mine[j0 + tid]) : 0;
+        const bool in = valid && (pass == 0 || (key >> (shift + bits)) == (prefix >> (shift + bits)));
+        const uint32_t digit = (key >> shift) & ((1u << bits) - 1u);
+        // equal weights crowd one bin: one addition when a warp agrees
+        const uint32_t first = __shfl_sync(0xffffffffu, digit, 0);
+        if (__all_sync(0xffffffffu, in && digit == first)) {
+          if ((tid & 31) == 0) atomicAdd(&sm.hist[digit], 32);
+        } else if (in) {
+          atomicAdd(&sm.hist[digit], 1);
+        }
+      }
+      if (CS > 1) {
+        // CTA r adds up the r-th part of the bins and hands the sums to all
+        constexpr int kPart = kBins / CS;
+        cg::this_cluster().sync();
+        if (tid < kPart) {
+          const int bin = rank * kPart + tid;
+          int sum = 0;
+#pragma unroll
+          for (int r = 0; r < CS; ++r) sum += cg::this_cluster().map_shared_rank(sm.hist, r)[bin];
+#pragma unroll
+          for (int r = 0; r < CS; ++r) cg::this_cluster().map_shared_rank(sm.all, r)[bin] = sum;
+        }
+        cg::this_cluster().sync();
+      } else {
+        __syncthreads();
+      }
+      // from the top: thread t has bins kBins - 1 - 2 t and the one below
+      const int* h = CS > 1 ? sm.all : sm.hist;
+      const int hi = kBins - 1 - 2 * tid, c0 = h[hi], c1 = h[hi - 1];
+      int2 total;
+      const int before = block_scan2(make_int2(c0 + c1, 0), sm.warp_sums, total).x;
+      if (before < need && need <= before + c0) {
+        sm.digit = hi;
+        sm.need = need - before;
+      } else if (before + c0 < need && need <= before + c0 + c1) {
+        sm.digit = hi - 1;
+        sm.need = need - before - c0;
       }
       __syncthreads();
-      if (tid == 0) {
-        int left = need, d = 255;
-        while (d > 0 && hist[d] < left) left -= hist[d--];
-        s_prefix = prefix | ((uint32_t)d << shift);
-        s_need = left;
-      }
-      __syncthreads();
-      prefix = s_prefix;
-      need = s_need;
+      prefix |= sm.digit << shift;
+      need = sm.need;
     }
   }
-  // in order of position: everything above the threshold key, the first
-  // `need` tokens equal to it, and the recent ones
-  int base = 0, eq_base = 0;
-  for (int i0 = 0; i0 < n; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    int above = 0, equal = 0;
-    float wi = 0.f;
-    if (i < n) {
-      wi = w[i];
-      if (i >= cand) {
-        above = 1;
-      } else if (want > 0) {
-        const uint32_t key = weight_key(wi);
-        above = key > prefix;
-        equal = key == prefix;
-      }
+
+  // in order of position: everything above the threshold and the recent tokens,
+  // and the first `need` equal to it; a thread has a run of tokens
+  const int per = (cnt + kSelThreads - 1) / kSelThreads, i0 = min(cnt, tid * per), i1 = min(cnt, i0 + per);
+  int2 have = make_int2(0, 0);
+  if (CACHED) __syncthreads();
+  for (int i = i0; i < i1; ++i) {
+    if (i >= comp) {
+      ++have.x;
+    } else if (want > 0) {
+      const uint32_t key = weight_key(mine[i]);
+      have.x += key > prefix;
+      have.y += key == prefix;
     }
-    int eq_total, total;
-    const int eq_rank = eq_base + block_scan(equal, warp_sums, eq_total);
-    eq_base += eq_total;
-    const int take = above || (equal && eq_rank < need);
-    const int slot = base + block_scan(take, warp_sums, total);
-    base += total;
-    if (take && slot < keep) {
-      idx[slot] = i;
+  }
+  int2 total;
+  int2 at = block_scan2(have, sm.warp_sums, total);
+  if (CS > 1) {
+    if (tid == 0) sm.sums = total;
+    cg::this_cluster().sync();
+    for (int r = 0; r < rank; ++r) {
+      const int2 o = *cg::this_cluster().map_shared_rank(&sm.sums, r);
+      at.x += o.x;
+      at.y += o.y;
+    }
+  }
+  for (int i = i0; i < i1; ++i) {
+    const float wi = mine[i];
+    bool above = true, equal = false;
+    if (i < comp) {
+      const uint32_t key = weight_key(wi);
+      above = want > 0 && key > prefix;
+      equal = want > 0 && key == prefix;
+    }
+    if (above || (equal && at.y < need)) {
+      const int slot = at.x + min(at.y, need);
+      idx[slot] = s0 + i;
       wo[slot] = wi;
     }
+    at.x += above;
+    at.y += equal;
   }
+  if (CS > 1) cg::this_cluster().sync();  // no CTA leaves while others read its sums
+}
+
+template <int CS, bool CACHED>
+cudaError_t launch_select(int heads, size_t smem, cudaStream_t st, const float* weights, const int32_t* lengths, int S,
+                          int H, int keep, int recent, int32_t* index, float* weights_out, int32_t* new_lengths) {
+  auto kern = evict_select_kernel<CS, CACHED>;
+  static std::atomic<uint64_t> done{0};
+  if (first_on_device(done)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)(sizeof(SelSmem) + (CACHED ? kSelCached * 4 : 0)));
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(heads * CS));
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CS;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CS > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, weights, lengths, S, H, keep, recent, index, weights_out, new_lengths);
 }
 
 // Rows of keys and values: one 16-byte vector per thread; output row (b, i, h)
@@ -177,11 +287,21 @@ extern "C" int oc_evict_tokens(const void* k, const void* v, int dtype, const fl
   const int64_t total = (int64_t)batch * keep * kv_heads * vecs;
   OC_REQUIRE((total + 255) / 256 < INT32_MAX, OC_ERR_SHAPE, "oc_evict_tokens: too many rows");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  evict_select_kernel<<<batch * kv_heads, kSelThreads, 0, st>>>(weights, lengths, seq_len, kv_heads, keep, recent,
-                                                                index, weights_out, new_lengths);
-  int rc = check_launch("evict_select_kernel");
-  if (rc) return rc;
-  cudaError_t e = launch_pdl(evict_gather_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st,
+  // a CTA per head up to 4096 tokens, a cluster of eight beyond (what a pass over
+  // 8192 weights in one CTA takes is about what the cluster's barriers cost)
+  const int heads = batch * kv_heads;
+  cudaError_t e;
+  if (seq_len <= 4096)
+    e = launch_select<1, true>(heads, sizeof(SelSmem) + (size_t)seq_len * 4, st, weights, lengths, seq_len, kv_heads,
+                               keep, recent, index, weights_out, new_lengths);
+  else if ((seq_len + 7) / 8 <= kSelCached)
+    e = launch_select<8, true>(heads, sizeof(SelSmem) + (size_t)((seq_len + 7) / 8) * 4, st, weights, lengths, seq_len,
+                               kv_heads, keep, recent, index, weights_out, new_lengths);
+  else
+    e = launch_select<8, false>(heads, sizeof(SelSmem), st, weights, lengths, seq_len, kv_heads, keep, recent, index,
+                                weights_out, new_lengths);
+  if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "evict_select_kernel: %s", cudaGetErrorString(e));
+  e = launch_pdl(evict_gather_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st,
                              static_cast<const uint4*>(k), static_cast<const uint4*>(v), index, seq_len, kv_heads,
                              keep, vecs, total, static_cast<uint4*>(k_out), static_cast<uint4*>(v_out));
   if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "evict_gather_kernel: %s", cudaGetErrorString(e));
