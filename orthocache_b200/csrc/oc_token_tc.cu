@@ -309,28 +309,35 @@ __device__ __forceinline__ bool cap_far(const float* s, float k_in) {
   return __any_sync(0xffffffffu, !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * k_in <= kCapPoly3));
 }
 
-// 2^x of a pair on the FMA pipe, for x >= -126 or clamped there: x = n + f, n =
-// floor(x) by adding 1.5 * 2^23 with rounding toward -inf (its low bits are then
-// n), 2^f on [0, 1) a least-squares polynomial of degree 4 with equalised
-// relative error (2.6e-6), times 2^n built in the exponent field.  NaN stays NaN.
-template <bool CLAMP>
+// 2^x of a pair on the FMA pipe, x clamped to >= -126: x = n + f, n = floor(x) by
+// adding 1.5 * 2^23 with rounding toward -inf (its low bits are then n), 2^f on [0,
+// 1) a least-squares polynomial with equalised relative error (degree 4: 2.6e-6,
+// degree 5: 7.5e-8), times 2^n built in the exponent field.  NaN stays NaN.
+template <int DEG>
 __device__ __forceinline__ uint64_t poly_ex2(uint64_t x) {
-  if (CLAMP) {
-    float a, b;
-    up2(x, a, b);
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
-    x = pk2(a, b);
-  }
+  float a, b;
+  up2(x, a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.f));
+  x = pk2(a, b);
   uint64_t t, n, f;
   const uint64_t magic = pk2(12582912.f, 12582912.f);
   asm("add.rm.f32x2 %0, %1, %2;" : "=l"(t) : "l"(x), "l"(magic));
   asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(n) : "l"(t), "l"(magic));
   asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(f) : "l"(x), "l"(n));
-  uint64_t p = fma2(pk2(0.013534166850149632f, 0.013534166850149632f), f, pk2(0.052011460065841675f, 0.052011460065841675f));
-  p = fma2(p, f, pk2(0.2414427548646927f, 0.2414427548646927f));
-  p = fma2(p, f, pk2(0.6930038332939148f, 0.6930038332939148f));
-  p = fma2(p, f, pk2(1.0000026226043701f, 1.0000026226043701f));
+  uint64_t p;
+  if (DEG == 4) {
+    p = fma2(pk2(0.013534166850149632f, 0.013534166850149632f), f, pk2(0.052011460065841675f, 0.052011460065841675f));
+    p = fma2(p, f, pk2(0.2414427548646927f, 0.2414427548646927f));
+    p = fma2(p, f, pk2(0.6930038332939148f, 0.6930038332939148f));
+    p = fma2(p, f, pk2(1.0000026226043701f, 1.0000026226043701f));
+  } else {
+    p = fma2(pk2(0.0018775765784084797f, 0.0018775765784084797f), f, pk2(0.008989340625703335f, 0.008989340625703335f));
+    p = fma2(p, f, pk2(0.05582631751894951f, 0.05582631751894951f));
+    p = fma2(p, f, pk2(0.24015361070632935f, 0.24015361070632935f));
+    p = fma2(p, f, pk2(0.6931530833244324f, 0.6931530833244324f));
+    p = fma2(p, f, pk2(0.9999999403953552f, 0.9999999403953552f));
+  }
   float t0, t1;
   up2(t, t0, t1);
   return mul2(p, pk2(__uint_as_float(__float_as_uint(t0) * (1u << 23) + 0x3f800000u),
@@ -365,7 +372,7 @@ __device__ __forceinline__ void chunk_exp(const float* s, int c, uint32_t* pk, u
     const uint64_t e = DEG ? cap.poly2<DEG ? DEG : 2>(v, off) : fma2(v, pk2(c_scale, c_scale), off);
     float e0, e1;
     if (D == 64 && !DEG && i % 8 == 0) {
-      up2(poly_ex2<true>(e), e0, e1);
+      up2(poly_ex2<4>(e), e0, e1);
     } else {
       up2(e, e0, e1);
       e0 = ex2(e0);
@@ -1023,7 +1030,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 // that a thread (a tensor-memory lane) owns one key and adds its weights over
 // all query rows in its own registers, in the order of the rows: no exchange
 // between threads, no atomics.  One MMA and one exponential per row and key:
-// bound by the exponentials.  A unit is two tiles of 128 keys of one (b, h)
+// bound by the exponentials, five in sixteen of which run on the FMA pipe (2 x
+// 1024 rows on 8K keys: 235 -> 221 us; more, or any beside a cap's polynomial,
+// costs).  A unit is two tiles of 128 keys of one (b, h)
 // that share every query tile; two score buffers per key tile in tensor memory
 // let the products run ahead of the exponentials.
 // ---------------------------------------------------------------------------
@@ -1114,42 +1123,46 @@ template <int D>
 __device__ void tw_mma(TwSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
   using C = TcCfg<D>;
   constexpr uint32_t kId = tc_idesc_bf16(kTok, kRows, 0);
-  const bool lead = (threadIdx.x & 31) == 0;
-  uint32_t k_ph = 0, L = 0, use[2] = {0, 0};
+  const uint64_t kd0 = sdesc(__shfl_sync(0xffffffffu, smem_u32(sm.k[0]), 0), 16, 1024);
+  const uint64_t qd0 = sdesc(__shfl_sync(0xffffffffu, smem_u32(sm.q[0]), 0), 16, 1024);
+  tmem = __shfl_sync(0xffffffffu, tmem, 0);
+  uint32_t k_ph = 0, slot = 0, ph = 0, use[2] = {0, 0};
   for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
     const int u = tc_deal(k);
     if (u >= x.units) continue;
     const TwUnit w = tw_unit(x, u);
-    if (w.n == 0) continue;
+    const int n = __shfl_sync(0xffffffffu, w.n, 0), ntile = __shfl_sync(0xffffffffu, w.ntile, 0);
+    if (n == 0) continue;
     if (!bar_wait_warp(&sm.abort, &sm.k_full, k_ph)) return;
     k_ph ^= 1;
-    for (int i = 0; i < w.n; ++i, ++L) {
-      const uint32_t slot = L % kWqSlots;
-      if (!bar_wait_warp(&sm.abort, &sm.q_full[slot], (L / kWqSlots) & 1)) return;
-      tc_fence_after();
+    for (int i = 0; i < n; ++i) {
+      const uint64_t qd = qd0 + slot * (C::kTileBytes >> 4);
+      if (!bar_wait_warp(&sm.abort, &sm.q_full[slot], ph)) return;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        if (t >= w.ntile) break;
+        if (t >= ntile) break;
         const uint32_t buf = use[t] & 1;
         if (!bar_wait_warp(&sm.abort, &sm.s_empty[t][buf], ((use[t] >> 1) & 1) ^ 1)) return;
         ++use[t];
         tc_fence_after();
-        if (lead) {
-          const uint32_t ka = smem_u32(sm.k[t]), qb = smem_u32(sm.q[slot]);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * C::kBox + (kk & 3) * 32;
-            umma_bf16(tmem + t * 256 + buf * 128, sdesc(ka + off, 16, 1024), sdesc(qb + off, 16, 1024), kId, kk > 0 ? 1 : 0);
+            const uint32_t off = ((kk >> 2) * C::kBox + (kk & 3) * 32) >> 4;
+            umma_bf16(tmem + t * 256 + buf * 128, kd0 + t * (C::kTileBytes >> 4) + off, qd + off, kId, kk > 0 ? 1 : 0);
           }
           umma_commit(&sm.s_full[t][buf]);
+          if (t == ntile - 1) {
+            umma_commit(&sm.q_empty[slot]);
+            if (i == n - 1) umma_commit(&sm.k_empty);
+          }
         }
         __syncwarp();
       }
-      if (lead) {
-        umma_commit(&sm.q_empty[slot]);
-        if (i == w.n - 1) umma_commit(&sm.k_empty);
+      if (++slot == kWqSlots) {
+        slot = 0;
+        ph ^= 1;
       }
-      __syncwarp();
     }
   }
 }
@@ -1191,29 +1204,32 @@ __device__ void tw_sum(TwSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem, con
 #pragma unroll
           for (int k = 0; k < 128; k += 4) {
             const float4 z = lse[k / 4];
-            const uint64_t n0 = pk2(-z.x, -z.y), n1 = pk2(-z.z, -z.w);
-            uint64_t e0, e1;
-            if (CAP) {
-              e0 = cap.poly2<3>(pk2(s[k], s[k + 1]), n0);
-              e1 = cap.poly2<3>(pk2(s[k + 2], s[k + 3]), n1);
-            } else {
-              e0 = fma2(pk2(s[k], s[k + 1]), sc2, n0);
-              e1 = fma2(pk2(s[k + 2], s[k + 3]), sc2, n1);
+            const uint64_t nz[2] = {pk2(-z.x, -z.y), pk2(-z.z, -z.w)};
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const uint64_t v = pk2(s[k + 2 * y], s[k + 2 * y + 1]);
+              uint64_t e = CAP ? cap.poly2<3>(v, nz[y]) : fma2(v, sc2, nz[y]);
+              if (!CAP && (k / 2 + y) % 16 < 5) {
+                e = poly_ex2<5>(e);
+              } else {
+                float e0, e1;
+                up2(e, e0, e1);
+                e = pk2(ex2(e0), ex2(e1));
+              }
+              acc[(k / 2 + y) & 3] = add2(acc[(k / 2 + y) & 3], e);
             }
-            float a0, a1, b0, b1;
-            up2(e0, a0, a1);
-            up2(e1, b0, b1);
-            acc[(k / 2) & 3] = add2(acc[(k / 2) & 3], pk2(ex2(a0), ex2(a1)));
-            acc[(k / 2 + 1) & 3] = add2(acc[(k / 2 + 1) & 3], pk2(ex2(b0), ex2(b1)));
           }
         } else {
           const int lo = max(0, (j - pos0) * x.Gp), hi = min(kRows, (a.Sq - p0) * x.Gp);
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int k = 0; k < 128; ++k) {
             const float v = CAP ? cap.exact(s[k]) : s[k] * c_scale;
             const float z = sm.lse[slot][k];
-            if (k >= lo && k < hi && z != INFINITY) edge += ex2(v - z);
+            const float e = ex2(v - z);
+            if (k >= lo && k < hi && z != INFINITY) sum[k & 3] += e;
           }
+          edge += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
       }
       __syncwarp();
@@ -1275,7 +1291,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == kMmaWarp) {
       tw_mma<D>(sm, x, tmem);
       __syncwarp();
-      if ((threadIdx.x & 31) == 0) {
+      if (elect_one()) {
         umma_commit(&sm.drain);
         if (!mbar_wait(&sm.drain, 0)) atomicExch(&g_token_status, 1);
       }
