@@ -39,19 +39,13 @@ def _on(x, device=None, dtype=None):
     return _lib.as_device(x, device=device, dtype=dtype)
 
 
-class _Device:
-    """``torch.cuda.device`` that does nothing on the current device."""
-
-    def __init__(self, device):
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *args):
-        if self.guard is not None:
-            self.guard.__exit__(*args)
+def _call(name, device, *args):
+    """A library call with ``device`` current, on its current stream."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, _lib.stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, _lib.stream_ptr(device))
 
 
 def _int_rows(x, shape, device, what):
@@ -66,7 +60,7 @@ def _int_rows(x, shape, device, what):
     t = _on(x, device)
     if t.dtype.is_floating_point or t.dtype == torch.bool:
         raise TypeError(f"{what} must be integers, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what} {tuple(t.shape)}, expected {tuple(shape)}")
     return t.to(torch.int32).contiguous()
 
@@ -82,14 +76,15 @@ def _cap_scale(cap, scale, dim):
 
 
 @functools.lru_cache(maxsize=1024)
-def _workspace_bytes(device, *sizes):
-    return _lib.query("oc_token_attention_workspace_bytes", *sizes)
+def _workspace_bytes(device_index, *sizes):
+    with torch.cuda.device(device_index):
+        return _lib.query("oc_token_attention_workspace_bytes", *sizes)
 
 
-def _workspace(q, dtype, kv_heads, seq_len, accumulate):
+def _workspace(device, *sizes):
     """Scratch of one call (what it needs depends on the sizes and the device alone)."""
-    n = _workspace_bytes(q.device, dtype, q.shape[0], q.shape[1], q.shape[2], kv_heads, q.shape[3], seq_len, accumulate)
-    return torch.empty((n,), dtype=torch.uint8, device=q.device), n
+    n = _workspace_bytes(device.index, *sizes)
+    return torch.empty((n,), dtype=torch.uint8, device=device), n
 
 
 def _ptr(t):
@@ -134,7 +129,7 @@ def tree_attention(q, keys, values, draft_keys, draft_values, tree_mask, lengths
     B, T, Hq, D = qq.shape
     Hkv = k.shape[-2]
     _check_heads(qq, Hkv)
-    if k.shape[-1] != D or tuple(dk.shape) != (B, T, Hkv, D):
+    if k.shape[-1] != D or dk.shape != (B, T, Hkv, D):
         raise ValueError(f"incompatible shapes q {tuple(qq.shape)}, keys {tuple(k.shape)}, draft {tuple(dk.shape)}")
     table = None
     if block_table is None:
@@ -152,20 +147,18 @@ def tree_attention(q, keys, values, draft_keys, draft_values, tree_mask, lengths
         S = stride * PAGE
     mask = _on(tree_mask, device=dev)
     mask_batched = mask.dim() == 3
-    if tuple(mask.shape) != ((B, T, T) if mask_batched else (T, T)):
+    if mask.shape != ((B, T, T) if mask_batched else (T, T)):
         raise ValueError(f"tree_mask {tuple(mask.shape)}, expected ({T}, {T}) or ({B}, {T}, {T})")
     if mask.dtype not in (torch.bool, torch.uint8):
         raise TypeError(f"tree_mask must be bool, got {mask.dtype}")
     lens = _int_rows(lengths, (B,), dev, "lengths")
     cap, scale = _cap_scale(cap, scale, D)
     code = _lib.dtype_code(k)
-    with _Device(dev):
-        out = torch.empty_like(qq)
-        ws, ws_bytes = _workspace(qq, code, Hkv, S, 0)
-        _lib.call("oc_tree_attention", _ptr(qq), _ptr(k), _ptr(v), code, _ptr(table),
-                  stride, pages, PAGE, _ptr(lens), _ptr(dk), _ptr(dv), _ptr(mask), int(mask_batched),
-                  B, T, Hq, Hkv, D, S, cap, scale, _ptr(out), code, _ptr(ws), ws_bytes,
-                  _lib.stream_ptr(dev))
+    out = torch.empty_like(qq)
+    ws, ws_bytes = _workspace(dev, code, B, T, Hq, Hkv, D, S, 0)
+    _call("oc_tree_attention", dev, _ptr(qq), _ptr(k), _ptr(v), code, _ptr(table), stride, pages, PAGE, _ptr(lens),
+          _ptr(dk), _ptr(dv), _ptr(mask), int(mask_batched), B, T, Hq, Hkv, D, S, cap, scale, _ptr(out), code, _ptr(ws),
+          ws_bytes)
     return out if batched else out[0]
 
 
@@ -219,15 +212,13 @@ def chunk_attention(q, keys, values, lengths=None, *, causal=True, prefix=None, 
     sl = None
     if slopes is not None:
         sl = _on(slopes, device=dev, dtype=torch.float32)
-        if tuple(sl.shape) != (Hq,):
+        if sl.shape != (Hq,):
             raise ValueError(f"slopes {tuple(sl.shape)}, expected ({Hq},)")
     code = _lib.dtype_code(k)
-    with _Device(dev):
-        out = torch.empty_like(qq)
-        ws, ws_bytes = _workspace(qq, code, Hkv, S, 0)
-        _lib.call("oc_chunk_attention", _ptr(qq), _ptr(k), _ptr(v), code, _ptr(lens),
-                  int(bool(causal)), _ptr(pre), _ptr(docs), _ptr(sl), B, Sq, Hq, Hkv, D, S, cap, scale,
-                  _ptr(out), code, _ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+    out = torch.empty_like(qq)
+    ws, ws_bytes = _workspace(dev, code, B, Sq, Hq, Hkv, D, S, 0)
+    _call("oc_chunk_attention", dev, _ptr(qq), _ptr(k), _ptr(v), code, _ptr(lens), int(bool(causal)), _ptr(pre),
+          _ptr(docs), _ptr(sl), B, Sq, Hq, Hkv, D, S, cap, scale, _ptr(out), code, _ptr(ws), ws_bytes)
     return out if batched else out[0]
 
 
@@ -249,22 +240,20 @@ def accumulate_attention(q, keys, values, weights=None, lengths=None, *, cap=0.0
     w = None
     if weights is not None:
         w = _on(weights, device=dev, dtype=torch.float32)
-        if tuple(w.shape) != shape:
+        if w.shape != shape:
             raise ValueError(f"weights {tuple(w.shape)}, expected {shape}")
     if out_weights is not None:
         o = out_weights
         if not (isinstance(o, torch.Tensor) and o.device == dev and o.dtype == torch.float32 and o.is_contiguous() and
-                tuple(o.shape) == shape):
+                o.shape == shape):
             raise ValueError(f"out_weights must be a contiguous float32 tensor {shape} on {dev}")
     code = _lib.dtype_code(k)
-    with _Device(dev):
-        if out_weights is None:
-            out_weights = torch.empty(shape, dtype=torch.float32, device=dev)
-        out = torch.empty_like(qq)
-        ws, ws_bytes = _workspace(qq, code, Hkv, S, 1)
-        _lib.call("oc_accumulate_attention", _ptr(qq), _ptr(k), _ptr(v), code,
-                  _ptr(lens), _ptr(w), _ptr(out_weights), B, Sq, Hq, Hkv, D, S, cap, scale, _ptr(out),
-                  code, _ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+    if out_weights is None:
+        out_weights = torch.empty(shape, dtype=torch.float32, device=dev)
+    out = torch.empty_like(qq)
+    ws, ws_bytes = _workspace(dev, code, B, Sq, Hq, Hkv, D, S, 1)
+    _call("oc_accumulate_attention", dev, _ptr(qq), _ptr(k), _ptr(v), code, _ptr(lens), _ptr(w), _ptr(out_weights), B, Sq,
+          Hq, Hkv, D, S, cap, scale, _ptr(out), code, _ptr(ws), ws_bytes)
     return (out if batched else out[0]), out_weights
 
 
@@ -285,7 +274,7 @@ def evict_tokens(keys, values, weights, keep, recent=0, lengths=None):
     batched = k.dim() == 4
     if not batched:
         k, v, w = k.unsqueeze(0), v.unsqueeze(0), w.unsqueeze(0)
-    if k.dim() != 4 or k.shape != v.shape or tuple(w.shape) != (k.shape[0], k.shape[2], k.shape[1]):
+    if k.dim() != 4 or k.shape != v.shape or w.shape != (k.shape[0], k.shape[2], k.shape[1]):
         raise ValueError(f"incompatible shapes keys {tuple(k.shape)}, values {tuple(v.shape)}, weights "
                          f"{tuple(w.shape)}")
     B, S, H, D = k.shape
@@ -296,13 +285,11 @@ def evict_tokens(keys, values, weights, keep, recent=0, lengths=None):
         raise ValueError(f"recent {recent}, keep {keep}")
     dev, code = k.device, _lib.dtype_code(k)
     lens = _int_rows(lengths, (B,), dev, "lengths")
-    with _Device(dev):
-        ko = torch.empty((B, keep, H, D), dtype=k.dtype, device=dev)
-        vo = torch.empty_like(ko)
-        wo = torch.empty((B, H, keep), dtype=torch.float32, device=dev)
-        index = torch.empty((B, H, keep), dtype=torch.int32, device=dev)
-        left = torch.empty((B,), dtype=torch.int32, device=dev)
-        _lib.call("oc_evict_tokens", _ptr(k), _ptr(v), code, _ptr(w), _ptr(lens), B, S,
-                  H, D, keep, recent, _ptr(ko), _ptr(vo), _ptr(wo), _ptr(index), _ptr(left),
-                  _lib.stream_ptr(dev))
+    ko = torch.empty((B, keep, H, D), dtype=k.dtype, device=dev)
+    vo = torch.empty_like(ko)
+    wo = torch.empty((B, H, keep), dtype=torch.float32, device=dev)
+    index = torch.empty_like(wo, dtype=torch.int32)
+    left = torch.empty((B,), dtype=torch.int32, device=dev)
+    _call("oc_evict_tokens", dev, _ptr(k), _ptr(v), code, _ptr(w), _ptr(lens), B, S, H, D, keep, recent, _ptr(ko),
+          _ptr(vo), _ptr(wo), _ptr(index), _ptr(left))
     return (ko, vo, wo, index, left) if batched else (ko[0], vo[0], wo[0], index[0], left[0])
