@@ -177,8 +177,8 @@ struct TokWalk {
 // a token whose page lies outside the pool.
 __device__ __forceinline__ int64_t tok_kv_row(const TokArgs& a, int b, int j) {
   if (!a.table) return (int64_t)b * a.S + j;
-  const int p = a.table[(size_t)b * a.table_stride + j / a.page];
-  return p < 0 || p >= a.num_pages ? -1 : (int64_t)p * a.page + j % a.page;
+  const int n = j / a.page, p = a.table[(size_t)b * a.table_stride + n];
+  return p < 0 || p >= a.num_pages ? -1 : (int64_t)p * a.page + (j - n * a.page);
 }
 
 // Element offset of the first channel of output / query row r of (b, h).
@@ -199,17 +199,18 @@ int tok_mma(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st);
 int tok_mma_tile(int head_dim);  // keys of its tiles
 
 // The bfloat16 kernel on the tcgen05 tensor cores (oc_token_tc.cu) for
-// head_dim 64 and 128 and a positive scale; a unit is a pair of row tiles.
+// a positive scale; a unit is one or two row tiles.
 // prep: tok_tc_prep_bytes of scratch.
 struct TokTcShape {
-  int Gp, nhs, P, npt, npairs;  // heads and positions of a row tile; head groups, position tiles, pairs of row tiles
+  int Gp, nhs, P, npt;  // heads and positions of a row tile; head groups, position tiles
+  int per_unit, units;  // row tiles of a unit (one at head_dim 256, else two); units per (b, h)
 };
-TokTcShape tok_tc_shape(int q_len, int G);
-size_t tok_tc_prep_bytes(int batch, int q_len, int G, int seq_len);
+TokTcShape tok_tc_shape(int q_len, int G, int head_dim);
+size_t tok_tc_prep_bytes(int batch, int q_len, int G, int head_dim, int seq_len);
 int tok_tc(const char* fn, const TokArgs& a, int head_dim, void* prep, cudaStream_t st);
 
 // Column sums of the softmax on the tcgen05 tensor cores, from a.lse
-// (bfloat16, head_dim 64 or 128, contiguous keys, positive scale).
+// (bfloat16, contiguous keys, positive scale).
 int tok_tc_weights(const char* fn, const TokArgs& a, int head_dim, const float* w_in, float* w_out, cudaStream_t st);
 
 // Merge of the partials of the even cut (oc_token_attention.cu).

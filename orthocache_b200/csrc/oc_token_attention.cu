@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs 
   if (parts <= 1) return;
   // a unit of one row tile has two partials of 128 rows a piece (both halves of its
   // CTA worked on it)
-  const int sub = tc.Gp && tc.npt * tc.nhs == 1 ? 2 : 1, nparts = parts * sub;
+  const int sub = tc.per_unit == 2 && tc.npt * tc.nhs == 1 ? 2 : 1, nparts = parts * sub;
   for (int e = tid; e < nparts; e += kMergeThreads) {
     const int c = c0 + e / sub;
     s_part[e] = (2 * (c * a.hg + h % a.hg) + (cut.first(c) >= start ? 0 : 1)) * sub + e % sub;
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs 
     int r;
     bool real = rl < rows;
     if (tc.Gp) {
-      const int t = 2 * rt + rl / 128, i = t / tc.nhs * tc.P + rl % 128 / tc.Gp;
+      const int t = tc.per_unit * rt + rl / 128, i = t / tc.nhs * tc.P + rl % 128 / tc.Gp;
       real = real && t < tc.npt * tc.nhs && i < a.Sq;
       r = i * a.G + t % tc.nhs * tc.Gp + rl % 128 % tc.Gp;
     } else {
@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(256) tok_sum_kernel(const TokArgs a, const flo
 }  // namespace
 
 int tok_merge(const TokArgs& a, int head_dim, bool tc, cudaStream_t st) {
-  const TokTcShape shape = tc ? tok_tc_shape(a.Sq, a.G) : TokTcShape{};
+  const TokTcShape shape = tc ? tok_tc_shape(a.Sq, a.G, head_dim) : TokTcShape{};
   return head_dim == 64 ? launch_merge<64>(a, shape, st)
                         : head_dim == 128 ? launch_merge<128>(a, shape, st) : launch_merge<256>(a, shape, st);
 }
@@ -572,7 +572,8 @@ inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // bfloat16 the m16n8k16 kernel (16, 32 or 64 rows, what the rows fill) or the
 // tcgen05 one, from the rows on where it is the faster (a tree over 64K tokens, 8
 // KV heads: at 128 channels 32 rows take 69 and 77 us, 64 rows 108 and 77; at 64
-// channels 48 rows 54 and 56, 96 rows 75 and 58).
+// channels 48 rows 54 and 56, 96 rows 75 and 58; 32K tokens, 16 heads of 256
+// channels: 16 rows 114 and 134, 24 rows 187 and 134).
 //
 // Cut: with few units (row tile, batch row, KV head) for the GPU, all their key
 // tiles are dealt out evenly over one (tcgen05) or two CTAs per SM, so that
@@ -595,12 +596,13 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
   TokPlan p;
   const int G = q_heads / kv_heads;
   const int64_t R = (int64_t)q_len * G;
-  p.tc = dtype == OC_BF16 && head_dim <= 128 && R > (head_dim == 128 ? 32 : 64) && scale > 0.f;
+  p.tc = dtype == OC_BF16 && R > (head_dim == 64 ? 64 : head_dim == 128 ? 32 : 16) && scale > 0.f;
   int64_t slots = device_sm_count();
   if (p.tc) {
     p.row_tile = 128;
-    p.nrt = tok_tc_shape(q_len, G).npairs;
-    p.unit_rows = 256;
+    const TokTcShape shape = tok_tc_shape(q_len, G, head_dim);
+    p.nrt = shape.units;
+    p.unit_rows = 128 * shape.per_unit;
     p.tile = 128;
   } else {
     p.row_tile = R <= 16 ? 16 : R <= 32 ? (dtype == OC_BF16 ? 32 : 16) : 64;
@@ -631,7 +633,7 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
   p.o_off = off;
   off += up256(parts * head_dim * sizeof(float));
   p.prep_off = off;
-  if (p.tc) off += up256(tok_tc_prep_bytes(batch, q_len, G, seq_len));
+  if (p.tc) off += up256(tok_tc_prep_bytes(batch, q_len, G, head_dim, seq_len));
   p.logit_off = off;
   p.logit_stride = 0;
   if (lse && dtype == OC_BF16 && !p.tc && R <= kLogitRows) {
@@ -759,7 +761,7 @@ int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void*
     if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_sum_kernel: %s", cudaGetErrorString(e));
     return OC_OK;
   }
-  if (dtype == OC_BF16 && head_dim <= 128 && a.scale > 0.f) return tok_tc_weights(fn, a, head_dim, w_in, w_out, st);
+  if (dtype == OC_BF16 && a.scale > 0.f) return tok_tc_weights(fn, a, head_dim, w_in, w_out, st);
   return dtype == OC_BF16 ? dispatch_weights<__nv_bfloat16>(a, head_dim, w_in, w_out, st)
                           : dispatch_weights<float>(a, head_dim, w_in, w_out, st);
 }

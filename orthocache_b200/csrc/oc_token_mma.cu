@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
       const int64_t row0 = draft ? (int64_t)b * a.Sq + j0 : tok_kv_row(a, b, j0);  // a tile lies inside one page
       const char* kp = static_cast<const char*>(draft ? a.dk : a.k);
       const char* vp = static_cast<const char*>(draft ? a.dv : a.v);
+      if (tid == 0) s_int[6 + t % ST] = row0 < 0;  // a page outside the pool
       const int64_t off0 = (row0 + r0) * row_bytes + (h * D + c_mine * 8) * 2;
       if (!draft && !a.docs && row0 >= 0 && j0 + TOK <= len) {
         kp += off0;
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
 #pragma unroll
       for (int kk = 0; kk < KQ; ++kk) ldsm_x4(qf[kk], sbase + C::kQOff + swz<RT>(q_row, 2 * kk + q_c));
     }
-    const bool draft = t >= ncache;
+    const bool draft = t >= ncache, hole = s_int[6 + t % ST] != 0;
     const int j0 = (draft ? (d0 + t - ncache) * TOK : t0 + t * TOK) + wt * C::TPW;
 
     // scores of this warp's tokens: B fragments are 8 tokens x 16 channels of
@@ -295,15 +296,14 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
           const uint32_t bits = j < kMaxNodes ? tree_bits[(wr * 16 + g + (y >> 1) * 8) * (kMaxNodes / 32) + (j >> 5)] : 0;
           if (!(bits >> (j & 31) & 1)) s[n][y] = -INFINITY;
         }
-    } else if (a.docs || a.table || j0 + C::TPW > min_hi) {
-      const bool page_ok = !a.table || tok_kv_row(a, b, min(j0, a.S - 1)) >= 0;
+    } else if (a.docs || hole || j0 + C::TPW > min_hi) {
 #pragma unroll
       for (int n = 0; n < C::NT; ++n)
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
           const int j = j0 + n * 8 + c2 + (y & 1);
           const TokRow& w = row[y >> 1];
-          if (!(page_ok && j < w.hi && (!a.docs || a.docs[(size_t)b * a.S + j] == w.doc))) s[n][y] = -INFINITY;
+          if (!(!hole && j < w.hi && (!a.docs || a.docs[(size_t)b * a.S + j] == w.doc))) s[n][y] = -INFINITY;
         }
     }
 

@@ -1,43 +1,46 @@
 // Token-level attention on the 5th-generation tensor cores (bfloat16, head_dim
-// 64 or 128): drafted trees and query chunks with enough rows per KV head to
+// 64, 128 or 256): drafted trees and query chunks with enough rows per KV head to
 // fill 128-row tiles.
 //
-// Mathematics and masks: oc_token.cuh.  Bound by the tensor cores and the
-// exponentials together: 4 D multiply-adds and one exponential (with a cap, a
-// five-term polynomial more) per row and key, 64 D bytes of keys and values per
-// 128-row tile and key.
+// Mathematics and masks: oc_token.cuh.  Per row and key 4 D multiply-adds and one
+// exponential (with a cap, a polynomial more); per 128-row tile and key 4 D bytes
+// of keys and values.  At D = 128 the products of two row tiles and a key tile
+// take 2,048 cycles and their exponentials as many on the MUFU unit; a pair takes
+// about 3,200.  Measured: 4 x 2048 rows x 32 heads on 8K keys without a mask 0.92
+// ms = 1,200 TFLOP/s (0.72 of the measured bf16 burst peak), causal on 32K 1,160,
+// capped 925-950; D = 64 690; D = 256 705; few rows on a long cache read it at 5
+// to 5.4 TB/s.
 //
 // Layout (one persistent CTA of 384 threads per SM):
 //   * a row tile is 128 rows of one KV head: Gp neighbouring heads (the largest
 //     power of two that divides G = Hq / Hkv) x 128 / Gp query positions, so
 //     that few drafted tokens of many heads still fill a tile; a work unit is two
-//     row tiles that share every key tile, and one chunk of the keys;
-//   * warp 8 loads by TMA (128-byte swizzle): the two query tiles, then K and V
-//     tiles of 128 tokens into a ring; from the cache, its pages, or the drafted
-//     tokens;
-//   * a thread of warp 17 issues the tcgen05.mma of tile 0, one of warp 18 those of
-//     tile 1: per key tile j PV_t(j-1), then S_t(j) (S_t = Q_t K^T into tensor
-//     memory, O_t += P_t V with P_t from tensor memory), so that one tile's
-//     softmax runs under the other's products, and the next unit's first S under
-//     the output of the last.  One thread for both tiles left the tensor cores
-//     idle at each of its waits (about 170 cycles apiece; period of a pair of
-//     tiles 4,300 cycles at head_dim 128 against 2,048 of products);
-//   * V of tokens that nobody may see (behind the sequence, padding) is
-//     overwritten with zeros before the tile is multiplied: their weights are
-//     zero, but zero times whatever memory holds may not be;
+//     row tiles that share every key tile (at D = 256, where O alone takes 256
+//     columns of tensor memory, one), over all keys that its rows may see or a run
+//     of them.  When there is one row tile in all (dual), both halves of the CTA
+//     work on it, on the even and the odd key tiles, as if on two tiles;
+//   * warp 8 loads by TMA (128-byte swizzle): the query tiles, then K and V tiles
+//     of 128 tokens into a ring; from the cache, its pages, or the drafted
+//     tokens.  The key tiles come nearest first;
+//   * warp 9 issues the tcgen05.mma: per key tile j and row tile t PV_t(j-1), then
+//     S_t(j) (S_t = Q_t K^T into tensor memory, O_t += P_t V with P_t from tensor
+//     memory over the scores), so that one tile's softmax runs under the other's
+//     products, and the next unit's first S under the output of the last.  Two
+//     threads, one per tile, fell into step and were slower (1,380 us against 1,075
+//     on the 8K case above);
+//   * warp 10 overwrites V of tokens that nobody may see (behind the sequence,
+//     padding) with zeros before the tile is multiplied: their weights are zero,
+//     but zero times whatever memory holds may not be;
 //   * warps 0-3 / 4-7 are the softmax of tile 0 / 1, a thread per row (setmaxnreg
-//     moves registers to them from the other warps); most tiles go through 32
-//     scores at a time: load, scale, 2^x, sum, pack.  No maximum is sought there
-//     (kRefMax below).  P is rounded to bfloat16 (half a step, 2^-8 of each
-//     weight); row sums are float32, taken before the rounding.
-//   * only key tiles that some row's limit or a document border cuts are masked
-//     element by element; tiles without a visible key are never loaded (causal
-//     limits; with documents, the span of tiles that hold a unit's documents,
-//     found by two small kernels beforehand).
-//   * cap tanh(x / cap): the score is odd in x, y = x (1 + u (a1 + ...)), u =
-//     (x / cap)^2, a least-squares fit of tanh(z) / z in z^2 on |z| <= 0.6 with
-//     equalised error (2.0e-8); a warp whose scores go beyond 0.6 cap takes cap -
-//     2 cap / (1 + e^(2 z)) instead, two MUFU operations a score more.
+//     moves registers to them from the other warps): 128 scores from tensor
+//     memory, scale, 2^x, sum, pack.  No maximum is sought (kRefMax below).  P is
+//     rounded to bfloat16 (half a step, 2^-8 of each weight); row sums are float32,
+//     taken before the rounding.  Sixteen warps with half a row each were slower
+//     without a cap (1,065 us against 935) and no faster with one;
+//   * only key tiles that some row's limit, a document border or the drafted tree
+//     cuts are masked, by a bit per key; tiles without a visible key are never
+//     loaded (causal limits; with documents, the span of tiles that hold a unit's
+//     documents, found by two small kernels beforehand).
 // Every wait is bounded; one that gives up sets a status and an abort flag, and
 // the CTA frees its tensor memory and returns.
 #include <cuda.h>
@@ -61,12 +64,15 @@ constexpr int kTmemCols = 512;
 template <int D> struct TcCfg {
   static constexpr int kTileBytes = kRows * D * 2;
   static constexpr int kBox = kRows * 128;               // one 128-row x 64-channel box
-  static constexpr int kSlots = D == 128 ? 5 : 10;
+  static constexpr int kPerUnit = D == 256 ? 1 : 2;      // row tiles of a unit
+  static constexpr int kSlots = D == 256 ? 2 : D == 128 ? 5 : 10;
+  static constexpr int kKeyTiles = D == 256 ? 1 : 2;     // column sums: key tiles of a unit
+  static constexpr int kQuerySlots = D == 256 ? 2 : 4;   // column sums: ring of query tiles
 };
 
 template <int D>
 struct TcSmem {
-  unsigned char q[2][TcCfg<D>::kTileBytes];
+  unsigned char q[TcCfg<D>::kPerUnit][TcCfg<D>::kTileBytes];
   unsigned char kv[TcCfg<D>::kSlots][TcCfg<D>::kTileBytes];
   uint64_t kv_full[TcCfg<D>::kSlots + 1], kv_empty[TcCfg<D>::kSlots + 1];
   uint64_t q_full, q_empty;
@@ -80,7 +86,8 @@ struct TcSmem {
 
 struct TcArgs {
   TokArgs t;
-  int Gp, nhs, P, tiles, npairs, units;  // row tiles per (b, h): nhs head groups x position tiles of P
+  int Gp, nhs, P, tiles;  // row tiles per (b, h): nhs head groups x position tiles of P
+  int per_unit, upb, units;  // row tiles of a unit, units per (b, h), in all
   const uint4* tree_bits;   // [(b, node)][2] ancestor bits; row T of each batch row: seen by any node
   const int2* key_docs;     // [(b, key tile)] least and largest document
   const int4* query_docs;   // [(b, position tile)] least, largest document; first key tile, last + 1
@@ -107,17 +114,17 @@ __device__ __forceinline__ int tc_deal(int k) {
 __device__ __forceinline__ TcUnit tc_unit(const TcArgs& x, const TokSeg& seg) {
   const TokArgs& a = x.t;
   TcUnit w;
-  const int pair = x.npairs == 1 ? 0 : seg.unit % x.npairs;
+  const int first_tile = x.upb == 1 ? 0 : seg.unit % x.upb * x.per_unit;
   w.b = seg.b;
-  w.h = x.npairs == 1 ? seg.unit : seg.unit / x.npairs;
+  w.h = x.upb == 1 ? seg.unit : seg.unit / x.upb;
   w.bh = w.b * a.Hkv + w.h;
   w.part = seg.part;
   w.len = tok_len(a, w.b);
-  w.ntile = 2 * pair + 1 < x.tiles ? 2 : 1;
+  w.ntile = x.per_unit == 2 && first_tile + 1 < x.tiles ? 2 : 1;
   int first = INT32_MAX, last = 0, top = 0;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int r = 2 * pair + t, pt = x.nhs == 1 ? r : r / x.nhs;
+    const int r = first_tile + t, pt = x.nhs == 1 ? r : r / x.nhs;
     w.hs[t] = r - pt * x.nhs;
     w.p0[t] = pt * x.P;
     w.min_hi[t] = 0;
@@ -152,7 +159,7 @@ __device__ __forceinline__ TcUnit tc_unit(const TcArgs& x, const TokSeg& seg) {
   w.ncache = max(0, min(last, seg.t1) - w.jt0);
   w.d0 = max(seg.t0 - nct, 0);
   w.n = w.ncache + (a.dk && seg.t1 > nct ? min(seg.t1 - nct, (a.Sq + kTok - 1) / kTok) - w.d0 : 0);
-  w.dual = x.tiles == 1 && seg.part >= 0;
+  w.dual = x.per_unit == 2 && x.tiles == 1 && seg.part >= 0;
   return w;
 }
 
@@ -178,7 +185,7 @@ struct TcWalk {
         u = tc_deal(k++);
       }
       const int BH = x.t.B * x.t.Hkv, bh = u % BH;  // the rows with most keys first
-      seg = TokSeg{bh / x.t.Hkv, bh % x.t.Hkv * x.npairs + x.npairs - 1 - u / BH, 0, INT32_MAX, -1};
+      seg = TokSeg{bh / x.t.Hkv, bh % x.t.Hkv * x.upb + x.upb - 1 - u / BH, 0, INT32_MAX, -1};
     }
     w = tc_unit(x, seg);
     return true;
@@ -609,7 +616,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
       tc_fence_after();
     }
     if (l == 0.f) m_used = -INFINITY;
-    const int64_t part = (int64_t)w.part * 256 + t * 128 + rl;
+    const int64_t part = (int64_t)w.part * (128 * TcCfg<D>::kPerUnit) + t * 128 + rl;
     const int64_t at = tok_q_offset(a, w.b, w.h, real ? r : 0, D);
     if (real) {
       if (w.part >= 0) {
@@ -623,7 +630,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
       // float32 rows leave in the accumulator layout: four lanes write 32 bytes of
       // a row (a thread writing its own row 16 bytes at a time takes 32 sectors an
       // instruction)
-      const int64_t base = (int64_t)w.part * 256 + t * 128 + (threadIdx.x & 96);
+      const int64_t base = part - rl + (threadIdx.x & 96);
 #pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         const int g = half * 16 + (lane >> 2);
@@ -681,11 +688,11 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
 // flight.
 template <int D>
 __device__ __forceinline__ unsigned char* tc_ring(TcSmem<D>& sm, const TcArgs& x) {
-  return x.tiles == 1 ? sm.q[1] : sm.kv[0];
+  return TcCfg<D>::kPerUnit == 2 && x.tiles == 1 ? sm.q[TcCfg<D>::kPerUnit - 1] : sm.kv[0];
 }
 template <int D>
 __device__ __forceinline__ uint32_t tc_slots(const TcArgs& x) {
-  return TcCfg<D>::kSlots + (x.tiles == 1 ? 1 : 0);
+  return TcCfg<D>::kSlots + (TcCfg<D>::kPerUnit == 2 && x.tiles == 1 ? 1 : 0);
 }
 
 template <int D>
@@ -710,7 +717,7 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
     q_ph ^= 1;
     mbar_expect_tx(&sm.q_full, (uint32_t)(w.ntile * C::kTileBytes));
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < C::kPerUnit; ++t)
       if (t < w.ntile)
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
@@ -855,7 +862,7 @@ __device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
     const bool cut = (w.jt0 + w.ncache) * kTok > w.len && w.ncache > 0;
     if (!bar_wait_warp(&sm.abort, &sm.q_full, q_ph)) return;
     q_ph ^= 1;
-    if (dual) {
+    if (C::kPerUnit == 2 && dual) {
       // half t takes the key tiles t, t + 2, ...: K of tile j is load 2 j of the
       // unit, V load 2 j + 1
       for (int j = 0; j < n + 2; ++j) {
@@ -907,7 +914,7 @@ __device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
     tc_fence_after();
     // S of the first key tile
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < C::kPerUnit; ++t) {
       if (t < ntile && elect_one()) {
         scores(t, qd0 + t * (C::kTileBytes >> 4), kp);
         umma_commit(&sm.s_full[t]);
@@ -925,7 +932,7 @@ __device__ void tc_mma(TcSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
       if ((always || (cut && j == 1)) && !wait_clean(vp)) return;
       if (j < n && !wait_full(kp)) return;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < C::kPerUnit; ++t) {
         if (t >= ntile) break;
         if (j == 1) {  // the softmax has read the previous unit's O_t
           if (!bar_wait_warp(&sm.abort, &sm.o_free[t], o_ph[t])) return;
@@ -1036,15 +1043,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 // that share every query tile; two score buffers per key tile in tensor memory
 // let the products run ahead of the exponentials.
 // ---------------------------------------------------------------------------
-constexpr int kWqSlots = 4;
-
 template <int D>
 struct TwSmem {
-  unsigned char k[2][TcCfg<D>::kTileBytes];
-  unsigned char q[kWqSlots][TcCfg<D>::kTileBytes];
-  float lse[kWqSlots][kRows];
+  unsigned char k[TcCfg<D>::kKeyTiles][TcCfg<D>::kTileBytes];
+  unsigned char q[TcCfg<D>::kQuerySlots][TcCfg<D>::kTileBytes];
+  float lse[TcCfg<D>::kQuerySlots][kRows];
   uint64_t k_full, k_empty;
-  uint64_t q_full[kWqSlots], q_empty[kWqSlots];
+  uint64_t q_full[TcCfg<D>::kQuerySlots], q_empty[TcCfg<D>::kQuerySlots];
   uint64_t s_full[2][2], s_empty[2][2];
   uint64_t drain;
   uint32_t tmem_base;
@@ -1055,6 +1060,7 @@ struct TwUnit {
   int b, h, bh, len, j0, ntile, r0, n;  // first key, key tiles with keys, first row tile, row tiles
 };
 
+template <int D>
 __device__ __forceinline__ TwUnit tw_unit(const TcArgs& x, int u) {
   const TokArgs& a = x.t;
   TwUnit w;
@@ -1063,8 +1069,8 @@ __device__ __forceinline__ TwUnit tw_unit(const TcArgs& x, int u) {
   w.b = w.bh / a.Hkv;
   w.h = w.bh % a.Hkv;
   w.len = tok_len(a, w.b);
-  w.j0 = u / BH * 2 * kTok;  // the first keys, which most rows see, come first
-  w.ntile = w.j0 + kTok < w.len ? 2 : 1;
+  w.j0 = u / BH * TcCfg<D>::kKeyTiles * kTok;  // the first keys, which most rows see, come first
+  w.ntile = TcCfg<D>::kKeyTiles == 2 && w.j0 + kTok < w.len ? 2 : 1;
   const int before = w.j0 - (w.len - a.Sq);  // query positions that lie before the unit's first key
   w.r0 = (before > 0 ? before / x.P : 0) * x.nhs;
   w.n = w.j0 < w.len ? max(0, x.tiles - w.r0) : 0;
@@ -1078,13 +1084,13 @@ __device__ void tw_producer(TwSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
   const int lane = threadIdx.x & 31;
   uint32_t k_ph = 0, L = 0;
   auto drain = [&]() {  // let the copies in flight land (bounded)
-    for (uint32_t s = 0; s < kWqSlots && s < L; ++s) mbar_wait(&sm.q_full[s], ((L - s - 1) / kWqSlots) & 1);
+    for (uint32_t s = 0; s < TcCfg<D>::kQuerySlots && s < L; ++s) mbar_wait(&sm.q_full[s], ((L - s - 1) / TcCfg<D>::kQuerySlots) & 1);
     mbar_wait(&sm.k_full, k_ph ^ 1);
   };
   for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
     const int u = tc_deal(k);
     if (u >= x.units) continue;
-    const TwUnit w = tw_unit(x, u);
+    const TwUnit w = tw_unit<D>(x, u);
     if (w.n == 0) continue;
     if (!bar_wait_warp(&sm.abort, &sm.k_empty, k_ph ^ 1)) return drain();
     k_ph ^= 1;
@@ -1103,8 +1109,8 @@ __device__ void tw_producer(TwSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
         const int col = 32 * k + lane, pos = p0 + col / x.Gp;
         lse[k] = pos < a.Sq ? a.lse[(int64_t)w.bh * a.R + (int64_t)pos * a.G + hs * x.Gp + col % x.Gp] : INFINITY;
       }
-      const uint32_t slot = L % kWqSlots;
-      if (!bar_wait_warp(&sm.abort, &sm.q_empty[slot], ((L / kWqSlots) & 1) ^ 1)) return drain();
+      const uint32_t slot = L % TcCfg<D>::kQuerySlots;
+      if (!bar_wait_warp(&sm.abort, &sm.q_empty[slot], ((L / TcCfg<D>::kQuerySlots) & 1) ^ 1)) return drain();
 #pragma unroll
       for (int k = 0; k < 4; ++k) sm.lse[slot][32 * k + lane] = lse[k];
       if (lane == 0) {
@@ -1130,7 +1136,7 @@ __device__ void tw_mma(TwSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
   for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
     const int u = tc_deal(k);
     if (u >= x.units) continue;
-    const TwUnit w = tw_unit(x, u);
+    const TwUnit w = tw_unit<D>(x, u);
     const int n = __shfl_sync(0xffffffffu, w.n, 0), ntile = __shfl_sync(0xffffffffu, w.ntile, 0);
     if (n == 0) continue;
     if (!bar_wait_warp(&sm.abort, &sm.k_full, k_ph)) return;
@@ -1139,7 +1145,7 @@ __device__ void tw_mma(TwSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
       const uint64_t qd = qd0 + slot * (C::kTileBytes >> 4);
       if (!bar_wait_warp(&sm.abort, &sm.q_full[slot], ph)) return;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < C::kKeyTiles; ++t) {
         if (t >= ntile) break;
         const uint32_t buf = use[t] & 1;
         if (!bar_wait_warp(&sm.abort, &sm.s_empty[t][buf], ((use[t] >> 1) & 1) ^ 1)) return;
@@ -1159,7 +1165,7 @@ __device__ void tw_mma(TwSmem<D>& sm, const TcArgs& x, uint32_t tmem) {
         }
         __syncwarp();
       }
-      if (++slot == kWqSlots) {
+      if (++slot == TcCfg<D>::kQuerySlots) {
         slot = 0;
         ph ^= 1;
       }
@@ -1178,13 +1184,13 @@ __device__ void tw_sum(TwSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem, con
   for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
     const int u = tc_deal(k);
     if (u >= x.units) continue;
-    const TwUnit w = tw_unit(x, u);
+    const TwUnit w = tw_unit<D>(x, u);
     const int j = w.j0 + t * kTok + kl;
     uint64_t acc[4] = {0, 0, 0, 0};
     float edge = 0.f;
     for (int i = 0; i < w.n; ++i, ++L) {
-      const uint32_t slot = L % kWqSlots;
-      if (!bar_wait_warp(&sm.abort, &sm.q_full[slot], (L / kWqSlots) & 1)) return;  // the denominators
+      const uint32_t slot = L % TcCfg<D>::kQuerySlots;
+      if (!bar_wait_warp(&sm.abort, &sm.q_full[slot], (L / TcCfg<D>::kQuerySlots) & 1)) return;  // the denominators
       if (t < w.ntile) {
         const uint32_t buf = use & 1;
         if (!bar_wait_warp(&sm.abort, &sm.s_full[t][buf], (use >> 1) & 1)) return;
@@ -1235,7 +1241,7 @@ __device__ void tw_sum(TwSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem, con
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.q_empty[slot]);
     }
-    if (j < a.S) {
+    if (t < TcCfg<D>::kKeyTiles && j < a.S) {
       const int64_t at = (int64_t)w.bh * a.S + j;
       float q[8];
 #pragma unroll
@@ -1257,7 +1263,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(&sm.k_full, 1);
     mbar_init(&sm.k_empty, 1);
-    for (int i = 0; i < kWqSlots; ++i) {
+    for (int i = 0; i < TcCfg<D>::kQuerySlots; ++i) {
       mbar_init(&sm.q_full[i], 32);  // 31 lanes, and the one that announces the copy
       mbar_init(&sm.q_empty[i], 9);  // eight summing warps and the tensor cores
     }
@@ -1427,34 +1433,36 @@ int launch_tc_form(const CUtensorMap (&m)[5], const TcArgs& x, cudaStream_t st) 
 }  // namespace
 
 // Row tiles: Gp heads x P positions.
-TokTcShape tok_tc_shape(int q_len, int G) {
+TokTcShape tok_tc_shape(int q_len, int G, int head_dim) {
   TokTcShape s;
   s.Gp = 1;
   while (s.Gp < kRows && G % (2 * s.Gp) == 0) s.Gp *= 2;
   s.nhs = G / s.Gp;
   s.P = kRows / s.Gp;
   s.npt = (q_len + s.P - 1) / s.P;
-  s.npairs = (s.npt * s.nhs + 1) / 2;
+  s.per_unit = head_dim == 256 ? TcCfg<256>::kPerUnit : TcCfg<128>::kPerUnit;
+  s.units = (s.npt * s.nhs + s.per_unit - 1) / s.per_unit;
   return s;
 }
 
-size_t tok_tc_prep_bytes(int batch, int q_len, int G, int seq_len) {
-  const TokTcShape s = tok_tc_shape(q_len, G);
+size_t tok_tc_prep_bytes(int batch, int q_len, int G, int head_dim, int seq_len) {
+  const TokTcShape s = tok_tc_shape(q_len, G, head_dim);
   const size_t tree = q_len <= kMaxNodes ? (size_t)batch * (q_len + 1) * 32 : 0;
   const size_t docs = (size_t)batch * s.npt * sizeof(int4) + (size_t)batch * ((seq_len + kTok - 1) / kTok) * sizeof(int2);
   return tree > docs ? tree : docs;
 }
 
 int tok_tc(const char* fn, const TokArgs& a, int head_dim, void* prep, cudaStream_t st) {
-  const TokTcShape s = tok_tc_shape(a.Sq, a.G);
+  const TokTcShape s = tok_tc_shape(a.Sq, a.G, head_dim);
   TcArgs x = {};
   x.t = a;
   x.Gp = s.Gp;
   x.nhs = s.nhs;
   x.P = s.P;
   x.tiles = s.npt * s.nhs;
-  x.npairs = s.npairs;
-  x.units = a.B * a.Hkv * s.npairs;
+  x.per_unit = s.per_unit;
+  x.upb = s.units;
+  x.units = a.B * a.Hkv * s.units;
   x.nkt = (a.S + kTok - 1) / kTok;
   x.npt = s.npt;
   x.k_in = a.cap > 0.f ? a.scale / a.cap : 0.f;
@@ -1490,7 +1498,8 @@ int tok_tc(const char* fn, const TokArgs& a, int head_dim, void* prep, cudaStrea
   } else if (a.docs) {
     x.t.docs = nullptr;  // an empty cache: no row sees anything
   }
-  return head_dim == 64 ? launch_tc_form<64>(m, x, st) : launch_tc_form<128>(m, x, st);
+  if (head_dim == 64) return launch_tc_form<64>(m, x, st);
+  return head_dim == 128 ? launch_tc_form<128>(m, x, st) : launch_tc_form<256>(m, x, st);
 }
 
 namespace {
@@ -1511,14 +1520,15 @@ int launch_tw(const CUtensorMap& mq, const CUtensorMap& mk, const TcArgs& x, con
 }  // namespace
 
 int tok_tc_weights(const char* fn, const TokArgs& a, int head_dim, const float* w_in, float* w_out, cudaStream_t st) {
-  const TokTcShape s = tok_tc_shape(a.Sq, a.G);
+  const TokTcShape s = tok_tc_shape(a.Sq, a.G, head_dim);
   TcArgs x = {};
   x.t = a;
   x.Gp = s.Gp;
   x.nhs = s.nhs;
   x.P = s.P;
   x.tiles = s.npt * s.nhs;
-  const int64_t units = (int64_t)((a.S + 2 * kTok - 1) / (2 * kTok)) * a.B * a.Hkv;
+  const int keys = kTok * (head_dim == 256 ? TcCfg<256>::kKeyTiles : TcCfg<128>::kKeyTiles);
+  const int64_t units = (int64_t)((a.S + keys - 1) / keys) * a.B * a.Hkv;
   OC_REQUIRE(units < INT32_MAX, OC_ERR_SHAPE, "%s: too many work units", fn);
   x.units = (int)units;
   x.k_in = a.cap > 0.f ? a.scale / a.cap : 0.f;
@@ -1526,11 +1536,12 @@ int tok_tc_weights(const char* fn, const TokArgs& a, int head_dim, const float* 
   int rc = tc_map(&mq, a.q, head_dim, a.Hq, (int64_t)a.B * a.Sq, s.Gp, s.P, fn);
   if (!rc) rc = tc_map(&mk, a.k, head_dim, a.Hkv, (int64_t)a.B * a.S, 1, kTok, fn);
   if (rc) return rc;
+  const bool cap = a.cap > 0.f;
   if (head_dim == 64)
-    return a.cap > 0.f ? launch_tw<64, true>(mq, mk, x, w_in, w_out, st)
-                       : launch_tw<64, false>(mq, mk, x, w_in, w_out, st);
-  return a.cap > 0.f ? launch_tw<128, true>(mq, mk, x, w_in, w_out, st)
-                     : launch_tw<128, false>(mq, mk, x, w_in, w_out, st);
+    return cap ? launch_tw<64, true>(mq, mk, x, w_in, w_out, st) : launch_tw<64, false>(mq, mk, x, w_in, w_out, st);
+  if (head_dim == 128)
+    return cap ? launch_tw<128, true>(mq, mk, x, w_in, w_out, st) : launch_tw<128, false>(mq, mk, x, w_in, w_out, st);
+  return cap ? launch_tw<256, true>(mq, mk, x, w_in, w_out, st) : launch_tw<256, false>(mq, mk, x, w_in, w_out, st);
 }
 
 int wait_limit_token(unsigned long long ns) { return set_wait_limit_here(ns); }

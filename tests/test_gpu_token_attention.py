@@ -477,3 +477,84 @@ def test_refusals():
     x = _randn(g, 1, 257, 2, 128)
     with pytest.raises(oc._lib.OrthoCacheError, match="256"):
         oc.tree_attention(x, k[:1], v[:1], x, x, wide)
+
+
+# ---------------------------------------------------------------------------
+# the cut of the keys over CTAs, and the softmax's reference point
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,D,Hq,Hkv", [(BF, 128, 8, 2), (BF, 128, 3, 3), (BF, 64, 16, 1), (BF, 256, 4, 2),
+                                            (F32, 64, 6, 2)])
+@pytest.mark.parametrize("T", [1, 11, 70])
+def test_ragged_batch_cut_over_many_ctas(T, D, Hq, Hkv, dtype):
+    """Sequences of very different lengths (none, one token, thousands), whose
+    key tiles are dealt out over all CTAs; every batch row, head and node."""
+    import orthocache_b200 as oc
+    g = _gen(T + D)
+    lengths = [7000, 1, 0, 2500, 129, 64]
+    B, S = len(lengths), 7040
+    q, k, v = _qkv(g, B, T, Hq, Hkv, S, D, dtype)
+    dk, dv = _randn(g, B, T, Hkv, D, dtype=dtype), _randn(g, B, T, Hkv, D, dtype=dtype)
+    mask = R.random_tree(T, g)
+    kd, vd = _dirty(k, v, lengths)
+    lens = torch.tensor(lengths)
+    out = oc.tree_attention(q, kd, vd, dk, dv, mask, lens)
+    vis = torch.cat([(torch.arange(S)[None] < lens[:, None])[:, None].expand(B, T, S), mask.expand(B, T, T)], 2).cuda()
+    want, _, tol, _ = R.attend(q, torch.cat([kd, dk], 1), torch.cat([vd, dv], 1), vis)
+    R.check(out, want, tol, "tree")
+    out, w = oc.accumulate_attention(q, kd, vd, None, lens)
+    want, p, tol, rel = R.attend(q, kd, vd, R.chunk_visible(lengths, T, S).cuda())
+    R.check(out, want, tol, "chunk")
+    sums, stol = R.column_sums(p, rel, Hkv)
+    R.check(w, sums, stol, "weights")
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("kw", [{}, dict(cap=100.0), dict(slopes=-0.6), dict(slopes=0.9), dict(slopes=-0.2, cap=20.0),
+                                dict(slopes=0.3, prefix=[500]), dict(causal=False, slopes=-0.4)])
+@pytest.mark.parametrize("N", [3, 160])
+def test_scores_that_grow_away_from_the_query(N, kw, D):
+    """The largest scores lie farthest from the query (by the keys, or by a
+    negative bias): a softmax that takes its reference point from the nearest
+    keys has to move it, by far more than float32 holds."""
+    import orthocache_b200 as oc
+    kw = dict(kw)
+    g = _gen(N + D)
+    B, Hq, Hkv, S = 1, 4, 2, 900
+    q, k, v = _qkv(g, B, N, Hq, Hkv, S, D, BF)
+    # one direction that every query shares; the keys have the more of it the farther back they lie
+    q = q * 0.3
+    q[..., 0] = 24.0
+    k[..., 0] = (torch.linspace(120.0, -120.0, S).view(1, S, 1) * D ** 0.5 / 11.3).to(BF).cuda()
+    bias = slopes = None
+    if "slopes" in kw:
+        slopes = kw.pop("slopes") * torch.linspace(0.5, 1.0, Hq)
+        bias = R.distance_bias([S], N, S, slopes).cuda()
+    prefix = kw.pop("prefix", None)
+    out = oc.chunk_attention(q, k, v, slopes=slopes, prefix=None if prefix is None else torch.tensor(prefix), **kw)
+    vis = R.chunk_visible([S], N, S, kw.get("causal", True), prefix).cuda()
+    want, _, tol, _ = R.attend(q, k, v, vis, cap=kw.get("cap", 0.0), bias=bias)
+    R.check(out, want, tol)
+
+
+def test_padding_fills_whole_tiles():
+    """Documents separated by padding longer than a tile, with queries of the
+    padding among the rows of a tile."""
+    import orthocache_b200 as oc
+    g = _gen(77)
+    B, N, Hq, Hkv, S, D = 1, 1200, 2, 2, 1200, 128
+    q, k, v = _qkv(g, B, N, Hq, Hkv, S, D, BF)
+    docs = torch.full((B, S), -1, dtype=torch.int32)
+    docs[:, :200], docs[:, 700:] = 5, 9
+    docs[:, 900:1190] = 5
+    k[docs.cuda() < 0] = math.nan
+    v[docs.cuda() < 0] = math.inf
+    out = oc.chunk_attention(q, k, v, documents=docs)
+    want, _, tol, _ = R.attend(q, k, v, R.chunk_visible([S], N, S, True, None, docs).cuda())
+    R.check(out, want, tol)
+    assert not out[:, 200:700].any()
+
+
+def test_no_wait_gave_up():
+    from orthocache_b200 import _lib
+    torch.cuda.synchronize()
+    assert _lib.load().oc_device_status(0) == 0
