@@ -9,8 +9,8 @@
 // row that has no position, or lies in padding, has hi_r = 0), and drafted
 // key s iff tree[b, i, s].  Its score is, in log2 units,
 //     s2 = log2(e) * (cap * tanh(scale * q.k / cap) - slope * |pos_r - j|)
-// (without the tanh when cap is 0), and the output softmax(s) . v; a row that
-// sees nothing is zero.
+// (without the tanh when cap is 0; the float32 kernel leaves log2(e) to the
+// exponential), and the output softmax(s) . v; a row that sees nothing is zero.
 #pragma once
 
 #include "oc_common.cuh"
@@ -18,6 +18,11 @@
 namespace oc {
 
 constexpr float kLog2e = 1.4426950408889634f;
+// tanh(z) = z (1 + u (c0 + u (c1 + u (c2 + u c3)))), u = z^2, |z| <= kTanhMax: a
+// least-squares fit with equalised relative error (1.3e-8).
+__device__ constexpr float kTanh[4] = {-0.3333306908607483f, 0.13324779272079468f, -0.05298607423901558f,
+                                       0.017135007306933403f};
+constexpr float kTanhMax = 0.5f;
 constexpr int kMaxNodes = 256;  // drafted tokens of one tree
 
 struct TokArgs {
@@ -44,7 +49,8 @@ struct TokArgs {
   float *pm, *pl, *po;        // partials: [part][unit_rows][(D)], parts 2 * cta and 2 * cta + 1
   float* logits;                 // (B * Hkv, R, logit_stride) scores in log2 units, -inf where masked; nullable
   int64_t logit_stride;
-  float* lse;                    // (B * Hkv, R) log2 of the softmax denominator, +inf for empty rows; nullable
+  float* lse;                    // (B * Hkv, R) log of the softmax denominator, +inf for empty rows; nullable
+  float unit;                    // 2^(unit * x) = e^x in the units of pm and lse: log2(e) for natural ones, else 1
 };
 
 __device__ __forceinline__ int tok_len(const TokArgs& a, int b) {
@@ -186,12 +192,13 @@ __device__ __forceinline__ int64_t tok_q_offset(const TokArgs& a, int b, int h, 
   return (((int64_t)b * a.Sq + r / a.G) * a.Hq + (int64_t)h * a.G + r % a.G) * D;
 }
 
-// The score in log2 units from the dot product (accurate form).
+// The score from the dot product, in natural units (the float32 kernel keeps
+// them: log2(e) times a score would round once more, and the exponential would
+// magnify that; here it multiplies the difference to the maximum).
 __device__ __forceinline__ float tok_score(const TokArgs& a, float dot, float slope2, int pos, int j) {
   float x = dot * a.scale;
   if (a.cap > 0.f) x = a.cap * tanhf(x / a.cap);
-  x *= kLog2e;
-  return slope2 != 0.f ? fmaf(-slope2, fabsf((float)(pos - j)), x) : x;
+  return slope2 != 0.f ? fmaf(-slope2 * (1.f / kLog2e), fabsf((float)(pos - j)), x) : x;
 }
 
 // The bfloat16 kernel for few rows (oc_token_mma.cu); row_tile 16, 32 or 64.

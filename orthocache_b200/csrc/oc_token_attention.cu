@@ -186,11 +186,11 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
       for (int d = 8; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
       const float m_new = fmaxf(m[i], mx);
       const float base = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = exp2f(m[i] - base);
+      const float alpha = exp2f((m[i] - base) * kLog2e);
       float sum = 0.f;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
-        const float p = exp2f(s[i][n] - base);
+        const float p = exp2f((s[i][n] - base) * kLog2e);
         sm.p[ty + 16 * i][tx + 16 * n] = p;
         sum += p;
       }
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
       continue;
     }
     const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);  // NaN stays NaN
-    if (a.lse && tx == 0) a.lse[(int64_t)bh * a.R + r] = l[i] == 0.f ? INFINITY : m[i] + log2f(l[i]);
+    if (a.lse && tx == 0) a.lse[(int64_t)bh * a.R + r] = l[i] == 0.f ? INFINITY : m[i] + logf(l[i]);
     const int64_t at = tok_q_offset(a, b, h, r, D);
 #pragma unroll
     for (int cc = 0; cc < NC; ++cc)
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs 
         }
       }
       const float m_new = fmaxf(M, fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])));
-      const float ref = m_new == -INFINITY ? 0.f : m_new, old = exp2f(M - ref);
+      const float ref = m_new == -INFINITY ? 0.f : m_new, old = exp2f((M - ref) * a.unit);
       L *= old;
 #pragma unroll
       for (int x = 0; x < D / 32; ++x) o[x] *= old;
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs 
 #pragma unroll
       for (int z = 0; z < 4; ++z) {
         const bool any = mc[z] != -INFINITY;  // else nothing was written but l: 0, or NaN when all its scores were
-        const float w = any ? exp2f(mc[z] - ref) : 1.f;
+        const float w = any ? exp2f((mc[z] - ref) * a.unit) : 1.f;
         L += w * lc[z];
 #pragma unroll
         for (int x = 0; x < D / 32; ++x)
@@ -384,12 +384,12 @@ __global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs 
         for (int w = 1; w < 8; ++w) M = fmaxf(M, s_m[w]);
 #pragma unroll
         for (int w = 0; w < 8; ++w) {
-          const float f = s_m[w] == -INFINITY ? 1.f : exp2f(s_m[w] - M);
+          const float f = s_m[w] == -INFINITY ? 1.f : exp2f((s_m[w] - M) * a.unit);
           L += f * s_l[w];
 #pragma unroll
           for (int y = 0; y < 4; ++y) acc[y] += f * s_o[w][4 * tid + y];
         }
-        if (a.lse && tid == 0) a.lse[(int64_t)(b * a.Hkv + h) * a.R + r] = L == 0.f ? INFINITY : M + log2f(L);
+        if (a.lse && tid == 0) a.lse[(int64_t)(b * a.Hkv + h) * a.R + r] = L == 0.f ? INFINITY : M + (a.unit == 1.f ? log2f(L) : logf(L));
         const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
         const int64_t at = tok_q_offset(a, b, h, r, D) + 4 * tid;
 #pragma unroll
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs 
       }
       continue;
     }
-    if (a.lse && lane == 0) a.lse[(int64_t)(b * a.Hkv + h) * a.R + r] = L == 0.f ? INFINITY : M + log2f(L);
+    if (a.lse && lane == 0) a.lse[(int64_t)(b * a.Hkv + h) * a.R + r] = L == 0.f ? INFINITY : M + (a.unit == 1.f ? log2f(L) : logf(L));
     const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
     const int64_t at = tok_q_offset(a, b, h, r, D);
 #pragma unroll
@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_weights_kernel(const TokArgs
     __syncthreads();
     if (tid < 32) {
       sm.row[tid] = tok_row(a, b, h, r0 + tid, len);
-      sm.lse[tid] = r0 + tid < a.R ? a.lse[(int64_t)bh * a.R + r0 + tid] : INFINITY;
+      sm.lse[tid] = r0 + tid < a.R ? a.lse[(int64_t)bh * a.R + r0 + tid] * (a.unit / kLog2e) : INFINITY;  // natural
     }
     for (int e = tid; e < 32 * (D / kVec); e += kSimtThreads) {
       const int r = e / (D / kVec), x = e % (D / kVec) * kVec;
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_weights_kernel(const TokArgs
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const int j = j0 + tx + 16 * n;
-        if (j < row.hi && lse != INFINITY) acc[n] += exp2f(tok_score(a, s[i][n], row.slope2, row.pos, j) - lse);
+        if (j < row.hi && lse != INFINITY) acc[n] += exp2f((tok_score(a, s[i][n], row.slope2, row.pos, j) - lse) * kLog2e);
       }
     }
   }
@@ -747,6 +747,7 @@ int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void*
   a.lse = lse ? reinterpret_cast<float*>(w + p.lse_off) : nullptr;
   a.logits = p.logit_stride ? reinterpret_cast<float*>(w + p.logit_off) : nullptr;
   a.logit_stride = (int64_t)p.logit_stride;
+  a.unit = dtype == OC_BF16 ? 1.f : kLog2e;
   int rc = p.tc ? tok_tc(fn, a, head_dim, w + p.prep_off, st)
            : dtype == OC_BF16 ? tok_mma(a, head_dim, p.row_tile, st)
                               : dispatch_simt<float>(a, head_dim, p.row_tile, st);

@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
   for (int i = 0; i < C::DW / 8; ++i)
 #pragma unroll
     for (int y = 0; y < 4; ++y) o[i][y] = 0.f;
-  const float c_scale = a.scale * kLog2e, c_cap = a.cap * kLog2e, c_in = a.cap > 0.f ? 2.f * kLog2e * a.scale / a.cap : 0.f;
+  const float c_scale = a.scale * kLog2e, c_cap = a.cap * kLog2e, c_in = a.cap > 0.f ? a.scale / a.cap : 0.f;
   // ldmatrix addresses: lanes 0-15 give rows (lane % 16) of the first 8
   // channels, lanes 16-31 of the next 8
   const int q_row = wr * 16 + (lane & 15), q_c = lane >> 4;
@@ -262,16 +262,31 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
 
     // log2 units: scale, cap, bias, masks
     if (a.cap > 0.f) {
-      // cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap))
+      float top = 0.f;
 #pragma unroll
       for (int n = 0; n < C::NT; ++n)
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          float e, r;
-          asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(s[n][y] * c_in));
-          asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-          s[n][y] = fmaf(-2.f * c_cap, r, c_cap);
+          s[n][y] *= c_in;  // scale / cap
+          top = fmaxf(top, fabsf(s[n][y]));
         }
+      if (__all_sync(0xffffffffu, top <= kTanhMax)) {  // (NaN may pass: it stays NaN)
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const float z = s[n][y], u = z * z;
+            float p = fmaf(kTanh[3], u, kTanh[2]);
+            p = fmaf(p, u, kTanh[1]);
+            p = fmaf(p, u, kTanh[0]);
+            s[n][y] = c_cap * fmaf(z * u, p, z);
+          }
+      } else {
+#pragma unroll
+        for (int n = 0; n < C::NT; ++n)
+#pragma unroll
+          for (int y = 0; y < 4; ++y) s[n][y] = c_cap * tanhf(s[n][y]);
+      }
     } else {
 #pragma unroll
       for (int n = 0; n < C::NT; ++n)

@@ -261,14 +261,15 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // The cap in log2 units: cap' tanh(k s) with cap' = cap log2(e), k = scale / cap.
-// tanh(z) / z by least-squares polynomials in z^2 with equalised error of tanh:
-// degree 2 for |z| <= 0.3 (1.7e-7), degree 3 for |z| <= 0.5 (1.3e-7); beyond, 1 - 2
-// / (1 + e^(2 z)).
-constexpr float kCapPoly2 = 0.3f, kCapPoly3 = 0.5f;
+// tanh(z) / z by least-squares polynomials in z^2: degree 2 for |z| <= 0.3 with
+// equalised error of tanh (1.7e-7, below what the rounding of P leaves), degree 4
+// for |z| <= 0.5 with equalised relative error (1.3e-8: where weights leave in
+// float32, kTanh in oc_token.cuh); beyond, tanhf.
+constexpr float kCapPoly2 = 0.3f;
 struct CapFn {
-  float k, cap2;         // k_in, cap * log2(e)
-  float b0, b1, b2;      // degree 2 in s^2, times cap' k
-  float a0, a1, a2, a3;  // degree 3
+  float k, cap2;             // k_in, cap * log2(e)
+  float b0, b1, b2;          // degree 2 in s^2, times cap' k
+  float a0, a1, a2, a3, a4;  // degree 4
   __device__ __forceinline__ CapFn(const TcArgs& x) {
     k = x.k_in;
     cap2 = x.t.cap * kLog2e;
@@ -276,16 +277,13 @@ struct CapFn {
     b0 = c * 0.9999960064888f;
     b1 = c * k2 * -0.33297479152679443f;
     b2 = c * k2 * k2 * 0.12522591650485992f;
-    a0 = c * 0.9999976754188538f;
-    a1 = c * k2 * -0.33320656418800354f;
-    a2 = c * k2 * k2 * 0.13145145773887634f;
-    a3 = c * k2 * k2 * k2 * -0.04337248206138611f;
+    a0 = c;
+    a1 = c * k2 * kTanh[0];
+    a2 = c * k2 * k2 * kTanh[1];
+    a3 = c * k2 * k2 * k2 * kTanh[2];
+    a4 = c * k2 * k2 * k2 * k2 * kTanh[3];
   }
-  __device__ __forceinline__ float exact(float s) const {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2(2.f * kLog2e * k * s)));
-    return fmaf(-2.f * cap2, r, cap2);
-  }
+  __device__ __forceinline__ float exact(float s) const { return cap2 * tanhf(k * s); }
   template <int DEG>
   __device__ __forceinline__ uint64_t poly2(uint64_t s, uint64_t off) const {  // cap' tanh(k s) + off
     const uint64_t u = mul2(s, s);
@@ -294,7 +292,8 @@ struct CapFn {
       p = fma2(pk2(b2, b2), u, pk2(b1, b1));
       p = fma2(p, u, pk2(b0, b0));
     } else {
-      p = fma2(pk2(a3, a3), u, pk2(a2, a2));
+      p = fma2(pk2(a4, a4), u, pk2(a3, a3));
+      p = fma2(p, u, pk2(a2, a2));
       p = fma2(p, u, pk2(a1, a1));
       p = fma2(p, u, pk2(a0, a0));
     }
@@ -313,7 +312,7 @@ __device__ __forceinline__ bool cap_far(const float* s, float k_in) {
   for (int i = 8; i < N; i += 8)
 #pragma unroll
     for (int k = 0; k < 4; ++k) top[k] = absmax3(top[k], s[i + k], s[i + 4 + k]);
-  return __any_sync(0xffffffffu, !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * k_in <= kCapPoly3));
+  return __any_sync(0xffffffffu, !(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * k_in <= kTanhMax));
 }
 
 // 2^x of a pair on the FMA pipe, x clamped to >= -126: x = n + f, n = floor(x) by
@@ -440,7 +439,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
     int4 qd = make_int4(0, 0, 0, 0);
     if (a.docs) qd = x.query_docs[(size_t)w.b * x.npt + p0 / x.P];
     float m_used = CAP == 1 || !real ? 0.f : -INFINITY, l = 0.f;
-    int level = 0;  // which of the cap's polynomials is in use
+    int level = a.lse ? 1 : 0;  // which of the cap's polynomials is in use
     // what a tile's masking depends on, loaded a tile ahead
     int2 kd = make_int2(0, 0);
     bool no_page = false;
@@ -480,14 +479,14 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
             chunk_exp<D, CAP ? 2 : 0, BIAS>(s + 32 * c, c, pk, r2, top, c_scale, nm2, sl2, b0, cap);
         } else {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) chunk_exp<D, 3, BIAS>(s + 32 * c, c, pk, r2, top, c_scale, nm2, sl2, b0, cap);
+          for (int c = 0; c < 4; ++c) chunk_exp<D, 4, BIAS>(s + 32 * c, c, pk, r2, top, c_scale, nm2, sl2, b0, cap);
         }
         float q[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) up2(r2[i], q[2 * i], q[2 * i + 1]);
         const float sum = ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
         // a score beyond the polynomial, or a sum that has grown too large?
-        const bool far = CAP && __any_sync(0xffffffffu, !(top * x.k_in <= (level ? kCapPoly3 : kCapPoly2)));
+        const bool far = CAP && __any_sync(0xffffffffu, !(top * x.k_in <= (level ? kTanhMax : kCapPoly2)));
         if (far) ++level;  // for the rest of the unit; 2: not this way
         const bool over = far || (CAP != 1 && real && !(sum < kRefMax));
         if (!__any_sync(0xffffffffu, over)) {
@@ -542,7 +541,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
               for (int i = 0; i < 32; ++i) s[i] = cap.exact(s[i]);
             } else {
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) up2(cap.poly2<3>(pk2(s[i], s[i + 1]), 0), s[i], s[i + 1]);
+              for (int i = 0; i < 32; i += 2) up2(cap.poly2<4>(pk2(s[i], s[i + 1]), 0), s[i], s[i + 1]);
             }
           } else {
 #pragma unroll
@@ -1214,7 +1213,7 @@ __device__ void tw_sum(TwSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem, con
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               const uint64_t v = pk2(s[k + 2 * y], s[k + 2 * y + 1]);
-              uint64_t e = CAP ? cap.poly2<3>(v, nz[y]) : fma2(v, sc2, nz[y]);
+              uint64_t e = CAP ? cap.poly2<4>(v, nz[y]) : fma2(v, sc2, nz[y]);
               if (!CAP && (k / 2 + y) % 16 < 5) {
                 e = poly_ex2<5>(e);
               } else {
