@@ -298,7 +298,10 @@ __global__ void __launch_bounds__(kMergeThreads) tok_merge_kernel(const TokArgs 
   const int start = upg * s_tiles[0] + (h / a.hg * a.nrt + rt) * s_tiles[2];
   const TokCut cut(a, upg * s_tiles[1]);
   const int c0 = cut.run(start), parts = cut.run(start + s_tiles[2] - 1) - c0 + 1;
-  if (parts <= 1) return;
+  if (parts <= 1) {
+    pdl_wait();  // what follows on the stream waits for this kernel alone, and through it for the partials' one
+    return;
+  }
   // a unit of one row tile has two partials of 128 rows a piece (both halves of its
   // CTA worked on it)
   const int sub = tc.per_unit == 2 && tc.npt * tc.nhs == 1 ? 2 : 1, nparts = parts * sub;
@@ -531,8 +534,9 @@ __global__ void __launch_bounds__(kSimtThreads) tok_weights_kernel(const TokArgs
 }
 
 // Column sums from stored scores (few rows): a thread per key, rows in order.
-__global__ void __launch_bounds__(256) tok_sum_kernel(const TokArgs a, const float* w_in, float* w_out) {
-  const int bh = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
+__global__ void __launch_bounds__(256) tok_sum_kernel(const TokArgs a, int blocks, const float* w_in,
+                                                      float* w_out) {
+  const int bh = blockIdx.x / blocks, j = blockIdx.x % blocks * 256 + threadIdx.x;
   if (j >= a.S) return;
   const int64_t at = (int64_t)bh * a.S + j;
   const int len = tok_len(a, bh / a.Hkv);
@@ -756,9 +760,9 @@ int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void*
   if (rc || !w_out || a.S == 0) return rc;
   // the column sums
   if (a.logits) {
-    const dim3 grid((unsigned)((a.S + 255) / 256), (unsigned)(a.B * a.Hkv));
-    OC_REQUIRE(grid.y <= 65535, OC_ERR_SHAPE, "%s: too many heads", fn);
-    cudaError_t e = launch_pdl(tok_sum_kernel, grid, dim3(256), 0, st, a, w_in, w_out);
+    const int blocks = (a.S + 255) / 256;  // per (b, h); fewer than 2^31 / 256 for all b
+    cudaError_t e = launch_pdl(tok_sum_kernel, dim3((unsigned)blocks * a.B * a.Hkv), dim3(256), 0, st, a, blocks, w_in,
+                               w_out);
     if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_sum_kernel: %s", cudaGetErrorString(e));
     return OC_OK;
   }

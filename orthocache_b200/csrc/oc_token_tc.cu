@@ -992,9 +992,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (x.t.even && warp == 0) tok_prefix(x.t, sm.pre);
-  pdl_wait();
+  pdl_wait();     // everything below, the lengths too, may come from the kernel before this one
   pdl_trigger();  // the merge may find its parts meanwhile
+  if (x.t.even && warp == 0) tok_prefix(x.t, sm.pre);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
