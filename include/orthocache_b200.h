@@ -457,9 +457,10 @@ int oc_score_from_metadata_paged(const float* dc_pool, const float* e_ac_pool, c
  * hq reads KV head hq / G, G = Hq / Hkv); seq_len = S is the capacity of a
  * batch row and lengths (B, nullable = S; clamped to [0, S]) the tokens it
  * holds: what lies behind them is never used, whatever its value.  Scores
- * are scale * q.k in float32; cap > 0 turns them into cap * tanh(s / cap).
- * A query row that sees no key gives zeros.  A key or value that some rows of
- * a call see and others do not must be finite for the others.  out
+ * are scale * q.k in float32; cap > 0 turns them into cap * tanh(s / cap)
+ * (then |scale| <= 4096 * cap and |scale| <= 2^24).  A query row that sees no
+ * key gives zeros.  Values inside a sequence must be finite, whether a row sees
+ * them or not (a hidden one has weight zero, and zero times infinity is NaN).  out
  * (B, Sq, Hq, D) in out_dtype.  k and v may be NULL when seq_len is 0.
  * Workspace: oc_token_attention_workspace_bytes (q_len: Sq or the drafted
  * tokens; accumulate: nonzero for oc_accumulate_attention), 16-byte aligned;
@@ -504,7 +505,7 @@ int oc_chunk_attention(const void* q, const void* k, const void* v, int dtype, c
  *   weights_out[b, h, j] = weights_in[b, h, j] + sum over i, g of
  *   softmax(s)[b, i, h * G + g, j];
  * weights (B, Hkv, S) float32; weights_in NULL counts as zero and may equal
- * weights_out.  Entries behind lengths[b] are copied.  The sums are taken in
+ * weights_out (but not overlap it in part).  Entries behind lengths[b] are copied.  The sums are taken in
  * a fixed order: the same call gives the same bits. */
 int oc_accumulate_attention(const void* q, const void* k, const void* v, int dtype, const int32_t* lengths,
                             const float* weights_in, float* weights_out, int batch, int q_len, int q_heads,

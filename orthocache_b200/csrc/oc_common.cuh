@@ -149,6 +149,21 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// Lets `kern` use `bytes` of dynamic shared memory on the current device; `done`
+// remembers the devices on which it may.  A device is marked only when the
+// driver has answered, so a second thread never launches too early.
+template <typename... KArgs>
+cudaError_t allow_smem(std::atomic<uint64_t>& done, void (*kern)(KArgs...), size_t bytes) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_acq_rel);
+  return e;
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Programmatic dependent launch.  A kernel launched with launch_pdl may

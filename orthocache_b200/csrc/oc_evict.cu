@@ -14,8 +14,8 @@
 // memory of a cluster of CTAs, and the threshold found by three histograms of 11,
 // 11 and 10 bits of the order-preserving key, added up over the cluster through
 // distributed shared memory, an eighth of the bins by each CTA (every CTA reading
-// all histograms took 8,000 cycles a pass, this 2,500).  The gather is bound by memory: every kept row read
-// and written once.
+// all histograms took 8,000 cycles a pass, this 2,500).  The gather is bound by
+// memory: every kept row read and written once.
 #include <cooperative_groups.h>
 
 #include "oc_common.cuh"
@@ -215,11 +215,8 @@ cudaError_t launch_select(int heads, size_t smem, cudaStream_t st, const float* 
                           int H, int keep, int recent, int32_t* index, float* weights_out, int32_t* new_lengths) {
   auto kern = evict_select_kernel<CS, CACHED>;
   static std::atomic<uint64_t> done{0};
-  if (first_on_device(done)) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)(sizeof(SelSmem) + (CACHED ? kSelCached * 4 : 0)));
-    if (e != cudaSuccess) return e;
-  }
+  const cudaError_t e = allow_smem(done, kern, sizeof(SelSmem) + (CACHED ? kSelCached * 4 : 0));
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(heads * CS));
   cfg.blockDim = dim3(kSelThreads);
@@ -280,7 +277,7 @@ extern "C" int oc_evict_tokens(const void* k, const void* v, int dtype, const fl
   OC_REQUIRE(recent >= 0 && recent <= keep, OC_ERR_SHAPE, "oc_evict_tokens: recent %d, keep %d", recent, keep);
   OC_REQUIRE(aligned16(k) && aligned16(v) && aligned16(k_out) && aligned16(v_out), OC_ERR_ALIGN,
              "oc_evict_tokens: keys / values must be 16-byte aligned");
-  OC_REQUIRE(k_out != k && v_out != v && k_out != v_out && k_out != v && v_out != k, OC_ERR_SHAPE,
+  OC_REQUIRE(k_out != k && v_out != v && k_out != v_out && k_out != v && v_out != k && weights_out != weights, OC_ERR_SHAPE,
              "oc_evict_tokens: the kept tokens need buffers of their own");
   OC_REQUIRE((int64_t)batch * kv_heads < 65536 * 16, OC_ERR_SHAPE, "oc_evict_tokens: too many heads");
   const int vecs = head_dim * es / 16;
@@ -302,8 +299,8 @@ extern "C" int oc_evict_tokens(const void* k, const void* v, int dtype, const fl
                                 weights_out, new_lengths);
   if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "evict_select_kernel: %s", cudaGetErrorString(e));
   e = launch_pdl(evict_gather_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st,
-                             static_cast<const uint4*>(k), static_cast<const uint4*>(v), index, seq_len, kv_heads,
-                             keep, vecs, total, static_cast<uint4*>(k_out), static_cast<uint4*>(v_out));
+                 static_cast<const uint4*>(k), static_cast<const uint4*>(v), index, seq_len, kv_heads, keep, vecs,
+                 total, static_cast<uint4*>(k_out), static_cast<uint4*>(v_out));
   if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "evict_gather_kernel: %s", cudaGetErrorString(e));
   return OC_OK;
 }

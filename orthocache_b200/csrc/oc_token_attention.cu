@@ -652,11 +652,8 @@ template <typename T, int D, int RPT>
 int launch_simt(const TokArgs& a, cudaStream_t st) {
   const size_t smem = sizeof(SimtSmem<D, RPT>);
   static std::atomic<uint64_t> done{0};
-  if (first_on_device(done)) {
-    cudaError_t e = cudaFuncSetAttribute(tok_simt_kernel<T, D, RPT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem);
-    if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_simt_kernel: %s", cudaGetErrorString(e));
-  }
+  const cudaError_t e = allow_smem(done, tok_simt_kernel<T, D, RPT>, smem);
+  if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_simt_kernel: %s", cudaGetErrorString(e));
   tok_simt_kernel<T, D, RPT><<<a.even ? a.ncta : a.B * a.Hkv * a.nrt, kSimtThreads, smem, st>>>(a);
   return check_launch("tok_simt_kernel");
 }
@@ -672,14 +669,10 @@ template <typename T, int D>
 int launch_weights(const TokArgs& a, const float* w_in, float* w_out, cudaStream_t st) {
   const size_t smem = sizeof(WeightSmem<T, D>);
   static std::atomic<uint64_t> done{0};
-  if (first_on_device(done)) {
-    cudaError_t e = cudaFuncSetAttribute(tok_weights_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem);
-    if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_weights_kernel: %s", cudaGetErrorString(e));
-  }
+  cudaError_t e = allow_smem(done, tok_weights_kernel<T, D>, smem);
+  if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_weights_kernel: %s", cudaGetErrorString(e));
   const int64_t blocks = (int64_t)((a.S + kSimtTok - 1) / kSimtTok) * a.B * a.Hkv;
-  cudaError_t e = launch_pdl(tok_weights_kernel<T, D>, dim3((unsigned)blocks), dim3(kSimtThreads), smem, st, a, w_in,
-                             w_out);
+  e = launch_pdl(tok_weights_kernel<T, D>, dim3((unsigned)blocks), dim3(kSimtThreads), smem, st, a, w_in, w_out);
   if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_weights_kernel: %s", cudaGetErrorString(e));
   return OC_OK;
 }
@@ -690,6 +683,8 @@ int dispatch_weights(const TokArgs& a, int D, const float* w_in, float* w_out, c
   if (D == 128) return launch_weights<T, 128>(a, w_in, w_out, st);
   return launch_weights<T, 256>(a, w_in, w_out, st);
 }
+
+constexpr float kMaxScaleOfCap = 4096.f;
 
 // Checks shared by the three entry points; fills the sizes of `a`.
 int tok_common(const char* fn, TokArgs& a, const void* q, const void* k, const void* v, int dtype, int batch,
@@ -709,6 +704,11 @@ int tok_common(const char* fn, TokArgs& a, const void* q, const void* k, const v
              OC_ERR_SHAPE, "%s: too many rows", fn);
   OC_REQUIRE(isfinite(cap) && cap >= 0.f, OC_ERR_SHAPE, "%s: cap must be finite and >= 0 (0: none)", fn);
   OC_REQUIRE(isfinite(scale), OC_ERR_SHAPE, "%s: scale must be finite", fn);
+  // the cap's polynomials have coefficients up to scale (scale / cap)^8
+  OC_REQUIRE(cap == 0.f || fabsf(scale) <= kMaxScaleOfCap * cap, OC_ERR_SHAPE,
+             "%s: cap %g is below a %gth of the scale %g", fn, cap, kMaxScaleOfCap, scale);
+  OC_REQUIRE(cap == 0.f || fabsf(scale) <= kMaxScaleOfCap * kMaxScaleOfCap, OC_ERR_SHAPE, "%s: scale %g with a cap", fn,
+             scale);
   OC_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), OC_ERR_ALIGN,
              "%s: q/k/v/out must be 16-byte aligned", fn);
   a = TokArgs{};
@@ -853,6 +853,10 @@ extern "C" int oc_accumulate_attention(const void* q, const void* k, const void*
                       cap, scale, out, out_dtype);
   if (rc) return rc;
   OC_REQUIRE(weights_out || seq_len == 0, OC_ERR_NULL, "oc_accumulate_attention: NULL pointer");
+  const uintptr_t wi = reinterpret_cast<uintptr_t>(weights_in), wo = reinterpret_cast<uintptr_t>(weights_out);
+  const uintptr_t wn = (uintptr_t)batch * kv_heads * seq_len * sizeof(float);
+  OC_REQUIRE(!weights_in || wi == wo || wi + wn <= wo || wo + wn <= wi, OC_ERR_SHAPE,
+             "oc_accumulate_attention: weights_in overlaps weights_out in part");
   a.lengths = lengths;
   a.causal = 1;
   return tok_run("oc_accumulate_attention", a, dtype, head_dim, true, workspace, workspace_bytes,

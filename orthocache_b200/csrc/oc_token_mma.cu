@@ -444,10 +444,8 @@ template <int D, int WR>
 int launch_mma(const TokArgs& a, cudaStream_t st) {
   using C = MmaShape<D, WR>;
   static std::atomic<uint64_t> done{0};
-  if (first_on_device(done)) {
-    cudaError_t e = cudaFuncSetAttribute(tok_mma_kernel<D, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-    if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_mma_kernel: %s", cudaGetErrorString(e));
-  }
+  const cudaError_t e = allow_smem(done, tok_mma_kernel<D, WR>, C::kSmem);
+  if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_mma_kernel: %s", cudaGetErrorString(e));
   tok_mma_kernel<D, WR><<<a.even ? a.ncta : a.B * a.Hkv * a.nrt, C::THREADS, C::kSmem, st>>>(a);
   return check_launch("tok_mma_kernel");
 }

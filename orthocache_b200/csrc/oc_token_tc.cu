@@ -1404,13 +1404,10 @@ int launch_tc(const CUtensorMap (&m)[5], const TcArgs& x, cudaStream_t st) {
   const size_t smem = sizeof(TcSmem<D>) + 1024;
   auto kern = tok_tc_kernel<D, CAP, BIAS>;
   static std::atomic<uint64_t> done{0};
-  if (first_on_device(done)) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_tc_kernel: %s", cudaGetErrorString(e));
-  }
+  cudaError_t e = allow_smem(done, kern, smem);
+  if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_tc_kernel: %s", cudaGetErrorString(e));
   const int sms = device_sm_count();
   const dim3 grid((unsigned)(x.t.even ? x.t.ncta : x.units < sms ? x.units : sms));
-  cudaError_t e;
   if (x.tree_bits || x.query_docs) {
     e = launch_pdl(kern, grid, dim3(kThreads), smem, st, m[0], m[1], m[2], m[3], m[4], x);
   } else {
@@ -1508,10 +1505,8 @@ int launch_tw(const CUtensorMap& mq, const CUtensorMap& mk, const TcArgs& x, con
   const size_t smem = sizeof(TwSmem<D>) + 1024;
   auto kern = tok_tc_weights_kernel<D, CAP>;
   static std::atomic<uint64_t> done{0};
-  if (first_on_device(done)) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_tc_weights_kernel: %s", cudaGetErrorString(e));
-  }
+  cudaError_t e = allow_smem(done, kern, smem);
+  if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_tc_weights_kernel: %s", cudaGetErrorString(e));
   const int sms = device_sm_count();
   kern<<<(unsigned)(x.units < sms ? x.units : sms), kThreads, smem, st>>>(mq, mk, x, w_in, w_out);
   return check_launch("tok_tc_weights_kernel");

@@ -18,6 +18,10 @@ Shapes: q (B, Sq, Hq, D), keys and values (B, S, Hkv, D), float32 or bfloat16,
 D in {64, 128, 256}, Hq a multiple of Hkv; without the batch dimension all
 per-row arguments lose theirs too.  q is brought to the keys' type and the output
 has it.  Inputs on the CPU are copied to the GPU.  Nothing waits for the GPU.
+Values inside a sequence are finite, seen by a row or not (a hidden one has
+weight zero, and zero times infinity is NaN); what lies behind lengths[b], in
+padding or in drafted tokens that no node sees may be anything.  With a cap, it is
+at least scale / 4096.
 """
 from __future__ import annotations
 
@@ -62,6 +66,8 @@ def _int_rows(x, shape, device, what):
         raise TypeError(f"{what} must be integers, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{what} {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype in (torch.int64, torch.uint32, torch.uint64):  # beyond the range: its nearest end, not another number
+        t = t.to(torch.int64).clamp(-2 ** 31, 2 ** 31 - 1)
     return t.to(torch.int32).contiguous()
 
 
@@ -72,6 +78,8 @@ def _cap_scale(cap, scale, dim):
         raise ValueError(f"cap must be finite and >= 0 (0: none), got {cap}")
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite, got {scale}")
+    if cap and abs(scale) > 4096.0 * min(cap, 4096.0):
+        raise ValueError(f"with a cap the scale may be 4096 times the cap, and 2^24, at most, got {scale}, {cap}")
     return cap, scale
 
 
@@ -192,8 +200,8 @@ def chunk_attention(q, keys, values, lengths=None, *, causal=True, prefix=None, 
 
     * the causal mask: not ``causal``, or j <= pos, or j < prefix[b]
       (``prefix`` (B,): tokens that every query may see);
-    * the document mask: ``documents`` (B, S) int, equal at pos and j and not
-      negative (negative: padding, seen by nobody).
+    * the document mask: ``documents`` (B, S) int in the range of int32, equal at
+      pos and j and not negative (negative: padding, seen by nobody).
 
     Scores: scale * q.k (1 / sqrt(D) by default), then cap * tanh(score / cap)
     if ``cap`` > 0, then minus slopes[head] * |pos - j| (``slopes`` (Hq,)
@@ -230,7 +238,7 @@ def accumulate_attention(q, keys, values, weights=None, lengths=None, *, cap=0.0
     queries and the Hq / Hkv heads.  ``weights``: (B, Hkv, S) float32, None for
     zeros; entries behind lengths[b] are copied.  ``out_weights``: a contiguous
     float32 CUDA tensor that receives the sums (``weights`` itself to add in
-    place); a new one by default.
+    place, but no other that shares memory with it); a new one by default.
     """
     qq, k, v, batched, lens = _chunk_inputs(q, keys, values, lengths)
     B, Sq, Hq, D = qq.shape

@@ -112,3 +112,30 @@ def test_evict_refusals(kw, rc, needle):
                               a["d"], a["keep"], a["recent"], a["ko"], ctypes.c_void_p(1 << 21), P, P, P, None)
     assert got == rc
     assert needle in lib.oc_last_error()
+
+
+@pytest.mark.parametrize("call", [_tree, _chunk, _acc])
+@pytest.mark.parametrize("cap,scale", [(1e-30, 0.1), (2e-5, 0.1), (2e-5, -0.1), (1e5, 2e7)])
+def test_cap_far_below_the_scale(call, cap, scale):
+    """The polynomials of the cap have coefficients up to scale (scale / cap)^8."""
+    lib = _lib()
+    assert call(lib, cap=cap, scale=scale) == -2
+    assert b"scale" in lib.oc_last_error()
+
+
+@pytest.mark.parametrize("shift", [4, 64, 16 * 1024 - 4, -4])
+def test_sums_that_overlap_in_part(shift):
+    lib = _lib()  # 1 x 4 heads x 1024 keys x 4 bytes
+    w = 1 << 20
+    got = lib.oc_accumulate_attention(P, P, P, 1, None, ctypes.c_void_p(w + shift), ctypes.c_void_p(w), 1, 4, 8, 4, 128,
+                                      1024, 0.0, 0.1, P, 1, P, BIG, None)
+    assert got == -2
+    assert b"overlap" in lib.oc_last_error()
+
+
+def test_evicted_weights_need_a_buffer_of_their_own():
+    lib = _lib()
+    p = [ctypes.c_void_p(1 << n) for n in range(20, 28)]
+    got = lib.oc_evict_tokens(p[0], p[1], 1, p[2], None, 1, 100, 2, 64, 50, 10, p[3], p[4], p[2], p[5], p[6], None)
+    assert got == -2
+    assert b"own" in lib.oc_last_error()
