@@ -13,6 +13,7 @@
 #include <math.h>
 
 #include "oc_mma.cuh"
+#include "oc_tma.cuh"
 #include "oc_token.cuh"
 
 namespace oc {
@@ -21,24 +22,29 @@ namespace {
 constexpr int kSimtThreads = 256;
 constexpr int kSimtTok = 64;  // keys per tile
 
+// Rows are padded by four floats, so that the 16 keys a half-warp reads at once,
+// and the rows of its two halves, fall into different banks.
 template <int D, int RPT>
 struct SimtSmem {
-  float q[16 * RPT][D];
-  float k[kSimtTok][D + 4];  // +4: the 16 keys a half-warp reads at once fall into different banks
-  float v[kSimtTok][D];
-  float p[16 * RPT][kSimtTok];
+  static constexpr int kStages = D == 64 || (D == 128 && RPT == 4) ? 2 : 1;  // two where that costs no CTA of the SM
+  float q[16 * RPT][D + 4];
+  float k[kStages][kSimtTok][D + 4];
+  float v[kStages][kSimtTok][D];
+  float p[16 * RPT][kSimtTok + 4];
   TokRow row[16 * RPT];
-  int doc[kSimtTok];
-  int seen[kSimtTok];
+  int doc[kStages + 1][kSimtTok];
+  int64_t src[kStages + 1][kSimtTok];  // row of the key in its tensor, -1 for one that nobody sees
   int hi;
   int pre[kMaxEvenBatch + 1];
 };
 
-// Load keys [j0, j0 + 64) of the cache (or of the drafted tokens) as float32.
-// Keys that no row may see (behind the sequence, padding, pages outside the
-// pool) become zero, so that whatever the memory holds there cannot reach a
-// result.
-template <typename T, int D>
+// Four floats to shared memory, or zeros.
+__device__ __forceinline__ void simt_cp16(float* dst, const float* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(real ? 16 : 0)
+               : "memory");
+}
+
+template <typename T>
 __device__ __forceinline__ void simt_load_vec(const T* src, float* dst) {
   constexpr int kVec = Elem<T>::kVec;
   const uint4 w = *reinterpret_cast<const uint4*>(src);
@@ -52,16 +58,18 @@ __device__ __forceinline__ void simt_load_vec(const T* src, float* dst) {
 // the running maximum and sum of the softmax; 256 threads as 16 x 16: thread
 // (ty, tx) owns rows ty + 16 i, the scores of keys tx + 16 n, and the output
 // channels 4 tx + 64 c of its rows, so that the softmax statistics stay in
-// registers (reduced over the 16 lanes of a half-warp).  Bound by the
-// shared-memory reads of the score product, about 1.2 per four FMA.
-template <typename T, int D, int RPT>
+// registers (reduced over the 16 lanes of a half-warp).  The next tile of keys and
+// values is on its way (cp.async) while one is multiplied; keys that no row may
+// see (behind the sequence, padding, pages outside the pool) are filled with
+// zeros, so that whatever the memory holds there cannot reach a result.
+template <int D, int RPT>
 __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a) {
   extern __shared__ __align__(16) unsigned char raw[];
-  SimtSmem<D, RPT>& sm = *reinterpret_cast<SimtSmem<D, RPT>*>(raw);
-  constexpr int RT = 16 * RPT, kVec = Elem<T>::kVec, NC = D / 64;
+  using Smem = SimtSmem<D, RPT>;
+  Smem& sm = *reinterpret_cast<Smem*>(raw);
+  constexpr int RT = 16 * RPT, NC = D / 64, ST = Smem::kStages, kRow = D / 4;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const T* kbase = static_cast<const T*>(a.k);
-  const T* vbase = static_cast<const T*>(a.v);
+  const float* qbase = static_cast<const float*>(a.q);
   pdl_trigger();  // the merge may find its parts meanwhile
   if (a.even) {
     if (tid < 32) tok_prefix(a, sm.pre);
@@ -80,20 +88,18 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
   }
   const int b = seg.b, h = seg.unit / a.nrt, rt = seg.unit % a.nrt, bh = b * a.Hkv + h;
   const int len = tok_len(a, b);
+  asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();  // the previous piece is done with shared memory
   if (tid == 0) sm.hi = 0;
+  for (int e = tid; e < RT * kRow; e += kSimtThreads) {
+    const int r = e / kRow, x = e % kRow * 4;
+    const bool real = rt * RT + r < a.R;
+    simt_cp16(&sm.q[r][x], qbase + (real ? tok_q_offset(a, b, h, rt * RT + r, D) + x : 0), real);
+  }
   __syncthreads();
   for (int r = tid; r < RT; r += kSimtThreads) {
     sm.row[r] = tok_row(a, b, h, rt * RT + r, len);
     if (sm.row[r].hi > 0) atomicMax(&sm.hi, sm.row[r].hi);
-  }
-  for (int e = tid; e < RT * (D / kVec); e += kSimtThreads) {
-    const int r = e / (D / kVec), x = e % (D / kVec) * kVec;
-    if (rt * RT + r < a.R)
-      simt_load_vec<T, D>(static_cast<const T*>(a.q) + tok_q_offset(a, b, h, rt * RT + r, D) + x, &sm.q[r][x]);
-    else
-#pragma unroll
-      for (int y = 0; y < kVec; ++y) sm.q[r][x + y] = 0.f;
   }
   __syncthreads();
   const int nct = (len + kSimtTok - 1) / kSimtTok;  // tiles of the cache; drafted tokens follow
@@ -101,6 +107,41 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
   const int ncache = (t1 - t0 + kSimtTok - 1) / kSimtTok;
   const int d0 = max(seg.t0 - nct, 0);
   const int ndraft = a.dk && seg.t1 > nct ? min(seg.t1 - nct, (a.Sq + kSimtTok - 1) / kSimtTok) - d0 : 0;
+  const int ntile = ncache + ndraft;
+
+  const auto first_key = [&](int tile) {
+    return tile >= ncache ? (d0 + tile - ncache) * kSimtTok : t0 + tile * kSimtTok;
+  };
+  // where the tile's keys lie, and their documents
+  const auto mark = [&](int tile) {
+    if (tile >= ntile || tid >= kSimtTok) return;
+    const int j = first_key(tile) + tid;
+    int64_t src = -1;
+    int doc = -1;
+    if (tile >= ncache) {
+      for (int i = 0; j < a.Sq && i < a.Sq && src < 0; ++i)
+        if (a.tree[b * a.tree_bstride + (int64_t)i * a.Sq + j]) src = (int64_t)b * a.Sq + j;
+    } else if (j < len) {
+      doc = a.docs ? a.docs[(size_t)b * a.S + j] : 0;
+      if (doc >= 0) src = tok_kv_row(a, b, j);
+    }
+    sm.doc[tile % (ST + 1)][tid] = doc;
+    sm.src[tile % (ST + 1)][tid] = src;
+  };
+  const auto issue = [&](int tile) {
+    if (tile < ntile) {
+      const float* kp = static_cast<const float*>(tile >= ncache ? a.dk : a.k);
+      const float* vp = static_cast<const float*>(tile >= ncache ? a.dv : a.v);
+#pragma unroll 4
+      for (int e = tid; e < kSimtTok * kRow; e += kSimtThreads) {
+        const int t = e / kRow, x = e % kRow * 4;
+        const int64_t src = sm.src[tile % (ST + 1)][t], at = (src * a.Hkv + h) * D + x;
+        simt_cp16(&sm.k[tile % ST][t][x], src >= 0 ? kp + at : qbase, src >= 0);
+        simt_cp16(&sm.v[tile % ST][t][x], src >= 0 ? vp + at : qbase, src >= 0);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
 
   TokRow row[RPT];
   float m[RPT], l[RPT], o[RPT][NC * 4];
@@ -113,36 +154,18 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
     for (int x = 0; x < NC * 4; ++x) o[i][x] = 0.f;
   }
 
-  for (int tile = 0; tile < ncache + ndraft; ++tile) {
+  for (int t = 0; t < ST; ++t) mark(t);
+  __syncthreads();
+  if (ST == 2) issue(0);
+  for (int tile = 0; tile < ntile; ++tile) {
     const bool draft = tile >= ncache;
-    const int j0 = draft ? (d0 + tile - ncache) * kSimtTok : t0 + tile * kSimtTok;
-    __syncthreads();  // the previous tile's keys and values are read
-    if (tid < kSimtTok) {
-      const int j = j0 + tid;
-      int seen = 0, doc = -1;
-      if (draft) {
-        if (j < a.Sq)
-          for (int i = 0; i < a.Sq && !seen; ++i) seen = a.tree[b * a.tree_bstride + (int64_t)i * a.Sq + j] != 0;
-      } else if (j < len) {
-        doc = a.docs ? a.docs[(size_t)b * a.S + j] : 0;
-        seen = doc >= 0 && tok_kv_row(a, b, j) >= 0;
-      }
-      sm.doc[tid] = doc;
-      sm.seen[tid] = seen;
-    }
-    __syncthreads();
-    for (int e = tid; e < kSimtTok * (D / kVec); e += kSimtThreads) {
-      const int t = e / (D / kVec), x = e % (D / kVec) * kVec, j = j0 + t;
-      if (sm.seen[t]) {
-        const int64_t at = draft ? (((int64_t)b * a.Sq + j) * a.Hkv + h) * D + x
-                                 : (tok_kv_row(a, b, j) * a.Hkv + h) * D + x;
-        simt_load_vec<T, D>((draft ? static_cast<const T*>(a.dk) : kbase) + at, &sm.k[t][x]);
-        simt_load_vec<T, D>((draft ? static_cast<const T*>(a.dv) : vbase) + at, &sm.v[t][x]);
-      } else {
-#pragma unroll
-        for (int y = 0; y < kVec; ++y) sm.k[t][x + y] = sm.v[t][x + y] = 0.f;
-      }
-    }
+    const int j0 = first_key(tile), at = tile % ST;
+    const int *doc = sm.doc[tile % (ST + 1)];
+    const int64_t* src = sm.src[tile % (ST + 1)];
+    __syncthreads();  // the tile before is read, the next one marked
+    issue(tile + ST - 1);
+    mark(tile + ST);
+    asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
     __syncthreads();
 
     float s[RPT][4];
@@ -154,7 +177,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
     for (int x = 0; x < D; x += 4) {
       float4 kk[4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) kk[n] = *reinterpret_cast<const float4*>(&sm.k[tx + 16 * n][x]);
+      for (int n = 0; n < 4; ++n) kk[n] = *reinterpret_cast<const float4*>(&sm.k[at][tx + 16 * n][x]);
 #pragma unroll
       for (int i = 0; i < RPT; ++i) {
         const float4 qq = *reinterpret_cast<const float4*>(&sm.q[ty + 16 * i][x]);
@@ -174,11 +197,11 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         const int t = tx + 16 * n, j = j0 + t;
-        bool vis = sm.seen[t] != 0;
+        bool vis = src[t] >= 0;
         if (draft)
           vis = vis && r < a.R && a.tree[b * a.tree_bstride + (int64_t)(r / a.G) * a.Sq + j] != 0;
         else
-          vis = vis && j < row[i].hi && j < t1 && (!a.docs || sm.doc[t] == row[i].doc);
+          vis = vis && j < row[i].hi && j < t1 && (!a.docs || doc[t] == row[i].doc);
         s[i][n] = vis ? tok_score(a, s[i][n], row[i].slope2, row[i].pos, j) : -INFINITY;
         mx = fmaxf(mx, s[i][n]);
       }
@@ -211,7 +234,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
       for (int u = 0; u < 4; ++u) {
 #pragma unroll
         for (int cc = 0; cc < NC; ++cc) {
-          const float4 vv = *reinterpret_cast<const float4*>(&sm.v[t + u][4 * tx + 64 * cc]);
+          const float4 vv = *reinterpret_cast<const float4*>(&sm.v[at][t + u][4 * tx + 64 * cc]);
 #pragma unroll
           for (int i = 0; i < RPT; ++i) {
             const float pp = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
@@ -466,7 +489,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_weights_kernel(const TokArgs
   for (int e = tid; e < kSimtTok * (D / kVec); e += kSimtThreads) {
     const int t = e / (D / kVec), x = e % (D / kVec) * kVec;
     if (j0 + t < len)
-      simt_load_vec<T, D>(static_cast<const T*>(a.k) + (((int64_t)b * a.S + j0 + t) * a.Hkv + h) * D + x, &sm.k[t][x]);
+      simt_load_vec<T>(static_cast<const T*>(a.k) + (((int64_t)b * a.S + j0 + t) * a.Hkv + h) * D + x, &sm.k[t][x]);
     else
 #pragma unroll
       for (int y = 0; y < kVec; ++y) sm.k[t][x + y] = 0.f;
@@ -486,7 +509,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_weights_kernel(const TokArgs
     for (int e = tid; e < 32 * (D / kVec); e += kSimtThreads) {
       const int r = e / (D / kVec), x = e % (D / kVec) * kVec;
       if (r0 + r < a.R)
-        simt_load_vec<T, D>(static_cast<const T*>(a.q) + tok_q_offset(a, b, h, r0 + r, D) + x, &sm.q[r][x]);
+        simt_load_vec<T>(static_cast<const T*>(a.q) + tok_q_offset(a, b, h, r0 + r, D) + x, &sm.q[r][x]);
       else
 #pragma unroll
         for (int y = 0; y < kVec; ++y) sm.q[r][x + y] = 0.f;
@@ -613,7 +636,8 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
     p.nrt = (int)((R + p.row_tile - 1) / p.row_tile);
     p.unit_rows = p.row_tile;
     p.tile = dtype == OC_BF16 ? tok_mma_tile(head_dim) : kSimtTok;
-    slots *= 2;
+    // CTAs of an SM: the float32 kernel's shared memory leaves room for one from 128 channels on
+    slots *= dtype == OC_BF16 || head_dim == 64 || (head_dim == 128 && p.row_tile == 16) ? 2 : 1;
   }
   p.units = (int64_t)batch * kv_heads * p.nrt;
   const int64_t tiles = p.units * ((seq_len + p.tile - 1) / p.tile + (draft_len + p.tile - 1) / p.tile);
@@ -648,21 +672,20 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
   return p;
 }
 
-template <typename T, int D, int RPT>
+template <int D, int RPT>
 int launch_simt(const TokArgs& a, cudaStream_t st) {
   const size_t smem = sizeof(SimtSmem<D, RPT>);
   static std::atomic<uint64_t> done{0};
-  const cudaError_t e = allow_smem(done, tok_simt_kernel<T, D, RPT>, smem);
+  const cudaError_t e = allow_smem(done, tok_simt_kernel<D, RPT>, smem);
   if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_simt_kernel: %s", cudaGetErrorString(e));
-  tok_simt_kernel<T, D, RPT><<<a.even ? a.ncta : a.B * a.Hkv * a.nrt, kSimtThreads, smem, st>>>(a);
+  tok_simt_kernel<D, RPT><<<a.even ? a.ncta : a.B * a.Hkv * a.nrt, kSimtThreads, smem, st>>>(a);
   return check_launch("tok_simt_kernel");
 }
 
-template <typename T>
 int dispatch_simt(const TokArgs& a, int D, int row_tile, cudaStream_t st) {
-  if (D == 64) return row_tile == 16 ? launch_simt<T, 64, 1>(a, st) : launch_simt<T, 64, 4>(a, st);
-  if (D == 128) return row_tile == 16 ? launch_simt<T, 128, 1>(a, st) : launch_simt<T, 128, 4>(a, st);
-  return row_tile == 16 ? launch_simt<T, 256, 1>(a, st) : launch_simt<T, 256, 4>(a, st);
+  if (D == 64) return row_tile == 16 ? launch_simt<64, 1>(a, st) : launch_simt<64, 4>(a, st);
+  if (D == 128) return row_tile == 16 ? launch_simt<128, 1>(a, st) : launch_simt<128, 4>(a, st);
+  return row_tile == 16 ? launch_simt<256, 1>(a, st) : launch_simt<256, 4>(a, st);
 }
 
 template <typename T, int D>
@@ -754,7 +777,7 @@ int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void*
   a.unit = dtype == OC_BF16 ? 1.f : kLog2e;
   int rc = p.tc ? tok_tc(fn, a, head_dim, w + p.prep_off, st)
            : dtype == OC_BF16 ? tok_mma(a, head_dim, p.row_tile, st)
-                              : dispatch_simt<float>(a, head_dim, p.row_tile, st);
+                              : dispatch_simt(a, head_dim, p.row_tile, st);
   if (rc) return rc;
   if (p.even) rc = tok_merge(a, head_dim, p.tc, st);
   if (rc || !w_out || a.S == 0) return rc;
