@@ -22,19 +22,20 @@ namespace {
 constexpr int kSimtThreads = 256;
 constexpr int kSimtTok = 64;  // keys per tile
 
-// Rows are padded by four floats, so that the 16 keys a half-warp reads at once,
-// and the rows of its two halves, fall into different banks.
+// Rows are padded, so that the 16 keys a half-warp reads at once, and the rows of
+// its two halves, fall into different banks.
 template <int D, int RPT>
 struct SimtSmem {
   static constexpr int kStages = D == 64 || (D == 128 && RPT == 4) ? 2 : 1;  // two where that costs no CTA of the SM
   float q[16 * RPT][D + 4];
   float k[kStages][kSimtTok][D + 4];
   float v[kStages][kSimtTok][D];
-  float p[16 * RPT][kSimtTok + 4];
+  float p[16 * RPT][kSimtTok + 16];
   TokRow row[16 * RPT];
   int doc[kStages + 1][kSimtTok];
   int64_t src[kStages + 1][kSimtTok];  // row of the key in its tensor, -1 for one that nobody sees
-  int hi;
+  int unseen[kStages + 1];  // has the tile such keys?
+  int hi, min_hi;
   int pre[kMaxEvenBatch + 1];
 };
 
@@ -90,7 +91,10 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
   const int len = tok_len(a, b);
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();  // the previous piece is done with shared memory
-  if (tid == 0) sm.hi = 0;
+  if (tid == 0) {
+    sm.hi = 0;
+    sm.min_hi = INT32_MAX;
+  }
   for (int e = tid; e < RT * kRow; e += kSimtThreads) {
     const int r = e / kRow, x = e % kRow * 4;
     const bool real = rt * RT + r < a.R;
@@ -99,7 +103,10 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
   __syncthreads();
   for (int r = tid; r < RT; r += kSimtThreads) {
     sm.row[r] = tok_row(a, b, h, rt * RT + r, len);
-    if (sm.row[r].hi > 0) atomicMax(&sm.hi, sm.row[r].hi);
+    if (rt * RT + r < a.R) {
+      atomicMax(&sm.hi, sm.row[r].hi);
+      atomicMin(&sm.min_hi, sm.row[r].hi);
+    }
   }
   __syncthreads();
   const int nct = (len + kSimtTok - 1) / kSimtTok;  // tiles of the cache; drafted tokens follow
@@ -107,14 +114,15 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
   const int ncache = (t1 - t0 + kSimtTok - 1) / kSimtTok;
   const int d0 = max(seg.t0 - nct, 0);
   const int ndraft = a.dk && seg.t1 > nct ? min(seg.t1 - nct, (a.Sq + kSimtTok - 1) / kSimtTok) - d0 : 0;
-  const int ntile = ncache + ndraft;
+  const int ntile = ncache + ndraft, min_hi = sm.min_hi;
+  if (tid <= ST) sm.unseen[tid] = -1;
 
   const auto first_key = [&](int tile) {
     return tile >= ncache ? (d0 + tile - ncache) * kSimtTok : t0 + tile * kSimtTok;
   };
   // where the tile's keys lie, and their documents
   const auto mark = [&](int tile) {
-    if (tile >= ntile || tid >= kSimtTok) return;
+    if (tile >= ntile || tid >= kSimtTok) return;  // whole warps
     const int j = first_key(tile) + tid;
     int64_t src = -1;
     int doc = -1;
@@ -127,6 +135,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
     }
     sm.doc[tile % (ST + 1)][tid] = doc;
     sm.src[tile % (ST + 1)][tid] = src;
+    if (__any_sync(0xffffffffu, src < 0) && (tid & 31) == 0) sm.unseen[tile % (ST + 1)] = tile;
   };
   const auto issue = [&](int tile) {
     if (tile < ntile) {
@@ -154,6 +163,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
     for (int x = 0; x < NC * 4; ++x) o[i][x] = 0.f;
   }
 
+  __syncthreads();
   for (int t = 0; t < ST; ++t) mark(t);
   __syncthreads();
   if (ST == 2) issue(0);
@@ -167,6 +177,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
     mark(tile + ST);
     asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
     __syncthreads();
+    const bool unseen = sm.unseen[tile % (ST + 1)] == tile;
 
     float s[RPT][4];
 #pragma unroll
@@ -190,21 +201,45 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
         }
       }
     }
+    // scale, cap, bias (natural units: log2(e) times a score would round once more,
+    // and the exponential magnify that; here it multiplies the difference to the
+    // maximum)
+#pragma unroll
+    for (int i = 0; i < RPT; ++i)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) s[i][n] *= a.scale;
+    if (a.cap > 0.f) {
+#pragma unroll
+      for (int i = 0; i < RPT; ++i)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) s[i][n] = a.cap * tanhf(s[i][n] / a.cap);
+    }
+    if (a.slopes) {
+#pragma unroll
+      for (int i = 0; i < RPT; ++i)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+          s[i][n] = fmaf(-row[i].slope2 * (1.f / kLog2e), fabsf((float)(row[i].pos - (j0 + tx + 16 * n))), s[i][n]);
+    }
+    if (draft || a.docs || unseen || j0 + kSimtTok > min_hi) {  // else every row sees every key
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        const int r = rt * RT + ty + 16 * i;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const int t = tx + 16 * n, j = j0 + t;
+          bool vis = src[t] >= 0;
+          if (draft)
+            vis = vis && r < a.R && a.tree[b * a.tree_bstride + (int64_t)(r / a.G) * a.Sq + j] != 0;
+          else
+            vis = vis && j < row[i].hi && (!a.docs || doc[t] == row[i].doc);
+          if (!vis) s[i][n] = -INFINITY;
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
-      const int r = rt * RT + ty + 16 * i;
-      float mx = -INFINITY;
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const int t = tx + 16 * n, j = j0 + t;
-        bool vis = src[t] >= 0;
-        if (draft)
-          vis = vis && r < a.R && a.tree[b * a.tree_bstride + (int64_t)(r / a.G) * a.Sq + j] != 0;
-        else
-          vis = vis && j < row[i].hi && j < t1 && (!a.docs || doc[t] == row[i].doc);
-        s[i][n] = vis ? tok_score(a, s[i][n], row[i].slope2, row[i].pos, j) : -INFINITY;
-        mx = fmaxf(mx, s[i][n]);
-      }
+      float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
 #pragma unroll
       for (int d = 8; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
       const float m_new = fmaxf(m[i], mx);
