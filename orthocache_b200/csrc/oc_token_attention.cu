@@ -237,6 +237,11 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
         }
       }
     }
+    if (RPT == 1 && a.logits && ty < a.R) {  // kept for the column sums (few rows only)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+        a.logits[((int64_t)bh * a.R + ty) * a.logit_stride + j0 + tx + 16 * n] = s[0][n];
+    }
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
       float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
@@ -503,19 +508,22 @@ int launch_merge(const TokArgs& a, const TokTcShape& tc, cudaStream_t st) {
 // of every query row, added in row order (no atomics: the same inputs give the
 // same sums).  The scores are recomputed from q and k, since the softmax
 // denominators are known only after all keys have been seen.
-template <typename T, int D>
+template <typename T, int D, int RW>
 struct WeightSmem {
   float k[kSimtTok][D + 4];
-  float q[32][D];
-  TokRow row[32];
-  float lse[32];
+  float q[RW][D + 4];
+  TokRow row[RW];
+  float lse[RW];
   float sum[16][kSimtTok];
 };
 
-template <typename T, int D>
+// RW query rows at a time: 64 (1,080 -> 931 us with the attention of 512 rows x 4K, 16
+// heads, D 128), but 32 where there are no more (152 us against 177 for 20 rows x 8K, 4
+// heads, D 256).
+template <typename T, int D, int RW>
 __global__ void __launch_bounds__(kSimtThreads) tok_weights_kernel(const TokArgs a, const float* w_in, float* w_out) {
   extern __shared__ __align__(16) unsigned char raw[];
-  WeightSmem<T, D>& sm = *reinterpret_cast<WeightSmem<T, D>*>(raw);
+  WeightSmem<T, D, RW>& sm = *reinterpret_cast<WeightSmem<T, D, RW>*>(raw);
   constexpr int kVec = Elem<T>::kVec;
   const int bh = blockIdx.x % (a.B * a.Hkv), j0 = blockIdx.x / (a.B * a.Hkv) * kSimtTok;
   const int b = bh / a.Hkv, h = bh % a.Hkv;
@@ -535,13 +543,13 @@ __global__ void __launch_bounds__(kSimtThreads) tok_weights_kernel(const TokArgs
   int first = 0;
   if (a.causal) first = max(0, j0 - (len - a.Sq)) * a.G;
   if (j0 >= len) first = a.R;
-  for (int r0 = first; r0 < a.R; r0 += 32) {
+  for (int r0 = first; r0 < a.R; r0 += RW) {
     __syncthreads();
-    if (tid < 32) {
+    if (tid < RW) {
       sm.row[tid] = tok_row(a, b, h, r0 + tid, len);
       sm.lse[tid] = r0 + tid < a.R ? a.lse[(int64_t)bh * a.R + r0 + tid] * (a.unit / kLog2e) : INFINITY;  // natural
     }
-    for (int e = tid; e < 32 * (D / kVec); e += kSimtThreads) {
+    for (int e = tid; e < RW * (D / kVec); e += kSimtThreads) {
       const int r = e / (D / kVec), x = e % (D / kVec) * kVec;
       if (r0 + r < a.R)
         simt_load_vec<T>(static_cast<const T*>(a.q) + tok_q_offset(a, b, h, r0 + r, D) + x, &sm.q[r][x]);
@@ -550,14 +558,14 @@ __global__ void __launch_bounds__(kSimtThreads) tok_weights_kernel(const TokArgs
         for (int y = 0; y < kVec; ++y) sm.q[r][x + y] = 0.f;
     }
     __syncthreads();
-    float s[2][4] = {};
+    float s[RW / 16][4] = {};
 #pragma unroll 4
     for (int x = 0; x < D; x += 4) {
       float4 kk[4];
 #pragma unroll
       for (int n = 0; n < 4; ++n) kk[n] = *reinterpret_cast<const float4*>(&sm.k[tx + 16 * n][x]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < RW / 16; ++i) {
         const float4 qq = *reinterpret_cast<const float4*>(&sm.q[ty + 16 * i][x]);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
@@ -569,7 +577,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_weights_kernel(const TokArgs
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < RW / 16; ++i) {
       const TokRow row = sm.row[ty + 16 * i];
       const float lse = sm.lse[ty + 16 * i];
 #pragma unroll
@@ -604,7 +612,7 @@ __global__ void __launch_bounds__(256) tok_sum_kernel(const TokArgs a, int block
   if (j < len) {
     const float* s = a.logits + (int64_t)bh * a.R * a.logit_stride + j;
 #pragma unroll 8
-    for (int r = 0; r < a.R; ++r) sum += exp2f(s[r * a.logit_stride] - a.lse[(int64_t)bh * a.R + r]);
+    for (int r = 0; r < a.R; ++r) sum += exp2f((s[r * a.logit_stride] - a.lse[(int64_t)bh * a.R + r]) * a.unit);
   }
   w_out[at] = before + sum;
 }
@@ -648,9 +656,9 @@ inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 constexpr int kMinTiles = 2;
 
 // The accumulating form needs every score again once the denominators are
-// known.  Up to kLogitRows rows per KV head the bfloat16 kernel stores them
-// (4 bytes a row and key, against 2 D bytes of a key to multiply again: at 16
-// rows and 128 channels 64 against 256); beyond, they are recomputed.
+// known.  Up to kLogitRows rows per KV head the kernels store them
+// (4 bytes a row and key, against 2 D or 4 D bytes of a key to multiply again: at
+// 16 rows and 128 channels 64 against 256 or 512); beyond, they are recomputed.
 constexpr int kLogitRows = 16;
 
 TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int head_dim, int seq_len, int draft_len,
@@ -699,7 +707,7 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
   if (p.tc) off += up256(tok_tc_prep_bytes(batch, q_len, G, head_dim, seq_len));
   p.logit_off = off;
   p.logit_stride = 0;
-  if (lse && dtype == OC_BF16 && !p.tc && R <= kLogitRows) {
+  if (lse && !p.tc && R <= kLogitRows) {
     p.logit_stride = (seq_len + 63) / 64 * 64;  // whole tiles
     off += up256((size_t)batch * kv_heads * R * p.logit_stride * sizeof(float));
   }
@@ -723,23 +731,25 @@ int dispatch_simt(const TokArgs& a, int D, int row_tile, cudaStream_t st) {
   return row_tile == 16 ? launch_simt<256, 1>(a, st) : launch_simt<256, 4>(a, st);
 }
 
-template <typename T, int D>
+template <typename T, int D, int RW>
 int launch_weights(const TokArgs& a, const float* w_in, float* w_out, cudaStream_t st) {
-  const size_t smem = sizeof(WeightSmem<T, D>);
+  const size_t smem = sizeof(WeightSmem<T, D, RW>);
   static std::atomic<uint64_t> done{0};
-  cudaError_t e = allow_smem(done, tok_weights_kernel<T, D>, smem);
+  cudaError_t e = allow_smem(done, tok_weights_kernel<T, D, RW>, smem);
   if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_weights_kernel: %s", cudaGetErrorString(e));
   const int64_t blocks = (int64_t)((a.S + kSimtTok - 1) / kSimtTok) * a.B * a.Hkv;
-  e = launch_pdl(tok_weights_kernel<T, D>, dim3((unsigned)blocks), dim3(kSimtThreads), smem, st, a, w_in, w_out);
+  e = launch_pdl(tok_weights_kernel<T, D, RW>, dim3((unsigned)blocks), dim3(kSimtThreads), smem, st, a, w_in, w_out);
   if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_weights_kernel: %s", cudaGetErrorString(e));
   return OC_OK;
 }
 
 template <typename T>
 int dispatch_weights(const TokArgs& a, int D, const float* w_in, float* w_out, cudaStream_t st) {
-  if (D == 64) return launch_weights<T, 64>(a, w_in, w_out, st);
-  if (D == 128) return launch_weights<T, 128>(a, w_in, w_out, st);
-  return launch_weights<T, 256>(a, w_in, w_out, st);
+  const bool few = a.R <= 32;
+  if (D == 64) return few ? launch_weights<T, 64, 32>(a, w_in, w_out, st) : launch_weights<T, 64, 64>(a, w_in, w_out, st);
+  if (D == 128)
+    return few ? launch_weights<T, 128, 32>(a, w_in, w_out, st) : launch_weights<T, 128, 64>(a, w_in, w_out, st);
+  return few ? launch_weights<T, 256, 32>(a, w_in, w_out, st) : launch_weights<T, 256, 64>(a, w_in, w_out, st);
 }
 
 constexpr float kMaxScaleOfCap = 4096.f;
