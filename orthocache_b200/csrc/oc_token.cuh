@@ -23,6 +23,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ constexpr float kTanh[4] = {-0.3333306908607483f, 0.13324779272079468f, -0.05298607423901558f,
                                        0.017135007306933403f};
 constexpr float kTanhMax = 0.5f;
+__device__ __forceinline__ float tok_tanh(float z) {
+  const float u = z * z;
+  float p = fmaf(kTanh[3], u, kTanh[2]);
+  p = fmaf(p, u, kTanh[1]);
+  p = fmaf(p, u, kTanh[0]);
+  return fmaf(z * u, p, z);
+}
 constexpr int kMaxNodes = 256;  // drafted tokens of one tree
 
 struct TokArgs {

@@ -36,6 +36,7 @@ struct SimtSmem {
   int64_t src[kStages + 1][kSimtTok];  // row of the key in its tensor, -1 for one that nobody sees
   int unseen[kStages + 1];  // has the tile such keys?
   int hi, min_hi;
+  int span[4];  // least and largest document of the rows, first key and last + 1 of those between
   int pre[kMaxEvenBatch + 1];
 };
 
@@ -94,6 +95,8 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
   if (tid == 0) {
     sm.hi = 0;
     sm.min_hi = INT32_MAX;
+    sm.span[0] = sm.span[2] = INT32_MAX;
+    sm.span[1] = sm.span[3] = -1;
   }
   for (int e = tid; e < RT * kRow; e += kSimtThreads) {
     const int r = e / kRow, x = e % kRow * 4;
@@ -106,11 +109,32 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
     if (rt * RT + r < a.R) {
       atomicMax(&sm.hi, sm.row[r].hi);
       atomicMin(&sm.min_hi, sm.row[r].hi);
+      if (a.docs && sm.row[r].hi > 0) {
+        atomicMin(&sm.span[0], sm.row[r].doc);
+        atomicMax(&sm.span[1], sm.row[r].doc);
+      }
     }
   }
   __syncthreads();
   const int nct = (len + kSimtTok - 1) / kSimtTok;  // tiles of the cache; drafted tokens follow
-  const int t0 = min(seg.t0, nct) * kSimtTok, t1 = max(t0, min(sm.hi, min(seg.t1, nct) * kSimtTok));
+  int t0 = min(seg.t0, nct) * kSimtTok, t1 = max(t0, min(sm.hi, min(seg.t1, nct) * kSimtTok));
+  if (a.docs && t0 < t1) {  // the tiles that hold any of the rows' documents
+    int first = INT32_MAX, last = -1;
+    for (int j = t0 + tid; j < t1; j += kSimtThreads) {
+      const int d = a.docs[(size_t)b * a.S + j];
+      if (d >= sm.span[0] && d <= sm.span[1]) {
+        first = min(first, j);
+        last = max(last, j + 1);
+      }
+    }
+    if (last >= 0) {
+      atomicMin(&sm.span[2], first);
+      atomicMax(&sm.span[3], last);
+    }
+    __syncthreads();
+    t1 = min(t1, max(t0, sm.span[3]));
+    if (sm.span[2] < t1) t0 = sm.span[2] / kSimtTok * kSimtTok;
+  }
   const int ncache = (t1 - t0 + kSimtTok - 1) / kSimtTok;
   const int d0 = max(seg.t0 - nct, 0);
   const int ndraft = a.dk && seg.t1 > nct ? min(seg.t1 - nct, (a.Sq + kSimtTok - 1) / kSimtTok) - d0 : 0;
@@ -204,15 +228,27 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
     // scale, cap, bias (natural units: log2(e) times a score would round once more,
     // and the exponential magnify that; here it multiplies the difference to the
     // maximum)
+    const float in = a.cap > 0.f ? a.scale / a.cap : a.scale;
+    float top = 0.f;
 #pragma unroll
     for (int i = 0; i < RPT; ++i)
 #pragma unroll
-      for (int n = 0; n < 4; ++n) s[i][n] *= a.scale;
+      for (int n = 0; n < 4; ++n) {
+        s[i][n] *= in;
+        top = fmaxf(top, fabsf(s[i][n]));
+      }
     if (a.cap > 0.f) {
+      if (__all_sync(0xffffffffu, top <= kTanhMax)) {  // (NaN may pass: it stays NaN)
 #pragma unroll
-      for (int i = 0; i < RPT; ++i)
+        for (int i = 0; i < RPT; ++i)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) s[i][n] = a.cap * tanhf(s[i][n] / a.cap);
+          for (int n = 0; n < 4; ++n) s[i][n] = a.cap * tok_tanh(s[i][n]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < RPT; ++i)
+#pragma unroll
+          for (int n = 0; n < 4; ++n) s[i][n] = a.cap * tanhf(s[i][n]);
+      }
     }
     if (a.slopes) {
 #pragma unroll

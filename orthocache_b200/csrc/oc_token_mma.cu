@@ -274,13 +274,7 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
 #pragma unroll
         for (int n = 0; n < C::NT; ++n)
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float z = s[n][y], u = z * z;
-            float p = fmaf(kTanh[3], u, kTanh[2]);
-            p = fmaf(p, u, kTanh[1]);
-            p = fmaf(p, u, kTanh[0]);
-            s[n][y] = c_cap * fmaf(z * u, p, z);
-          }
+          for (int y = 0; y < 4; ++y) s[n][y] = c_cap * tok_tanh(s[n][y]);
       } else {
 #pragma unroll
         for (int n = 0; n < C::NT; ++n)
