@@ -212,6 +212,10 @@ __device__ __forceinline__ float tok_score(const TokArgs& a, float dot, float sl
 int tok_mma(const TokArgs& a, int head_dim, int row_tile, cudaStream_t st);
 int tok_mma_tile(int head_dim);  // keys of its tiles
 
+// The float32 kernel for few rows (oc_token_few.cu): units of 16 rows.
+int tok_few(const TokArgs& a, int head_dim, cudaStream_t st);
+int tok_few_tile(int head_dim);
+
 // The bfloat16 kernel on the tcgen05 tensor cores (oc_token_tc.cu) for
 // a positive scale; a unit is one or two row tiles.
 // prep: tok_tc_prep_bytes of scratch.

@@ -21,12 +21,13 @@ namespace {
 
 constexpr int kSimtThreads = 256;
 constexpr int kSimtTok = 64;  // keys per tile
+constexpr int RPT = 4;        // rows of a thread
 
 // Rows are padded, so that the 16 keys a half-warp reads at once, and the rows of
 // its two halves, fall into different banks.
-template <int D, int RPT>
+template <int D>
 struct SimtSmem {
-  static constexpr int kStages = D == 64 || (D == 128 && RPT == 4) ? 2 : 1;  // two where that costs no CTA of the SM
+  static constexpr int kStages = D <= 128 ? 2 : 1;  // what fits beside the queries
   float q[16 * RPT][D + 4];
   float k[kStages][kSimtTok][D + 4];
   float v[kStages][kSimtTok][D];
@@ -64,10 +65,10 @@ __device__ __forceinline__ void simt_load_vec(const T* src, float* dst) {
 // values is on its way (cp.async) while one is multiplied; keys that no row may
 // see (behind the sequence, padding, pages outside the pool) are filled with
 // zeros, so that whatever the memory holds there cannot reach a result.
-template <int D, int RPT>
+template <int D>
 __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a) {
   extern __shared__ __align__(16) unsigned char raw[];
-  using Smem = SimtSmem<D, RPT>;
+  using Smem = SimtSmem<D>;
   Smem& sm = *reinterpret_cast<Smem*>(raw);
   constexpr int RT = 16 * RPT, NC = D / 64, ST = Smem::kStages, kRow = D / 4;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
@@ -272,11 +273,6 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
           if (!vis) s[i][n] = -INFINITY;
         }
       }
-    }
-    if (RPT == 1 && a.logits && ty < a.R) {  // kept for the column sums (few rows only)
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-        a.logits[((int64_t)bh * a.R + ty) * a.logit_stride + j0 + tx + 16 * n] = s[0][n];
     }
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
@@ -714,8 +710,8 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
     p.row_tile = R <= 16 ? 16 : R <= 32 ? (dtype == OC_BF16 ? 32 : 16) : 64;
     p.nrt = (int)((R + p.row_tile - 1) / p.row_tile);
     p.unit_rows = p.row_tile;
-    p.tile = dtype == OC_BF16 ? tok_mma_tile(head_dim) : kSimtTok;
-    // CTAs of an SM: the float32 kernel's shared memory leaves room for one from 128 channels on
+    p.tile = dtype == OC_BF16 ? tok_mma_tile(head_dim) : p.row_tile == 16 ? tok_few_tile(head_dim) : kSimtTok;
+    // CTAs that an SM's shared memory holds
     slots *= dtype == OC_BF16 || head_dim == 64 || (head_dim == 128 && p.row_tile == 16) ? 2 : 1;
   }
   p.units = (int64_t)batch * kv_heads * p.nrt;
@@ -751,20 +747,18 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
   return p;
 }
 
-template <int D, int RPT>
+template <int D>
 int launch_simt(const TokArgs& a, cudaStream_t st) {
-  const size_t smem = sizeof(SimtSmem<D, RPT>);
+  const size_t smem = sizeof(SimtSmem<D>);
   static std::atomic<uint64_t> done{0};
-  const cudaError_t e = allow_smem(done, tok_simt_kernel<D, RPT>, smem);
+  const cudaError_t e = allow_smem(done, tok_simt_kernel<D>, smem);
   if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_simt_kernel: %s", cudaGetErrorString(e));
-  tok_simt_kernel<D, RPT><<<a.even ? a.ncta : a.B * a.Hkv * a.nrt, kSimtThreads, smem, st>>>(a);
+  tok_simt_kernel<D><<<a.even ? a.ncta : a.B * a.Hkv * a.nrt, kSimtThreads, smem, st>>>(a);
   return check_launch("tok_simt_kernel");
 }
 
-int dispatch_simt(const TokArgs& a, int D, int row_tile, cudaStream_t st) {
-  if (D == 64) return row_tile == 16 ? launch_simt<64, 1>(a, st) : launch_simt<64, 4>(a, st);
-  if (D == 128) return row_tile == 16 ? launch_simt<128, 1>(a, st) : launch_simt<128, 4>(a, st);
-  return row_tile == 16 ? launch_simt<256, 1>(a, st) : launch_simt<256, 4>(a, st);
+int dispatch_simt(const TokArgs& a, int D, cudaStream_t st) {
+  return D == 64 ? launch_simt<64>(a, st) : D == 128 ? launch_simt<128>(a, st) : launch_simt<256>(a, st);
 }
 
 template <typename T, int D, int RW>
@@ -858,7 +852,8 @@ int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void*
   a.unit = dtype == OC_BF16 ? 1.f : kLog2e;
   int rc = p.tc ? tok_tc(fn, a, head_dim, w + p.prep_off, st)
            : dtype == OC_BF16 ? tok_mma(a, head_dim, p.row_tile, st)
-                              : dispatch_simt(a, head_dim, p.row_tile, st);
+           : p.row_tile == 16 ? tok_few(a, head_dim, st)
+                              : dispatch_simt(a, head_dim, st);
   if (rc) return rc;
   if (p.even) rc = tok_merge(a, head_dim, p.tc, st);
   if (rc || !w_out || a.S == 0) return rc;
