@@ -1,6 +1,6 @@
-// Token-level attention: entry points, the float32-arithmetic kernel that
-// serves every type and size, the merge of partials split over the keys, and
-// the column sums of the attention weights.
+// Token-level attention: entry points, the float32 kernel for more than a few
+// rows, the merge of partials split over the keys, and the column sums of the
+// attention weights.
 //
 // oc_tree_attention: T drafted tokens, arranged in a tree, attend to a
 // cache and to their own ancestors.  oc_chunk_attention: a query chunk at the
@@ -21,18 +21,18 @@ namespace {
 
 constexpr int kSimtThreads = 256;
 constexpr int kSimtTok = 64;  // keys per tile
-constexpr int RPT = 4;        // rows of a thread
+constexpr int kRpt = 4;        // rows of a thread
 
 // Rows are padded, so that the 16 keys a half-warp reads at once, and the rows of
 // its two halves, fall into different banks.
 template <int D>
 struct SimtSmem {
   static constexpr int kStages = D <= 128 ? 2 : 1;  // what fits beside the queries
-  float q[16 * RPT][D + 4];
+  float q[16 * kRpt][D + 4];
   float k[kStages][kSimtTok][D + 4];
   float v[kStages][kSimtTok][D];
-  float p[16 * RPT][kSimtTok + 16];
-  TokRow row[16 * RPT];
+  float p[16 * kRpt][kSimtTok + 16];
+  TokRow row[16 * kRpt];
   int doc[kStages + 1][kSimtTok];
   int64_t src[kStages + 1][kSimtTok];  // row of the key in its tensor, -1 for one that nobody sees
   int unseen[kStages + 1];  // has the tile such keys?
@@ -57,7 +57,7 @@ __device__ __forceinline__ void simt_load_vec(const T* src, float* dst) {
   for (int c = 0; c < kVec; ++c) dst[c] = f[c];
 }
 
-// Row tiles of 16 * RPT query rows against tiles of 64 keys, one pass with
+// Row tiles of 64 query rows against tiles of 64 keys, one pass with
 // the running maximum and sum of the softmax; 256 threads as 16 x 16: thread
 // (ty, tx) owns rows ty + 16 i, the scores of keys tx + 16 n, and the output
 // channels 4 tx + 64 c of its rows, so that the softmax statistics stay in
@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
   extern __shared__ __align__(16) unsigned char raw[];
   using Smem = SimtSmem<D>;
   Smem& sm = *reinterpret_cast<Smem*>(raw);
-  constexpr int RT = 16 * RPT, NC = D / 64, ST = Smem::kStages, kRow = D / 4;
+  constexpr int RT = 16 * kRpt, NC = D / 64, ST = Smem::kStages, kRow = D / 4;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const float* qbase = static_cast<const float*>(a.q);
   pdl_trigger();  // the merge may find its parts meanwhile
@@ -81,277 +81,277 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
   TokWalk walk(a, sm.pre, blockIdx.x);
   TokSeg seg;
   for (bool more = true; more;) {
-  if (a.even) {
-    if (!walk.next(a, sm.pre, blockIdx.x, seg)) break;
-  } else {
-    // a CTA per unit, the rows with most keys first
-    const int bh = blockIdx.x % (a.B * a.Hkv);
-    seg = TokSeg{bh / a.Hkv, bh % a.Hkv * a.nrt + a.nrt - 1 - (int)(blockIdx.x / (a.B * a.Hkv)), 0, INT32_MAX, -1};
-    more = false;
-  }
-  const int b = seg.b, h = seg.unit / a.nrt, rt = seg.unit % a.nrt, bh = b * a.Hkv + h;
-  const int len = tok_len(a, b);
-  asm volatile("cp.async.wait_all;" ::: "memory");
-  __syncthreads();  // the previous piece is done with shared memory
-  if (tid == 0) {
-    sm.hi = 0;
-    sm.min_hi = INT32_MAX;
-    sm.span[0] = sm.span[2] = INT32_MAX;
-    sm.span[1] = sm.span[3] = -1;
-  }
-  for (int e = tid; e < RT * kRow; e += kSimtThreads) {
-    const int r = e / kRow, x = e % kRow * 4;
-    const bool real = rt * RT + r < a.R;
-    simt_cp16(&sm.q[r][x], qbase + (real ? tok_q_offset(a, b, h, rt * RT + r, D) + x : 0), real);
-  }
-  __syncthreads();
-  for (int r = tid; r < RT; r += kSimtThreads) {
-    sm.row[r] = tok_row(a, b, h, rt * RT + r, len);
-    if (rt * RT + r < a.R) {
-      atomicMax(&sm.hi, sm.row[r].hi);
-      atomicMin(&sm.min_hi, sm.row[r].hi);
-      if (a.docs && sm.row[r].hi > 0) {
-        atomicMin(&sm.span[0], sm.row[r].doc);
-        atomicMax(&sm.span[1], sm.row[r].doc);
-      }
+    if (a.even) {
+      if (!walk.next(a, sm.pre, blockIdx.x, seg)) break;
+    } else {
+      // a CTA per unit, the rows with most keys first
+      const int bh = blockIdx.x % (a.B * a.Hkv);
+      seg = TokSeg{bh / a.Hkv, bh % a.Hkv * a.nrt + a.nrt - 1 - (int)(blockIdx.x / (a.B * a.Hkv)), 0, INT32_MAX, -1};
+      more = false;
     }
-  }
-  __syncthreads();
-  const int nct = (len + kSimtTok - 1) / kSimtTok;  // tiles of the cache; drafted tokens follow
-  int t0 = min(seg.t0, nct) * kSimtTok, t1 = max(t0, min(sm.hi, min(seg.t1, nct) * kSimtTok));
-  if (a.docs && t0 < t1) {  // the tiles that hold any of the rows' documents
-    int first = INT32_MAX, last = -1;
-    for (int j = t0 + tid; j < t1; j += kSimtThreads) {
-      const int d = a.docs[(size_t)b * a.S + j];
-      if (d >= sm.span[0] && d <= sm.span[1]) {
-        first = min(first, j);
-        last = max(last, j + 1);
-      }
+    const int b = seg.b, h = seg.unit / a.nrt, rt = seg.unit % a.nrt, bh = b * a.Hkv + h;
+    const int len = tok_len(a, b);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // the previous piece is done with shared memory
+    if (tid == 0) {
+      sm.hi = 0;
+      sm.min_hi = INT32_MAX;
+      sm.span[0] = sm.span[2] = INT32_MAX;
+      sm.span[1] = sm.span[3] = -1;
     }
-    if (last >= 0) {
-      atomicMin(&sm.span[2], first);
-      atomicMax(&sm.span[3], last);
+    for (int e = tid; e < RT * kRow; e += kSimtThreads) {
+      const int r = e / kRow, x = e % kRow * 4;
+      const bool real = rt * RT + r < a.R;
+      simt_cp16(&sm.q[r][x], qbase + (real ? tok_q_offset(a, b, h, rt * RT + r, D) + x : 0), real);
     }
     __syncthreads();
-    t1 = min(t1, max(t0, sm.span[3]));
-    if (sm.span[2] < t1) t0 = sm.span[2] / kSimtTok * kSimtTok;
-  }
-  const int ncache = (t1 - t0 + kSimtTok - 1) / kSimtTok;
-  const int d0 = max(seg.t0 - nct, 0);
-  const int ndraft = a.dk && seg.t1 > nct ? min(seg.t1 - nct, (a.Sq + kSimtTok - 1) / kSimtTok) - d0 : 0;
-  const int ntile = ncache + ndraft, min_hi = sm.min_hi;
-  if (tid <= ST) sm.unseen[tid] = -1;
-
-  const auto first_key = [&](int tile) {
-    return tile >= ncache ? (d0 + tile - ncache) * kSimtTok : t0 + tile * kSimtTok;
-  };
-  // where the tile's keys lie, and their documents
-  const auto mark = [&](int tile) {
-    if (tile >= ntile || tid >= kSimtTok) return;  // whole warps
-    const int j = first_key(tile) + tid;
-    int64_t src = -1;
-    int doc = -1;
-    if (tile >= ncache) {
-      for (int i = 0; j < a.Sq && i < a.Sq && src < 0; ++i)
-        if (a.tree[b * a.tree_bstride + (int64_t)i * a.Sq + j]) src = (int64_t)b * a.Sq + j;
-    } else if (j < len) {
-      doc = a.docs ? a.docs[(size_t)b * a.S + j] : 0;
-      if (doc >= 0) src = tok_kv_row(a, b, j);
-    }
-    sm.doc[tile % (ST + 1)][tid] = doc;
-    sm.src[tile % (ST + 1)][tid] = src;
-    if (__any_sync(0xffffffffu, src < 0) && (tid & 31) == 0) sm.unseen[tile % (ST + 1)] = tile;
-  };
-  const auto issue = [&](int tile) {
-    if (tile < ntile) {
-      const float* kp = static_cast<const float*>(tile >= ncache ? a.dk : a.k);
-      const float* vp = static_cast<const float*>(tile >= ncache ? a.dv : a.v);
-#pragma unroll 4
-      for (int e = tid; e < kSimtTok * kRow; e += kSimtThreads) {
-        const int t = e / kRow, x = e % kRow * 4;
-        const int64_t src = sm.src[tile % (ST + 1)][t], at = (src * a.Hkv + h) * D + x;
-        simt_cp16(&sm.k[tile % ST][t][x], src >= 0 ? kp + at : qbase, src >= 0);
-        simt_cp16(&sm.v[tile % ST][t][x], src >= 0 ? vp + at : qbase, src >= 0);
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-
-  TokRow row[RPT];
-  float m[RPT], l[RPT], o[RPT][NC * 4];
-#pragma unroll
-  for (int i = 0; i < RPT; ++i) {
-    row[i] = sm.row[ty + 16 * i];
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-#pragma unroll
-    for (int x = 0; x < NC * 4; ++x) o[i][x] = 0.f;
-  }
-
-  __syncthreads();
-  for (int t = 0; t < ST; ++t) mark(t);
-  __syncthreads();
-  if (ST == 2) issue(0);
-  for (int tile = 0; tile < ntile; ++tile) {
-    const bool draft = tile >= ncache;
-    const int j0 = first_key(tile), at = tile % ST;
-    const int *doc = sm.doc[tile % (ST + 1)];
-    const int64_t* src = sm.src[tile % (ST + 1)];
-    __syncthreads();  // the tile before is read, the next one marked
-    issue(tile + ST - 1);
-    mark(tile + ST);
-    asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
-    __syncthreads();
-    const bool unseen = sm.unseen[tile % (ST + 1)] == tile;
-
-    float s[RPT][4];
-#pragma unroll
-    for (int i = 0; i < RPT; ++i)
-#pragma unroll
-      for (int n = 0; n < 4; ++n) s[i][n] = 0.f;
-#pragma unroll 4
-    for (int x = 0; x < D; x += 4) {
-      float4 kk[4];
-#pragma unroll
-      for (int n = 0; n < 4; ++n) kk[n] = *reinterpret_cast<const float4*>(&sm.k[at][tx + 16 * n][x]);
-#pragma unroll
-      for (int i = 0; i < RPT; ++i) {
-        const float4 qq = *reinterpret_cast<const float4*>(&sm.q[ty + 16 * i][x]);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          s[i][n] = fmaf(qq.x, kk[n].x, s[i][n]);
-          s[i][n] = fmaf(qq.y, kk[n].y, s[i][n]);
-          s[i][n] = fmaf(qq.z, kk[n].z, s[i][n]);
-          s[i][n] = fmaf(qq.w, kk[n].w, s[i][n]);
+    for (int r = tid; r < RT; r += kSimtThreads) {
+      sm.row[r] = tok_row(a, b, h, rt * RT + r, len);
+      if (rt * RT + r < a.R) {
+        atomicMax(&sm.hi, sm.row[r].hi);
+        atomicMin(&sm.min_hi, sm.row[r].hi);
+        if (a.docs && sm.row[r].hi > 0) {
+          atomicMin(&sm.span[0], sm.row[r].doc);
+          atomicMax(&sm.span[1], sm.row[r].doc);
         }
       }
     }
-    // scale, cap, bias (natural units: log2(e) times a score would round once more,
-    // and the exponential magnify that; here it multiplies the difference to the
-    // maximum)
-    const float in = a.cap > 0.f ? a.scale / a.cap : a.scale;
-    float top = 0.f;
-#pragma unroll
-    for (int i = 0; i < RPT; ++i)
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        s[i][n] *= in;
-        top = fmaxf(top, fabsf(s[i][n]));
-      }
-    if (a.cap > 0.f) {
-      if (__all_sync(0xffffffffu, top <= kTanhMax)) {  // (NaN may pass: it stays NaN)
-#pragma unroll
-        for (int i = 0; i < RPT; ++i)
-#pragma unroll
-          for (int n = 0; n < 4; ++n) s[i][n] = a.cap * tok_tanh(s[i][n]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < RPT; ++i)
-#pragma unroll
-          for (int n = 0; n < 4; ++n) s[i][n] = a.cap * tanhf(s[i][n]);
-      }
-    }
-    if (a.slopes) {
-#pragma unroll
-      for (int i = 0; i < RPT; ++i)
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-          s[i][n] = fmaf(-row[i].slope2 * (1.f / kLog2e), fabsf((float)(row[i].pos - (j0 + tx + 16 * n))), s[i][n]);
-    }
-    if (draft || a.docs || unseen || j0 + kSimtTok > min_hi) {  // else every row sees every key
-#pragma unroll
-      for (int i = 0; i < RPT; ++i) {
-        const int r = rt * RT + ty + 16 * i;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const int t = tx + 16 * n, j = j0 + t;
-          bool vis = src[t] >= 0;
-          if (draft)
-            vis = vis && r < a.R && a.tree[b * a.tree_bstride + (int64_t)(r / a.G) * a.Sq + j] != 0;
-          else
-            vis = vis && j < row[i].hi && (!a.docs || doc[t] == row[i].doc);
-          if (!vis) s[i][n] = -INFINITY;
+    __syncthreads();
+    const int nct = (len + kSimtTok - 1) / kSimtTok;  // tiles of the cache; drafted tokens follow
+    int t0 = min(seg.t0, nct) * kSimtTok, t1 = max(t0, min(sm.hi, min(seg.t1, nct) * kSimtTok));
+    if (a.docs && t0 < t1) {  // the tiles that hold any of the rows' documents
+      int first = INT32_MAX, last = -1;
+      for (int j = t0 + tid; j < t1; j += kSimtThreads) {
+        const int d = a.docs[(size_t)b * a.S + j];
+        if (d >= sm.span[0] && d <= sm.span[1]) {
+          first = min(first, j);
+          last = max(last, j + 1);
         }
       }
+      if (last >= 0) {
+        atomicMin(&sm.span[2], first);
+        atomicMax(&sm.span[3], last);
+      }
+      __syncthreads();
+      t1 = min(t1, max(t0, sm.span[3]));
+      if (sm.span[2] < t1) t0 = sm.span[2] / kSimtTok * kSimtTok;
     }
+    const int ncache = (t1 - t0 + kSimtTok - 1) / kSimtTok;
+    const int d0 = max(seg.t0 - nct, 0);
+    const int ndraft = a.dk && seg.t1 > nct ? min(seg.t1 - nct, (a.Sq + kSimtTok - 1) / kSimtTok) - d0 : 0;
+    const int ntile = ncache + ndraft, min_hi = sm.min_hi;
+    if (tid <= ST) sm.unseen[tid] = -1;
+
+    const auto first_key = [&](int tile) {
+      return tile >= ncache ? (d0 + tile - ncache) * kSimtTok : t0 + tile * kSimtTok;
+    };
+    // where the tile's keys lie, and their documents
+    const auto mark = [&](int tile) {
+      if (tile >= ntile || tid >= kSimtTok) return;  // whole warps
+      const int j = first_key(tile) + tid;
+      int64_t src = -1;
+      int doc = -1;
+      if (tile >= ncache) {
+        for (int i = 0; j < a.Sq && i < a.Sq && src < 0; ++i)
+          if (a.tree[b * a.tree_bstride + (int64_t)i * a.Sq + j]) src = (int64_t)b * a.Sq + j;
+      } else if (j < len) {
+        doc = a.docs ? a.docs[(size_t)b * a.S + j] : 0;
+        if (doc >= 0) src = tok_kv_row(a, b, j);
+      }
+      sm.doc[tile % (ST + 1)][tid] = doc;
+      sm.src[tile % (ST + 1)][tid] = src;
+      if (__any_sync(0xffffffffu, src < 0) && (tid & 31) == 0) sm.unseen[tile % (ST + 1)] = tile;
+    };
+    const auto issue = [&](int tile) {
+      if (tile < ntile) {
+        const float* kp = static_cast<const float*>(tile >= ncache ? a.dk : a.k);
+        const float* vp = static_cast<const float*>(tile >= ncache ? a.dv : a.v);
+#pragma unroll 4
+        for (int e = tid; e < kSimtTok * kRow; e += kSimtThreads) {
+          const int t = e / kRow, x = e % kRow * 4;
+          const int64_t src = sm.src[tile % (ST + 1)][t], at = (src * a.Hkv + h) * D + x;
+          simt_cp16(&sm.k[tile % ST][t][x], src >= 0 ? kp + at : qbase, src >= 0);
+          simt_cp16(&sm.v[tile % ST][t][x], src >= 0 ? vp + at : qbase, src >= 0);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    TokRow row[kRpt];
+    float m[kRpt], l[kRpt], o[kRpt][NC * 4];
 #pragma unroll
-    for (int i = 0; i < RPT; ++i) {
-      float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
+    for (int i = 0; i < kRpt; ++i) {
+      row[i] = sm.row[ty + 16 * i];
+      m[i] = -INFINITY;
+      l[i] = 0.f;
 #pragma unroll
-      for (int d = 8; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-      const float m_new = fmaxf(m[i], mx);
-      const float base = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = exp2f((m[i] - base) * kLog2e);
-      float sum = 0.f;
+      for (int x = 0; x < NC * 4; ++x) o[i][x] = 0.f;
+    }
+
+    __syncthreads();
+    for (int t = 0; t < ST; ++t) mark(t);
+    __syncthreads();
+    if (ST == 2) issue(0);
+    for (int tile = 0; tile < ntile; ++tile) {
+      const bool draft = tile >= ncache;
+      const int j0 = first_key(tile), at = tile % ST;
+      const int *doc = sm.doc[tile % (ST + 1)];
+      const int64_t* src = sm.src[tile % (ST + 1)];
+      __syncthreads();  // the tile before is read, the next one marked
+      issue(tile + ST - 1);
+      mark(tile + ST);
+      asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
+      __syncthreads();
+      const bool unseen = sm.unseen[tile % (ST + 1)] == tile;
+
+      float s[kRpt][4];
 #pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const float p = exp2f((s[i][n] - base) * kLog2e);
-        sm.p[ty + 16 * i][tx + 16 * n] = p;
-        sum += p;
+      for (int i = 0; i < kRpt; ++i)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) s[i][n] = 0.f;
+#pragma unroll 4
+      for (int x = 0; x < D; x += 4) {
+        float4 kk[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) kk[n] = *reinterpret_cast<const float4*>(&sm.k[at][tx + 16 * n][x]);
+#pragma unroll
+        for (int i = 0; i < kRpt; ++i) {
+          const float4 qq = *reinterpret_cast<const float4*>(&sm.q[ty + 16 * i][x]);
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            s[i][n] = fmaf(qq.x, kk[n].x, s[i][n]);
+            s[i][n] = fmaf(qq.y, kk[n].y, s[i][n]);
+            s[i][n] = fmaf(qq.z, kk[n].z, s[i][n]);
+            s[i][n] = fmaf(qq.w, kk[n].w, s[i][n]);
+          }
+        }
+      }
+      // scale, cap, bias (natural units: log2(e) times a score would round once more,
+      // and the exponential magnify that; here it multiplies the difference to the
+      // maximum)
+      const float in = a.cap > 0.f ? a.scale / a.cap : a.scale;
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < kRpt; ++i)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          s[i][n] *= in;
+          top = fmaxf(top, fabsf(s[i][n]));
+        }
+      if (a.cap > 0.f) {
+        if (__all_sync(0xffffffffu, top <= kTanhMax)) {  // (NaN may pass: it stays NaN)
+#pragma unroll
+          for (int i = 0; i < kRpt; ++i)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) s[i][n] = a.cap * tok_tanh(s[i][n]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kRpt; ++i)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) s[i][n] = a.cap * tanhf(s[i][n]);
+        }
+      }
+      if (a.slopes) {
+#pragma unroll
+        for (int i = 0; i < kRpt; ++i)
+#pragma unroll
+          for (int n = 0; n < 4; ++n)
+            s[i][n] = fmaf(-row[i].slope2 * (1.f / kLog2e), fabsf((float)(row[i].pos - (j0 + tx + 16 * n))), s[i][n]);
+      }
+      if (draft || a.docs || unseen || j0 + kSimtTok > min_hi) {  // else every row sees every key
+#pragma unroll
+        for (int i = 0; i < kRpt; ++i) {
+          const int r = rt * RT + ty + 16 * i;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const int t = tx + 16 * n, j = j0 + t;
+            bool vis = src[t] >= 0;
+            if (draft)
+              vis = vis && r < a.R && a.tree[b * a.tree_bstride + (int64_t)(r / a.G) * a.Sq + j] != 0;
+            else
+              vis = vis && j < row[i].hi && (!a.docs || doc[t] == row[i].doc);
+            if (!vis) s[i][n] = -INFINITY;
+          }
+        }
       }
 #pragma unroll
-      for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      l[i] = l[i] * alpha + sum;
-      m[i] = m_new;
+      for (int i = 0; i < kRpt; ++i) {
+        float mx = fmaxf(fmaxf(s[i][0], s[i][1]), fmaxf(s[i][2], s[i][3]));
 #pragma unroll
-      for (int x = 0; x < NC * 4; ++x) o[i][x] *= alpha;
-    }
-    __syncwarp();  // a half-warp reads back only the rows it wrote
+        for (int d = 8; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        const float m_new = fmaxf(m[i], mx);
+        const float base = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = exp2f((m[i] - base) * kLog2e);
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const float p = exp2f((s[i][n] - base) * kLog2e);
+          sm.p[ty + 16 * i][tx + 16 * n] = p;
+          sum += p;
+        }
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        l[i] = l[i] * alpha + sum;
+        m[i] = m_new;
+#pragma unroll
+        for (int x = 0; x < NC * 4; ++x) o[i][x] *= alpha;
+      }
+      __syncwarp();  // a half-warp reads back only the rows it wrote
 #pragma unroll 2
-    for (int t = 0; t < kSimtTok; t += 4) {
-      float4 p[RPT];
+      for (int t = 0; t < kSimtTok; t += 4) {
+        float4 p[kRpt];
 #pragma unroll
-      for (int i = 0; i < RPT; ++i) p[i] = *reinterpret_cast<const float4*>(&sm.p[ty + 16 * i][t]);
+        for (int i = 0; i < kRpt; ++i) p[i] = *reinterpret_cast<const float4*>(&sm.p[ty + 16 * i][t]);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < 4; ++u) {
 #pragma unroll
-        for (int cc = 0; cc < NC; ++cc) {
-          const float4 vv = *reinterpret_cast<const float4*>(&sm.v[at][t + u][4 * tx + 64 * cc]);
+          for (int cc = 0; cc < NC; ++cc) {
+            const float4 vv = *reinterpret_cast<const float4*>(&sm.v[at][t + u][4 * tx + 64 * cc]);
 #pragma unroll
-          for (int i = 0; i < RPT; ++i) {
-            const float pp = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
-            o[i][4 * cc + 0] = fmaf(pp, vv.x, o[i][4 * cc + 0]);
-            o[i][4 * cc + 1] = fmaf(pp, vv.y, o[i][4 * cc + 1]);
-            o[i][4 * cc + 2] = fmaf(pp, vv.z, o[i][4 * cc + 2]);
-            o[i][4 * cc + 3] = fmaf(pp, vv.w, o[i][4 * cc + 3]);
+            for (int i = 0; i < kRpt; ++i) {
+              const float pp = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
+              o[i][4 * cc + 0] = fmaf(pp, vv.x, o[i][4 * cc + 0]);
+              o[i][4 * cc + 1] = fmaf(pp, vv.y, o[i][4 * cc + 1]);
+              o[i][4 * cc + 2] = fmaf(pp, vv.z, o[i][4 * cc + 2]);
+              o[i][4 * cc + 3] = fmaf(pp, vv.w, o[i][4 * cc + 3]);
+            }
           }
         }
       }
     }
-  }
 
-  // results: the output itself when the keys are not split, else a partial
+    // results: the output itself when the keys are not split, else a partial
 #pragma unroll
-  for (int i = 0; i < RPT; ++i) {
-    const int rl = ty + 16 * i, r = rt * RT + rl;
-    if (r >= a.R) continue;
-    if (seg.part >= 0) {
-      const int64_t part = (int64_t)seg.part * RT + rl;
-      if (tx == 0) {
-        a.pm[part] = m[i];
-        a.pl[part] = l[i];
+    for (int i = 0; i < kRpt; ++i) {
+      const int rl = ty + 16 * i, r = rt * RT + rl;
+      if (r >= a.R) continue;
+      if (seg.part >= 0) {
+        const int64_t part = (int64_t)seg.part * RT + rl;
+        if (tx == 0) {
+          a.pm[part] = m[i];
+          a.pl[part] = l[i];
+        }
+        if (m[i] == -INFINITY) continue;
+#pragma unroll
+        for (int cc = 0; cc < NC; ++cc)
+          *reinterpret_cast<float4*>(&a.po[part * D + 4 * tx + 64 * cc]) =
+              make_float4(o[i][4 * cc], o[i][4 * cc + 1], o[i][4 * cc + 2], o[i][4 * cc + 3]);
+        continue;
       }
-      if (m[i] == -INFINITY) continue;
+      const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);  // NaN stays NaN
+      if (a.lse && tx == 0) a.lse[(int64_t)bh * a.R + r] = l[i] == 0.f ? INFINITY : m[i] + logf(l[i]);
+      const int64_t at = tok_q_offset(a, b, h, r, D);
 #pragma unroll
       for (int cc = 0; cc < NC; ++cc)
-        *reinterpret_cast<float4*>(&a.po[part * D + 4 * tx + 64 * cc]) =
-            make_float4(o[i][4 * cc], o[i][4 * cc + 1], o[i][4 * cc + 2], o[i][4 * cc + 3]);
-      continue;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float val = o[i][4 * cc + y] * inv;
+          if (a.out_dtype == OC_BF16)
+            static_cast<__nv_bfloat16*>(a.out)[at + 4 * tx + 64 * cc + y] = __float2bfloat16_rn(val);
+          else
+            static_cast<float*>(a.out)[at + 4 * tx + 64 * cc + y] = val;
+        }
     }
-    const float inv = l[i] > 0.f ? 1.f / l[i] : (l[i] == 0.f ? 0.f : l[i]);  // NaN stays NaN
-    if (a.lse && tx == 0) a.lse[(int64_t)bh * a.R + r] = l[i] == 0.f ? INFINITY : m[i] + logf(l[i]);
-    const int64_t at = tok_q_offset(a, b, h, r, D);
-#pragma unroll
-    for (int cc = 0; cc < NC; ++cc)
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const float val = o[i][4 * cc + y] * inv;
-        if (a.out_dtype == OC_BF16)
-          static_cast<__nv_bfloat16*>(a.out)[at + 4 * tx + 64 * cc + y] = __float2bfloat16_rn(val);
-        else
-          static_cast<float*>(a.out)[at + 4 * tx + 64 * cc + y] = val;
-      }
-  }
   }
 }
 
@@ -670,11 +670,13 @@ struct TokPlan {
 
 inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-// Kernel: float32 takes the float32-arithmetic kernel (row tiles of 16 or 64);
-// bfloat16 the m16n8k16 kernel (16, 32 or 64 rows, what the rows fill) or the
-// tcgen05 one, from the rows on where it is the faster (a tree over 64K tokens, 8
-// KV heads: at 128 channels 32 rows take 69 and 77 us, 64 rows 108 and 77; at 64
-// channels 48 rows 54 and 56, 96 rows 75 and 58; 32K tokens, 16 heads of 256
+// Kernel: float32 takes the one for few rows (units of 16) up to 32 rows, beyond the
+// one with row tiles of 64 (16K tokens, 4 KV heads: 32 rows take 44 and 52 us at 64
+// channels, 69 and 89 at 128, 116 and 144 at 256; 36 rows 58 and 52, 95 and 87, 163
+// and 146).  bfloat16 takes the m16n8k16 kernel (16, 32 or 64 rows, what the rows
+// fill) or the tcgen05 one, from the rows on where it is the faster (a tree over 64K
+// tokens, 8 KV heads: at 128 channels 32 rows take 69 and 77 us, 64 rows 108 and 77;
+// at 64 channels 48 rows 54 and 56, 96 rows 75 and 58; 32K tokens, 16 heads of 256
 // channels: 16 rows 114 and 134, 24 rows 187 and 134).
 //
 // Cut: with few units (row tile, batch row, KV head) for the GPU, all their key
