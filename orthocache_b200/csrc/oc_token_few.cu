@@ -14,6 +14,11 @@
 //     running maximum and sum of the row in registers and leaves the weights;
 //   * output: thread (4 channels, token group), RR x 4 sums in registers, joined
 //     over the token groups once, at the end.
+// Measured (D = 128): 1 token x 64K, 8 heads 111 us = 4.8 TB/s; 4 rows a head x 16K,
+// 8 heads 41 us; 16 rows x 32K, 4 heads 68 us = 2 TB/s.  A register tile of 1 row x 4
+// keys read keys and values from shared memory once per two rows: 315, 96 and 98 us.
+// Three stages instead of two (119, 46 us at four rows), and three CTAs per SM (120,
+// 44 us), are slower.
 #include "oc_mma.cuh"
 #include "oc_tma.cuh"
 #include "oc_token.cuh"

@@ -287,3 +287,45 @@ def test_memory_around_the_results_is_left_alone(N, dtype):
     want, sums = oc.accumulate_attention(q, k, v, None, lens, scale=0.1)
     assert torch.equal(out.view(dtype).view_as(q), want)
     assert torch.equal(w.view(F32).view(B, Hkv, S), sums)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("N,G", [(3, 1), (1, 8), (4, 3), (8, 3), (6, 5), (31, 1)])
+def test_few_rows_with_every_mask(N, G, D, dtype):
+    """3 to 31 rows per KV head: a ragged batch with padding, documents, a prefix,
+    a bias and a cap together, and the sums; keys enough for many runs."""
+    import orthocache_b200 as oc
+    g = _gen(N + G)
+    B, Hkv, S = 3, 2, 1301
+    Hq = Hkv * G
+    q, k, v = _qkv(g, B, N, Hq, Hkv, S, D, dtype)
+    lengths, prefix = [1301, 640, N], [900, 0, 2]
+    docs = (torch.arange(S) // 450).int().repeat(B, 1)
+    docs[0, 700:760] = -1
+    docs[1, 100:400] = -1
+    docs[1, :100] = 1
+    kd, vd = k.clone(), v.clone()
+    for b, n in enumerate(lengths):
+        hidden = (torch.arange(S) >= n) | (docs[b] < 0)
+        kd[b, hidden] = math.nan
+        vd[b, hidden] = math.inf
+    lens, slopes = torch.tensor(lengths), torch.linspace(0.001, 0.02, Hq)
+    for kw in (dict(), dict(documents=docs), dict(documents=docs, prefix=prefix, slopes=slopes, cap=8.0)):
+        if kw:
+            vis = R.chunk_visible(lengths, N, S, prefix=kw.get("prefix"), documents=docs).cuda()
+            ins = (q, kd, vd)
+        else:
+            vis = R.chunk_visible(lengths, N, S).cuda()
+            ins = (q, k, v)
+        bias = R.distance_bias(lengths, N, S, slopes).cuda() if "slopes" in kw else None
+        args = {**kw, **({"prefix": torch.tensor(prefix)} if "prefix" in kw else {})}
+        out = oc.chunk_attention(*ins, lens, **args)
+        kz, vz = (torch.where(torch.isfinite(x), x, torch.zeros_like(x)) for x in ins[1:])
+        want, p, tol, rel = R.attend(q, kz, vz, vis, cap=kw.get("cap", 0.0), bias=bias)
+        R.check(out, want, tol, str(list(kw)))
+        if not kw:
+            out, sums = oc.accumulate_attention(*ins, None, lens)
+            R.check(out, want, tol)
+            ws, wtol = R.column_sums(p, rel, Hkv)
+            R.check(sums, ws, wtol)
