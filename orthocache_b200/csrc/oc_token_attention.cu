@@ -21,21 +21,20 @@ namespace {
 
 constexpr int kSimtThreads = 256;
 constexpr int kSimtTok = 64;  // keys per tile
-constexpr int kRpt = 4;        // rows of a thread
 
 // Rows are padded, so that the 16 keys a half-warp reads at once, and the rows of
 // its two halves, fall into different banks.
-template <int D>
+template <int D, int kRpt>
 struct SimtSmem {
-  static constexpr int kStages = D <= 128 ? 2 : 1;  // what fits beside the queries
+  static constexpr int kStages = D == 64 ? 2 : 1;
   float q[16 * kRpt][D + 4];
   float k[kStages][kSimtTok][D + 4];
   float v[kStages][kSimtTok][D];
   float p[16 * kRpt][kSimtTok + 16];
   TokRow row[16 * kRpt];
-  int doc[kStages + 1][kSimtTok];
-  int64_t src[kStages + 1][kSimtTok];  // row of the key in its tensor, -1 for one that nobody sees
-  int unseen[kStages + 1];  // has the tile such keys?
+  int doc[3][kSimtTok];
+  int64_t src[3][kSimtTok];  // row of the key in its tensor, -1 for one that nobody sees
+  int unseen[3];  // has the tile such keys?
   int hi, min_hi;
   int span[4];  // least and largest document of the rows, first key and last + 1 of those between
   int pre[kMaxEvenBatch + 1];
@@ -57,21 +56,23 @@ __device__ __forceinline__ void simt_load_vec(const T* src, float* dst) {
   for (int c = 0; c < kVec; ++c) dst[c] = f[c];
 }
 
-// Row tiles of 64 query rows against tiles of 64 keys, one pass with
-// the running maximum and sum of the softmax; 256 threads as 16 x 16: thread
+// Row tiles of 16 kRpt (64 or 128) query rows against tiles of 64 keys, one pass
+// with the running maximum and sum of the softmax; 256 threads as 16 x 16: thread
 // (ty, tx) owns rows ty + 16 i, the scores of keys tx + 16 n, and the output
 // channels 4 tx + 64 c of its rows, so that the softmax statistics stay in
-// registers (reduced over the 16 lanes of a half-warp).  The next tile of keys and
-// values is on its way (cp.async) while one is multiplied; keys that no row may
-// see (behind the sequence, padding, pages outside the pool) are filled with
-// zeros, so that whatever the memory holds there cannot reach a result.  Bound by
-// the FMA pipe (42 % busy) and the latency of its shared-memory reads: 512 rows x 4K,
-// 16 heads, D 128 take 562 us = 29 TFLOP/s; loading each tile in turn, without the
-// padding and masking every tile, 784 us.
-template <int D>
-__global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a) {
+// registers (reduced over the 16 lanes of a half-warp).  Keys and values come by
+// cp.async: at 64 channels the next tile while one is multiplied, beyond, where
+// there is room for one, the next keys during the softmax and output of a tile and
+// the next values during the scores.  Keys that no row may see (behind the
+// sequence, padding, pages outside the pool) are filled with zeros, so that
+// whatever the memory holds there cannot reach a result.  Bound by the FMA pipe and
+// the latency of the shared-memory reads: 512 rows x 4K, 16 heads, D 128 take 435 us
+// = 37 TFLOP/s (row tiles of 64: 562; loading each tile in turn and masking all of
+// them: 784).
+template <int D, int kRpt>
+__global__ void __launch_bounds__(kSimtThreads, D == 64 ? 2 : 1) tok_simt_kernel(const TokArgs a) {
   extern __shared__ __align__(16) unsigned char raw[];
-  using Smem = SimtSmem<D>;
+  using Smem = SimtSmem<D, kRpt>;
   Smem& sm = *reinterpret_cast<Smem*>(raw);
   constexpr int RT = 16 * kRpt, NC = D / 64, ST = Smem::kStages, kRow = D / 4;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
     const int d0 = max(seg.t0 - nct, 0);
     const int ndraft = a.dk && seg.t1 > nct ? min(seg.t1 - nct, (a.Sq + kSimtTok - 1) / kSimtTok) - d0 : 0;
     const int ntile = ncache + ndraft, min_hi = sm.min_hi;
-    if (tid <= ST) sm.unseen[tid] = -1;
+    if (tid < 3) sm.unseen[tid] = -1;
 
     const auto first_key = [&](int tile) {
       return tile >= ncache ? (d0 + tile - ncache) * kSimtTok : t0 + tile * kSimtTok;
@@ -161,30 +162,30 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
         doc = a.docs ? a.docs[(size_t)b * a.S + j] : 0;
         if (doc >= 0) src = tok_kv_row(a, b, j);
       }
-      sm.doc[tile % (ST + 1)][tid] = doc;
-      sm.src[tile % (ST + 1)][tid] = src;
-      if (__any_sync(0xffffffffu, src < 0) && (tid & 31) == 0) sm.unseen[tile % (ST + 1)] = tile;
+      sm.doc[tile % 3][tid] = doc;
+      sm.src[tile % 3][tid] = src;
+      if (__any_sync(0xffffffffu, src < 0) && (tid & 31) == 0) sm.unseen[tile % 3] = tile;
     };
-    const auto issue = [&](int tile) {
-      if (tile < ntile) {
-        const float* kp = static_cast<const float*>(tile >= ncache ? a.dk : a.k);
-        const float* vp = static_cast<const float*>(tile >= ncache ? a.dv : a.v);
+    const auto issue = [&](int tile, bool keys, bool values) {
+      if (tile >= ntile) return;
+      const float* kp = static_cast<const float*>(tile >= ncache ? a.dk : a.k);
+      const float* vp = static_cast<const float*>(tile >= ncache ? a.dv : a.v);
 #pragma unroll 4
-        for (int e = tid; e < kSimtTok * kRow; e += kSimtThreads) {
-          const int t = e / kRow, x = e % kRow * 4;
-          const int64_t src = sm.src[tile % (ST + 1)][t], at = (src * a.Hkv + h) * D + x;
-          simt_cp16(&sm.k[tile % ST][t][x], src >= 0 ? kp + at : qbase, src >= 0);
-          simt_cp16(&sm.v[tile % ST][t][x], src >= 0 ? vp + at : qbase, src >= 0);
-        }
+      for (int e = tid; e < kSimtTok * kRow; e += kSimtThreads) {
+        const int t = e / kRow, x = e % kRow * 4;
+        const int64_t src = sm.src[tile % 3][t], at = (src * a.Hkv + h) * D + x;
+        if (keys) simt_cp16(&sm.k[tile % ST][t][x], src >= 0 ? kp + at : qbase, src >= 0);
+        if (values) simt_cp16(&sm.v[tile % ST][t][x], src >= 0 ? vp + at : qbase, src >= 0);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    const auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
 
-    TokRow row[kRpt];
+    TokRow rows[kRpt == 4 ? 4 : 1];  // in registers while there are enough
+    const auto row_of = [&](int i) { return kRpt == 4 ? rows[kRpt == 4 ? i : 0] : sm.row[ty + 16 * i]; };
     float m[kRpt], l[kRpt], o[kRpt][NC * 4];
 #pragma unroll
     for (int i = 0; i < kRpt; ++i) {
-      row[i] = sm.row[ty + 16 * i];
+      if (kRpt == 4) rows[kRpt == 4 ? i : 0] = sm.row[ty + 16 * i];
       m[i] = -INFINITY;
       l[i] = 0.f;
 #pragma unroll
@@ -192,20 +193,29 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
     }
 
     __syncthreads();
-    for (int t = 0; t < ST; ++t) mark(t);
+    for (int t = 0; t < 2; ++t) mark(t);
     __syncthreads();
-    if (ST == 2) issue(0);
+    issue(0, true, ST == 2);
+    commit();
+    if (ST == 1) {
+      issue(0, false, true);
+      commit();
+    }
     for (int tile = 0; tile < ntile; ++tile) {
       const bool draft = tile >= ncache;
-      const int j0 = first_key(tile), at = tile % ST;
-      const int *doc = sm.doc[tile % (ST + 1)];
-      const int64_t* src = sm.src[tile % (ST + 1)];
-      __syncthreads();  // the tile before is read, the next one marked
-      issue(tile + ST - 1);
-      mark(tile + ST);
-      asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
-      __syncthreads();
-      const bool unseen = sm.unseen[tile % (ST + 1)] == tile;
+      const int j0 = first_key(tile);
+      const int *doc = sm.doc[tile % 3];
+      const int64_t* src = sm.src[tile % 3];
+      const int at = tile % ST;
+      if (ST == 2) {
+        __syncthreads();  // the tile before is read
+        issue(tile + 1, true, true);
+        commit();
+        mark(tile + 2);
+      }
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncthreads();  // the keys are there
+      const bool unseen = sm.unseen[tile % 3] == tile;
 
       float s[kRpt][4];
 #pragma unroll
@@ -228,6 +238,11 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
             s[i][n] = fmaf(qq.w, kk[n].w, s[i][n]);
           }
         }
+      }
+      if (ST == 1) {
+        __syncthreads();  // the keys are read
+        issue(tile + 1, true, false);
+        commit();
       }
       // scale, cap, bias (natural units: log2(e) times a score would round once more,
       // and the exponential magnify that; here it multiplies the difference to the
@@ -256,14 +271,17 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
       }
       if (a.slopes) {
 #pragma unroll
-        for (int i = 0; i < kRpt; ++i)
+        for (int i = 0; i < kRpt; ++i) {
+          const TokRow row = row_of(i);
 #pragma unroll
           for (int n = 0; n < 4; ++n)
-            s[i][n] = fmaf(-row[i].slope2 * (1.f / kLog2e), fabsf((float)(row[i].pos - (j0 + tx + 16 * n))), s[i][n]);
+            s[i][n] = fmaf(-row.slope2 * (1.f / kLog2e), fabsf((float)(row.pos - (j0 + tx + 16 * n))), s[i][n]);
+        }
       }
       if (draft || a.docs || unseen || j0 + kSimtTok > min_hi) {  // else every row sees every key
 #pragma unroll
         for (int i = 0; i < kRpt; ++i) {
+          const TokRow row = row_of(i);
           const int r = rt * RT + ty + 16 * i;
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
@@ -272,7 +290,7 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
             if (draft)
               vis = vis && r < a.R && a.tree[b * a.tree_bstride + (int64_t)(r / a.G) * a.Sq + j] != 0;
             else
-              vis = vis && j < row[i].hi && (!a.docs || doc[t] == row[i].doc);
+              vis = vis && j < row.hi && (!a.docs || doc[t] == row.doc);
             if (!vis) s[i][n] = -INFINITY;
           }
         }
@@ -299,7 +317,12 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
 #pragma unroll
         for (int x = 0; x < NC * 4; ++x) o[i][x] *= alpha;
       }
-      __syncwarp();  // a half-warp reads back only the rows it wrote
+      if (ST == 1) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncthreads();  // the values are there
+      } else {
+        __syncwarp();  // a half-warp reads back only the weights it wrote
+      }
 #pragma unroll 2
       for (int t = 0; t < kSimtTok; t += 4) {
         float4 p[kRpt];
@@ -320,6 +343,12 @@ __global__ void __launch_bounds__(kSimtThreads) tok_simt_kernel(const TokArgs a)
             }
           }
         }
+      }
+      if (ST == 1) {
+        __syncthreads();  // the values are read
+        issue(tile + 1, false, true);
+        commit();
+        mark(tile + 2);
       }
     }
 
@@ -674,7 +703,7 @@ struct TokPlan {
 inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 // Kernel: float32 takes the one for few rows (units of 16) up to 32 rows, beyond the
-// one with row tiles of 64 (16K tokens, 4 KV heads: 32 rows take 44 and 52 us at 64
+// one with row tiles of 64 or 128 (16K tokens, 4 KV heads: 32 rows take 44 and 52 us at 64
 // channels, 69 and 89 at 128, 116 and 144 at 256; 36 rows 58 and 52, 95 and 87, 163
 // and 146).  bfloat16 takes the m16n8k16 kernel (16, 32 or 64 rows, what the rows
 // fill) or the tcgen05 one, from the rows on where it is the faster (a tree over 64K
@@ -699,7 +728,7 @@ constexpr int kMinTiles = 2;
 constexpr int kLogitRows = 16;
 
 TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int head_dim, int seq_len, int draft_len,
-                 float scale, bool uneven, bool lse) {
+                 float scale, bool uneven, bool docs, bool lse) {
   TokPlan p;
   const int G = q_heads / kv_heads;
   const int64_t R = (int64_t)q_len * G;
@@ -713,6 +742,11 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
     p.tile = 128;
   } else {
     p.row_tile = R <= 16 ? 16 : R <= 32 ? (dtype == OC_BF16 ? 32 : 16) : 64;
+    // float32 with 128 channels: a tile of 128 rows takes about 3/2 the time of one of
+    // 64 (72 rows x 16K, 2 heads: 83 and 95 us), but visits more keys of other documents
+    // (200-token documents: 111 and 71 us)
+    if (dtype == OC_F32 && head_dim == 128 && R > 64 && !docs && 3 * ((R + 127) / 128) < 2 * ((R + 63) / 64))
+      p.row_tile = 128;
     p.nrt = (int)((R + p.row_tile - 1) / p.row_tile);
     p.unit_rows = p.row_tile;
     p.tile = dtype == OC_BF16 ? tok_mma_tile(head_dim) : p.row_tile == 16 ? tok_few_tile(head_dim) : kSimtTok;
@@ -752,18 +786,20 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
   return p;
 }
 
-template <int D>
+template <int D, int kRpt>
 int launch_simt(const TokArgs& a, cudaStream_t st) {
-  const size_t smem = sizeof(SimtSmem<D>);
+  const size_t smem = sizeof(SimtSmem<D, kRpt>);
   static std::atomic<uint64_t> done{0};
-  const cudaError_t e = allow_smem(done, tok_simt_kernel<D>, smem);
+  const cudaError_t e = allow_smem(done, tok_simt_kernel<D, kRpt>, smem);
   if (e != cudaSuccess) return set_error(OC_ERR_CUDA, "tok_simt_kernel: %s", cudaGetErrorString(e));
-  tok_simt_kernel<D><<<a.even ? a.ncta : a.B * a.Hkv * a.nrt, kSimtThreads, smem, st>>>(a);
+  tok_simt_kernel<D, kRpt><<<a.even ? a.ncta : a.B * a.Hkv * a.nrt, kSimtThreads, smem, st>>>(a);
   return check_launch("tok_simt_kernel");
 }
 
-int dispatch_simt(const TokArgs& a, int D, cudaStream_t st) {
-  return D == 64 ? launch_simt<64>(a, st) : D == 128 ? launch_simt<128>(a, st) : launch_simt<256>(a, st);
+int dispatch_simt(const TokArgs& a, int D, int row_tile, cudaStream_t st) {
+  if (D == 64) return launch_simt<64, 4>(a, st);
+  if (D == 128) return row_tile == 64 ? launch_simt<128, 4>(a, st) : launch_simt<128, 8>(a, st);
+  return launch_simt<256, 4>(a, st);
 }
 
 template <typename T, int D, int RW>
@@ -835,7 +871,8 @@ int tok_common(const char* fn, TokArgs& a, const void* q, const void* k, const v
 int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void* workspace, size_t workspace_bytes,
             cudaStream_t st, const float* w_in = nullptr, float* w_out = nullptr) {
   const bool uneven = a.docs || (a.causal && a.Sq > a.S / 4);
-  const TokPlan p = tok_plan(dtype, a.B, a.Sq, a.Hq, a.Hkv, head_dim, a.S, a.dk ? a.Sq : 0, a.scale, uneven, lse);
+  const TokPlan p = tok_plan(dtype, a.B, a.Sq, a.Hq, a.Hkv, head_dim, a.S, a.dk ? a.Sq : 0, a.scale, uneven,
+                            a.docs != nullptr, lse);
   OC_REQUIRE(p.units < INT32_MAX, OC_ERR_SHAPE, "%s: too many work units", fn);
   OC_REQUIRE(workspace_bytes >= p.bytes, OC_ERR_CAPACITY, "%s: workspace %zu < %zu bytes", fn, workspace_bytes,
              p.bytes);
@@ -858,7 +895,7 @@ int tok_run(const char* fn, TokArgs& a, int dtype, int head_dim, bool lse, void*
   int rc = p.tc ? tok_tc(fn, a, head_dim, w + p.prep_off, st)
            : dtype == OC_BF16 ? tok_mma(a, head_dim, p.row_tile, st)
            : p.row_tile == 16 ? tok_few(a, head_dim, st)
-                              : dispatch_simt(a, head_dim, st);
+                              : dispatch_simt(a, head_dim, p.row_tile, st);
   if (rc) return rc;
   if (p.even) rc = tok_merge(a, head_dim, p.tc, st);
   if (rc || !w_out || a.S == 0) return rc;
@@ -887,9 +924,9 @@ extern "C" size_t oc_token_attention_workspace_bytes(int dtype, int batch, int q
     return 0;
   // the most that any call of these sizes needs
   size_t most = 0;
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 16; ++i) {
     const size_t n = tok_plan(dtype, batch, q_len, q_heads, kv_heads, head_dim, seq_len, i & 4 ? q_len : 0,
-                              i & 1 ? 1.f : 0.f, (i & 2) != 0, accumulate != 0).bytes;
+                              i & 1 ? 1.f : 0.f, (i & 2) != 0, (i & 8) != 0, accumulate != 0).bytes;
     if (n > most) most = n;
   }
   return most;
