@@ -722,10 +722,12 @@ inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 constexpr int kMinTiles = 2;
 
 // The accumulating form needs every score again once the denominators are
-// known.  Up to kLogitRows rows per KV head the kernels store them
-// (4 bytes a row and key, against 2 D or 4 D bytes of a key to multiply again: at
-// 16 rows and 128 channels 64 against 256 or 512); beyond, they are recomputed.
-constexpr int kLogitRows = 16;
+// known.  Up to kLogitRows rows per KV head the kernels for few rows store them (4
+// bytes a row and key, against 2 D or 4 D bytes of a key to multiply again);
+// beyond, they are recomputed.  Stored and recomputed, bfloat16: 32 rows x 32K, 8
+// heads, D 128 take 57 and 77 us, 24 rows x 16K, 2 x 4 heads, D 64 32 and 48;
+// float32: 239 and 337, 83 and 103.
+constexpr int kLogitRows = 32;
 
 TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int head_dim, int seq_len, int draft_len,
                  float scale, bool uneven, bool docs, bool lse) {

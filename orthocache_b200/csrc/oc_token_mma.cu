@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
           }
       }
 
-      if (WR == 1 && a.logits && wd == 0) {  // kept for the column sums (few rows only)
+      if (WR <= 2 && a.logits && wd == 0) {  // kept for the column sums (few rows only)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int r = rt * RT + wr * 16 + g + 8 * i;
