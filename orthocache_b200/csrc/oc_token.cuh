@@ -54,7 +54,9 @@ struct TokArgs {
   int hg;                     // heads that are cut alike; divides Hkv and ncta
   int unit_rows;              // rows of a unit's partial
   float *pm, *pl, *po;        // partials: [part][unit_rows][(D)], parts 2 * cta and 2 * cta + 1
-  float* logits;                 // (B * Hkv, R, logit_stride) scores in the units of pm, -inf where masked; nullable
+  // (B * Hkv, R, logit_stride) scores in the units of pm, -inf where masked, written for the
+  // key tiles that a row's unit visits (with a causal mask: all that the row sees); nullable
+  float* logits;
   int64_t logit_stride;
   float* lse;                    // (B * Hkv, R) log of the softmax denominator, +inf for empty rows; nullable
   float unit;                    // 2^(unit * x) = e^x in the units of pm and lse: log2(e) for natural ones, else 1

@@ -663,7 +663,9 @@ __global__ void __launch_bounds__(kSimtThreads) tok_weights_kernel(const TokArgs
   }
 }
 
-// Column sums from stored scores (few rows): a thread per key, rows in order.
+// Column sums from stored scores (few rows): a thread per key, rows in order, from the
+// first that sees the key on.  Rows before it may lie in a unit that ends before the
+// key, whose scores nobody has stored.
 __global__ void __launch_bounds__(256) tok_sum_kernel(const TokArgs a, int blocks, const float* w_in,
                                                       float* w_out) {
   const int bh = blockIdx.x / blocks, j = blockIdx.x % blocks * 256 + threadIdx.x;
@@ -676,7 +678,8 @@ __global__ void __launch_bounds__(256) tok_sum_kernel(const TokArgs a, int block
   if (j < len) {
     const float* s = a.logits + (int64_t)bh * a.R * a.logit_stride + j;
 #pragma unroll 8
-    for (int r = 0; r < a.R; ++r) sum += exp2f((s[r * a.logit_stride] - a.lse[(int64_t)bh * a.R + r]) * a.unit);
+    for (int r = max(0, j - (len - a.Sq)) * a.G; r < a.R; ++r)
+      sum += exp2f((s[r * a.logit_stride] - a.lse[(int64_t)bh * a.R + r]) * a.unit);
   }
   w_out[at] = before + sum;
 }
