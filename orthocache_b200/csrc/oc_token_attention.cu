@@ -665,10 +665,11 @@ __global__ void __launch_bounds__(kSimtThreads) tok_weights_kernel(const TokArgs
 
 // Column sums from stored scores (few rows): a thread per key, rows in order, from the
 // first that sees the key on.  Rows before it may lie in a unit that ends before the
-// key, whose scores nobody has stored.
+// key, whose scores nobody has stored.  (A start of its own for every key in all blocks:
+// 66 us for a bfloat16 call of 32 rows x 32K, 8 heads, D 128; this 61.)
 __global__ void __launch_bounds__(256) tok_sum_kernel(const TokArgs a, int blocks, const float* w_in,
                                                       float* w_out) {
-  const int bh = blockIdx.x / blocks, j = blockIdx.x % blocks * 256 + threadIdx.x;
+  const int bh = blockIdx.x / blocks, j0 = blockIdx.x % blocks * 256, j = j0 + threadIdx.x;
   if (j >= a.S) return;
   const int64_t at = (int64_t)bh * a.S + j;
   const int len = tok_len(a, bh / a.Hkv);
@@ -677,9 +678,15 @@ __global__ void __launch_bounds__(256) tok_sum_kernel(const TokArgs a, int block
   float sum = 0.f;
   if (j < len) {
     const float* s = a.logits + (int64_t)bh * a.R * a.logit_stride + j;
+    const auto weight = [&](int r) { return exp2f((s[r * a.logit_stride] - a.lse[(int64_t)bh * a.R + r]) * a.unit); };
+    const int all = len - a.Sq;  // keys up to this one are seen by every row
+    if (j0 + 255 <= all) {  // a loop that is the same for the block
 #pragma unroll 8
-    for (int r = max(0, j - (len - a.Sq)) * a.G; r < a.R; ++r)
-      sum += exp2f((s[r * a.logit_stride] - a.lse[(int64_t)bh * a.R + r]) * a.unit);
+      for (int r = 0; r < a.R; ++r) sum += weight(r);
+    } else {
+#pragma unroll 8
+      for (int r = max(0, j - all) * a.G; r < a.R; ++r) sum += weight(r);
+    }
   }
   w_out[at] = before + sum;
 }
