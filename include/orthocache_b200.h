@@ -460,7 +460,9 @@ int oc_score_from_metadata_paged(const float* dc_pool, const float* e_ac_pool, c
  * are scale * q.k in float32; cap > 0 turns them into cap * tanh(s / cap)
  * (then |scale| <= 4096 * cap and |scale| <= 2^24).  A query row that sees no
  * key gives zeros.  Values inside a sequence must be finite, whether a row sees
- * them or not (a hidden one has weight zero, and zero times infinity is NaN).  out
+ * them or not (a hidden one has weight zero, and zero times infinity is NaN), and at
+ * most 2^50 in magnitude (the weights are divided by the softmax denominator at the
+ * end, and may be up to 2^48 before).  out
  * (B, Sq, Hq, D) in out_dtype.  k and v may be NULL when seq_len is 0.
  * Workspace: oc_token_attention_workspace_bytes (q_len: Sq or the drafted
  * tokens; accumulate: nonzero for oc_accumulate_attention), 16-byte aligned;

@@ -401,19 +401,25 @@ __device__ __forceinline__ bool tc_dirty(const TcArgs& x, const TcUnit& w, int j
          (a.docs && x.key_docs[(size_t)w.b * x.nkt + jt].x < 0);
 }
 
-// CAP 0: no cap.  CAP 1 (cap <= kCapFixed, no bias): a capped score lies within
-// cap log2(e) <= 90 of zero in log2 units, so neither 2^score nor its sums leave
-// float32: the reference point of the softmax is 0 for every row, with no
-// maximum to find and nothing to rescale.  CAP 2: larger caps, or with a bias; a
-// running maximum.
-constexpr float kCapFixed = 62.f;
-
 // The reference point m of a row's softmax is exact whatever it is, as long as
-// 2^(score - m) and its sums stay in range, and bfloat16 has the range of
-// float32.  So a row takes the maximum of its first visible tile, and the tiles
-// after it are exponentiated without looking for one; a tile whose sum comes to
-// kRefMax or more is done over, with the rescaling.
-constexpr float kRefMax = 1.152921504606846976e18f;  // 2^60
+// 2^(score - m), its sums and its products with the values stay in range, and
+// bfloat16 has the range of float32.  So a row takes the maximum of its first
+// visible tile, and the tiles after it are exponentiated without looking for one; a
+// tile whose sum comes to kRefMax or more is done over, with the rescaling.
+//
+// CAP 0: no cap.  CAP 1 (cap <= kCapFixed, no bias): m is 0, with no maximum to
+// find, while |score| <= tanh(kTanhMax) cap, at most 41.4 in log2 units: 2^score is
+// bounded by the polynomials' range, which is looked at anyway.  A tile beyond it, or
+// masked, finds its rows' maxima, unless the cap is that small itself, and moves m
+// where that is more than kCapSlack away (down as long as the row has summed nothing).
+// (Looking at the sums of the fast tiles instead: a capped 2048-token chunk on 32K 1,104
+// -> 1,174 us.)  CAP 2: larger caps, or with a bias.
+//
+// In all of them the weights of 128 keys sum to less than 2^49, those of 2^31 to
+// less than 2^73: values up to 2^50, and their sums, stay far inside float32.
+constexpr float kCapFixed = 62.f;
+constexpr float kCapSlack = 42.f;
+constexpr float kRefMax = 281474976710656.f;  // 2^48
 
 template <int D, int CAP, bool BIAS>
 __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem) {
@@ -460,16 +466,17 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
       if (!bar_wait_warp(&sm.abort, &sm.s_full[t], s_ph)) return;
       s_ph ^= 1;
       tc_fence_after();
-      // Fast: every key visible, every row with a reference point.
+      // Fast: every key visible, every row with a reference point (with CAP 1, the first).
       bool done = false;
       const float d0 = (float)(row.pos - j0);
       const bool behind = !BIAS || (a.causal && !a.prefix);
-      if (!part && behind && level < 2 && !__any_sync(0xffffffffu, m_used == -INFINITY)) {
+      if (!part && behind && level < 2 && (CAP == 1 || !__any_sync(0xffffffffu, m_used == -INFINITY))) {
         uint32_t pk[64];
-        const uint64_t nm2 = pk2(-m_used, -m_used);
+        const float ref = CAP == 1 ? 0.f : m_used;
+        const uint64_t nm2 = pk2(-ref, -ref);
         const uint64_t sl2 = pk2(row.slope2, row.slope2);
         // |d| = d behind the query: bias and reference point are linear along the tile
-        const float b0 = fmaf(-row.slope2, d0, -m_used);
+        const float b0 = fmaf(-row.slope2, d0, -ref);
         uint64_t r2[4] = {0, 0, 0, 0};
         float s[128], top = 0.f;
         tmem_ld128_wait(t_s, s);
@@ -533,6 +540,12 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
         // memory once for the maximum and once for the exponentials: the code stays
         // a quarter as long (a CTA's first tile comes this way, with cold
         // instruction caches)
+        const auto mask = [&](int c, float (&s)[32]) {
+          const uint32_t word = c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(word >> i & 1)) s[i] = -INFINITY;
+        };
         const auto scores = [&](int c, float (&s)[32]) {
           tmem_ld32_wait(t_s + 32 * c, s);
           if (CAP) {
@@ -552,17 +565,19 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
 #pragma unroll
             for (int i = 0; i < 32; ++i) s[i] = fmaf(-row.slope2, fabsf(dc - (float)i), s[i]);
           }
-          const uint32_t word = c == 0 ? vis[0] : c == 1 ? vis[1] : c == 2 ? vis[2] : vis[3];
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!(word >> i & 1)) s[i] = -INFINITY;
+          mask(c, s);
         };
-        if (CAP != 1) {
+        if (CAP != 1 || cap.cap2 > kCapSlack) {
           float mx = -INFINITY;
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             float s[32];
-            scores(c, s);
+            if (CAP == 1) {  // the cap keeps the order: the largest product has the largest score
+              tmem_ld32_wait(t_s + 32 * c, s);
+              mask(c, s);
+            } else {
+              scores(c, s);
+            }
             float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
@@ -570,9 +585,16 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
               for (int y = 0; y < 4; ++y) m4[y] = max3(m4[y], s[i + y], s[i + 4 + y]);
             mx = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
           }
-          const bool need = mx > m_used + 8.f;
+          bool need;
+          if (CAP == 1) {
+            const bool sees = mx > -INFINITY;
+            mx = cap.exact(mx);
+            need = sees && (mx > m_used + kCapSlack || (l == 0.f && mx < m_used - kCapSlack));
+          } else {
+            need = mx > m_used + 8.f;
+          }
           if (__any_sync(0xffffffffu, need)) {
-            const float alpha = need ? ex2(m_used - mx) : 1.f;  // 0 on a row's first visible tile
+            const float alpha = need ? ex2(m_used - mx) : 1.f;  // 0 on a row's first visible tile without a cap
             if (j > j_first) {
 #pragma unroll 1
               for (int c = 0; c < D / 32; ++c) {
@@ -585,6 +607,7 @@ __device__ void tc_softmax(TcSmem<D>& sm, const TcArgs& x, int t, uint32_t tmem)
             }
             l *= alpha;
             if (need) m_used = mx;
+            if (CAP == 1) level = 2;  // the fast path takes 0
           }
         }
         const float base = m_used == -INFINITY ? 0.f : m_used;

@@ -18,10 +18,10 @@ Shapes: q (B, Sq, Hq, D), keys and values (B, S, Hkv, D), float32 or bfloat16,
 D in {64, 128, 256}, Hq a multiple of Hkv; without the batch dimension all
 per-row arguments lose theirs too.  q is brought to the keys' type and the output
 has it.  Inputs on the CPU are copied to the GPU.  Nothing waits for the GPU.
-Values inside a sequence are finite, seen by a row or not (a hidden one has
-weight zero, and zero times infinity is NaN); what lies behind lengths[b], in
-padding or in drafted tokens that no node sees may be anything.  With a cap, it is
-at least scale / 4096.
+Values inside a sequence are finite and at most 2^50 in magnitude, seen by a row
+or not (a hidden one has weight zero, and zero times infinity is NaN); what lies
+behind lengths[b], in padding or in drafted tokens that no node sees may be
+anything.  With a cap, it is at least scale / 4096.
 """
 from __future__ import annotations
 
