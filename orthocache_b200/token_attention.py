@@ -16,8 +16,10 @@ The three operators here attend to single tokens of a cache that holds
 
 Shapes: q (B, Sq, Hq, D), keys and values (B, S, Hkv, D), float32 or bfloat16,
 D in {64, 128, 256}, Hq a multiple of Hkv; without the batch dimension all
-per-row arguments lose theirs too.  q is brought to the keys' type and the output
-has it.  Inputs on the CPU are copied to the GPU.  Nothing waits for the GPU.
+per-row arguments lose theirs too (a length is then a number or a tensor without
+a dimension; either also stands for a whole batch).  q is brought to the keys'
+type and the output has it.  Inputs on the CPU are copied to the GPU.  Nothing
+waits for the GPU.
 Values inside a sequence are finite and at most 2^50 in magnitude, seen by a row
 or not (a hidden one has weight zero, and zero times infinity is NaN); what lies
 behind lengths[b], in padding or in drafted tokens that no node sees may be
@@ -27,6 +29,7 @@ from __future__ import annotations
 
 import functools
 import math
+import numbers
 
 import torch
 
@@ -53,17 +56,19 @@ def _call(name, device, *args):
 
 
 def _int_rows(x, shape, device, what):
-    """An int32 device tensor of ``shape`` (None stays None; a number fills it)."""
+    """An int32 device tensor of ``shape`` (None stays None; a number fills it, a tensor without a dimension a row)."""
     if x is None:
         return None
     if isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.shape == shape and x.device == device and \
             x.is_contiguous():
         return x
-    if isinstance(x, int):
-        return torch.full(shape, x, dtype=torch.int32, device=device)
+    if isinstance(x, numbers.Integral):
+        return torch.full(shape, min(max(int(x), -2 ** 31), 2 ** 31 - 1), dtype=torch.int32, device=device)
     t = _on(x, device)
     if t.dtype.is_floating_point or t.dtype == torch.bool:
         raise TypeError(f"{what} must be integers, got {t.dtype}")
+    if t.dim() == 0 and len(shape) == 1:
+        t = t.expand(shape)
     if t.shape != shape:
         raise ValueError(f"{what} {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype in (torch.int64, torch.uint32, torch.uint64):  # beyond the range: its nearest end, not another number
@@ -150,6 +155,8 @@ def tree_attention(q, keys, values, draft_keys, draft_values, tree_mask, lengths
         table = _on(block_table, device=dev)
         if table.dim() == 1:
             table = table.unsqueeze(0)
+        if table.dim() != 2:
+            raise ValueError(f"block_table {tuple(table.shape)}, expected ({B}, blocks)")
         table = _int_rows(table, (B, table.shape[-1]), dev, "block_table")
         pages, stride = k.shape[0] // PAGE, table.shape[1]
         S = stride * PAGE
