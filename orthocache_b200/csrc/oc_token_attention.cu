@@ -736,15 +736,39 @@ constexpr int kMinTiles = 2;
 // bytes a row and key, against 2 D or 4 D bytes of a key to multiply again);
 // beyond, they are recomputed.  Stored and recomputed, bfloat16: 32 rows x 32K, 8
 // heads, D 128 take 57 and 77 us, 24 rows x 16K, 2 x 4 heads, D 64 32 and 48;
-// float32: 239 and 337, 83 and 103.
+// float32: 239 and 337, 83 and 103.  Not where a positive scale takes the tcgen05
+// kernel anyway, and in 512 MiB at most, so that no call needs the memory of its keys
+// once more: a batch with more of them goes by groups of its rows (16 x 32 rows x 32K,
+// 16 heads, D 128, bfloat16: three groups 1,111 us, at once with 1 GiB 1,102; half as many
+// recomputed 776, stored 541).
 constexpr int kLogitRows = 32;
+constexpr size_t kLogitBytes = (size_t)512 << 20;
+
+// Rows that the kernels for few rows take.
+inline bool tok_few_rows(int dtype, int64_t R, int head_dim) {
+  return dtype == OC_F32 || R <= (head_dim == 64 ? 64 : head_dim == 128 ? 32 : 16);
+}
+
+inline size_t tok_logit_stride(int seq_len) { return ((size_t)seq_len + 63) / 64 * 64; }  // whole tiles
+
+// Batch rows of one pass of the accumulating form: all of them, or as many as have
+// their scores stored within kLogitBytes.
+int tok_batch_group(int dtype, int batch, int q_len, int q_heads, int kv_heads, int head_dim, int seq_len) {
+  const int64_t R = (int64_t)q_len * (q_heads / kv_heads);
+  if (R > kLogitRows || !tok_few_rows(dtype, R, head_dim) || seq_len == 0) return batch;
+  const size_t n = kLogitBytes / ((size_t)kv_heads * R * tok_logit_stride(seq_len) * sizeof(float));
+  if (n < 1 || n >= (size_t)batch) return batch;
+  const int groups = (batch + (int)n - 1) / (int)n;
+  return (batch + groups - 1) / groups;
+}
 
 TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int head_dim, int seq_len, int draft_len,
                  float scale, bool uneven, bool docs, bool lse) {
   TokPlan p;
   const int G = q_heads / kv_heads;
   const int64_t R = (int64_t)q_len * G;
-  p.tc = dtype == OC_BF16 && R > (head_dim == 64 ? 64 : head_dim == 128 ? 32 : 16) && scale > 0.f;
+  const bool few = tok_few_rows(dtype, R, head_dim);
+  p.tc = !few && scale > 0.f;
   int64_t slots = device_sm_count();
   if (p.tc) {
     p.row_tile = 128;
@@ -790,9 +814,13 @@ TokPlan tok_plan(int dtype, int batch, int q_len, int q_heads, int kv_heads, int
   if (p.tc) off += up256(tok_tc_prep_bytes(batch, q_len, G, head_dim, seq_len));
   p.logit_off = off;
   p.logit_stride = 0;
-  if (lse && !p.tc && R <= kLogitRows) {
-    p.logit_stride = (seq_len + 63) / 64 * 64;  // whole tiles
-    off += up256((size_t)batch * kv_heads * R * p.logit_stride * sizeof(float));
+  if (lse && few && R <= kLogitRows) {
+    const size_t stride = tok_logit_stride(seq_len);
+    const size_t logit_bytes = (size_t)batch * kv_heads * R * stride * sizeof(float);
+    if (logit_bytes <= kLogitBytes) {
+      p.logit_stride = stride;
+      off += up256(logit_bytes);
+    }
   }
   p.bytes = off;
   return p;
@@ -935,9 +963,12 @@ extern "C" size_t oc_token_attention_workspace_bytes(int dtype, int batch, int q
       (head_dim != 64 && head_dim != 128 && head_dim != 256))
     return 0;
   // the most that any call of these sizes needs
+  const int group = accumulate ? tok_batch_group(dtype, batch, q_len, q_heads, kv_heads, head_dim, seq_len) : batch;
   size_t most = 0;
-  for (int i = 0; i < 16; ++i) {
-    const size_t n = tok_plan(dtype, batch, q_len, q_heads, kv_heads, head_dim, seq_len, i & 4 ? q_len : 0,
+  for (int i = 0; i < 32; ++i) {
+    const int rows = i & 16 ? batch % group : group;  // the last group may be smaller
+    if (rows == 0) continue;
+    const size_t n = tok_plan(dtype, rows, q_len, q_heads, kv_heads, head_dim, seq_len, i & 4 ? q_len : 0,
                               i & 1 ? 1.f : 0.f, (i & 2) != 0, (i & 8) != 0, accumulate != 0).bytes;
     if (n > most) most = n;
   }
@@ -1010,8 +1041,22 @@ extern "C" int oc_accumulate_attention(const void* q, const void* k, const void*
   const uintptr_t wn = (uintptr_t)batch * kv_heads * seq_len * sizeof(float);
   OC_REQUIRE(!weights_in || wi == wo || wi + wn <= wo || wo + wn <= wi, OC_ERR_SHAPE,
              "oc_accumulate_attention: weights_in overlaps weights_out in part");
-  a.lengths = lengths;
   a.causal = 1;
-  return tok_run("oc_accumulate_attention", a, dtype, head_dim, true, workspace, workspace_bytes,
-                 reinterpret_cast<cudaStream_t>(stream), weights_in, weights_out);
+  const int group = tok_batch_group(dtype, batch, q_len, q_heads, kv_heads, head_dim, seq_len);
+  const size_t es = dtype == OC_BF16 ? 2 : 4, out_es = out_dtype == OC_BF16 ? 2 : 4;
+  const size_t q_row = (size_t)q_len * q_heads * head_dim, k_row = (size_t)seq_len * kv_heads * head_dim;
+  for (int b = 0; b < batch; b += group) {  // one after the other on the stream, in the same workspace
+    TokArgs g = a;
+    g.B = batch - b < group ? batch - b : group;
+    g.q = static_cast<const char*>(q) + b * q_row * es;
+    g.k = static_cast<const char*>(k) + b * k_row * es;
+    g.v = static_cast<const char*>(v) + b * k_row * es;
+    g.out = static_cast<char*>(out) + b * q_row * out_es;
+    g.lengths = lengths ? lengths + b : nullptr;
+    const size_t at = (size_t)b * kv_heads * seq_len;
+    rc = tok_run("oc_accumulate_attention", g, dtype, head_dim, true, workspace, workspace_bytes,
+                 reinterpret_cast<cudaStream_t>(stream), weights_in ? weights_in + at : nullptr, weights_out + at);
+    if (rc) return rc;
+  }
+  return OC_OK;
 }
