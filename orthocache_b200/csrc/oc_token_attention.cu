@@ -95,7 +95,6 @@ __global__ void __launch_bounds__(kSimtThreads, D == 64 ? 2 : 1) tok_simt_kernel
     }
     const int b = seg.b, h = seg.unit / a.nrt, rt = seg.unit % a.nrt, bh = b * a.Hkv + h;
     const int len = tok_len(a, b);
-    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();  // the previous piece is done with shared memory
     if (tid == 0) {
       sm.hi = 0;
@@ -351,6 +350,7 @@ __global__ void __launch_bounds__(kSimtThreads, D == 64 ? 2 : 1) tok_simt_kernel
         mark(tile + 2);
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");  // the queries of a piece without tiles
 
     // results: the output itself when the keys are not split, else a partial
 #pragma unroll

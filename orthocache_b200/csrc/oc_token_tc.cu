@@ -725,17 +725,12 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
   uint32_t q_ph = 0, L = 0;
   unsigned char* ring = tc_ring<D>(sm, x);
   const uint32_t slots = tc_slots<D>(x);
-  // after a wait that gave up: let the copies in flight land (bounded) before
-  // the CTA ends
-  auto drain = [&]() {
-    for (uint32_t s = 0; s < slots && s < L; ++s) mbar_wait(&sm.kv_full[s], ((L - s - 1) / slots) & 1);
-    mbar_wait(&sm.q_full, q_ph ^ 1);
-  };
+  bool go = true;
   TcWalk walk(x, sm.pre);
   TcUnit w;
-  while (walk.next(x, sm.pre, w)) {
+  while (go && walk.next(x, sm.pre, w)) {
     if (w.n == 0) continue;
-    if (!bar_wait(&sm.abort, &sm.q_empty, q_ph ^ 1)) return drain();
+    if (!bar_wait(&sm.abort, &sm.q_empty, q_ph ^ 1)) break;
     q_ph ^= 1;
     mbar_expect_tx(&sm.q_full, (uint32_t)(w.ntile * C::kTileBytes));
 #pragma unroll
@@ -744,14 +739,17 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
           tma_load_3d(sm.q[t] + c * C::kBox, mq, &sm.q_full, 64 * c, w.h * a.G + w.hs[t] * x.Gp, w.b * a.Sq + w.p0[t]);
-    for (int j = 0; j < w.n; ++j) {
+    for (int j = 0; go && j < w.n; ++j) {
       const bool draft = j >= w.ncache;
       int key = draft ? w.b * a.Sq + tc_tile(w, j) * kTok : tc_key_row(a, w.b, tc_tile(w, j));
       if (key < 0) key = 0;  // a page outside the pool: loaded from page 0, masked and zeroed
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv, ++L) {
         const uint32_t slot = L % slots;
-        if (!bar_wait(&sm.abort, &sm.kv_empty[slot], ((L / slots) & 1) ^ 1)) return drain();
+        if (!bar_wait(&sm.abort, &sm.kv_empty[slot], ((L / slots) & 1) ^ 1)) {
+          go = false;
+          break;
+        }
         mbar_expect_tx(&sm.kv_full[slot], C::kTileBytes);
         const CUtensorMap* m = kv ? (draft ? mdv : mv) : (draft ? mdk : mk);
 #pragma unroll
@@ -760,6 +758,11 @@ __device__ void tc_producer(TcSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
       }
     }
   }
+  // let the copies in flight land (bounded) before the CTA ends: this role, or another that
+  // has not read them, may have given up
+#pragma unroll 1
+  for (uint32_t s = 0; s < slots && s < L; ++s) mbar_wait(&sm.kv_full[s], ((L - s - 1) / slots) & 1);
+  mbar_wait(&sm.q_full, q_ph ^ 1);
 }
 
 // Where padding, pages or drafted tokens make it a matter of memory reads whether
@@ -1105,16 +1108,13 @@ __device__ void tw_producer(TwSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
   const TokArgs& a = x.t;
   const int lane = threadIdx.x & 31;
   uint32_t k_ph = 0, L = 0;
-  auto drain = [&]() {  // let the copies in flight land (bounded)
-    for (uint32_t s = 0; s < TcCfg<D>::kQuerySlots && s < L; ++s) mbar_wait(&sm.q_full[s], ((L - s - 1) / TcCfg<D>::kQuerySlots) & 1);
-    mbar_wait(&sm.k_full, k_ph ^ 1);
-  };
-  for (int k = 0; k * (int)gridDim.x < x.units; ++k) {
+  bool go = true;
+  for (int k = 0; go && k * (int)gridDim.x < x.units; ++k) {
     const int u = tc_deal(k);
     if (u >= x.units) continue;
     const TwUnit w = tw_unit<D>(x, u);
     if (w.n == 0) continue;
-    if (!bar_wait_warp(&sm.abort, &sm.k_empty, k_ph ^ 1)) return drain();
+    if (!bar_wait_warp(&sm.abort, &sm.k_empty, k_ph ^ 1)) break;
     k_ph ^= 1;
     if (lane == 0) {
       mbar_expect_tx(&sm.k_full, (uint32_t)(w.ntile * C::kTileBytes));
@@ -1132,7 +1132,10 @@ __device__ void tw_producer(TwSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
         lse[k] = pos < a.Sq ? a.lse[(int64_t)w.bh * a.R + (int64_t)pos * a.G + hs * x.Gp + col % x.Gp] : INFINITY;
       }
       const uint32_t slot = L % TcCfg<D>::kQuerySlots;
-      if (!bar_wait_warp(&sm.abort, &sm.q_empty[slot], ((L / TcCfg<D>::kQuerySlots) & 1) ^ 1)) return drain();
+      if (!bar_wait_warp(&sm.abort, &sm.q_empty[slot], ((L / TcCfg<D>::kQuerySlots) & 1) ^ 1)) {
+        go = false;
+        break;
+      }
 #pragma unroll
       for (int k = 0; k < 4; ++k) sm.lse[slot][32 * k + lane] = lse[k];
       if (lane == 0) {
@@ -1145,6 +1148,11 @@ __device__ void tw_producer(TwSmem<D>& sm, const TcArgs& x, const CUtensorMap* m
       }
     }
   }
+  // the copies in flight land (bounded) before the CTA ends, as above
+#pragma unroll 1
+  for (uint32_t s = 0; s < TcCfg<D>::kQuerySlots && s < L; ++s)
+    mbar_wait(&sm.q_full[s], ((L - s - 1) / TcCfg<D>::kQuerySlots) & 1);
+  mbar_wait(&sm.k_full, k_ph ^ 1);
 }
 
 template <int D>
