@@ -68,6 +68,11 @@ __device__ __forceinline__ int tok_len(const TokArgs& a, int b) {
   return n < 0 ? 0 : (n > a.S ? a.S : n);
 }
 
+// Does another kernel of the same call follow the attention kernel?  Only then may it
+// let the next one start early: a kernel of another call may read its queries before
+// it waits, and they may be this call's output.
+__device__ __forceinline__ bool tok_followed(const TokArgs& a) { return a.even || a.lse; }
+
 // What one query row may see and how its scores are biased.
 struct TokRow {
   int hi;       // keys [0, hi)

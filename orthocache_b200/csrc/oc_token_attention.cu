@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kSimtThreads, D == 64 ? 2 : 1) tok_simt_kernel
   constexpr int RT = 16 * kRpt, NC = D / 64, ST = Smem::kStages, kRow = D / 4;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const float* qbase = static_cast<const float*>(a.q);
-  pdl_trigger();  // the merge may find its parts meanwhile
+  if (tok_followed(a)) pdl_trigger();  // the merge may find its parts meanwhile
   if (a.even) {
     if (tid < 32) tok_prefix(a, sm.pre);
     __syncthreads();

@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kFewThreads, D == 256 ? 1 : 2) tok_few_kernel(
   const int tok = tid % TOK, cg = tid / TOK;        // scores
   const int xo = tid % kRow * 4, kg = tid / kRow;   // output
   const float* qbase = static_cast<const float*>(a.q);
-  pdl_trigger();  // the merge may find its parts meanwhile
+  if (tok_followed(a)) pdl_trigger();  // the merge may find its parts meanwhile
   if (a.even) {
     if (tid < 32) tok_prefix(a, sm.pre);
     __syncthreads();

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(MmaShape<D, WR>::THREADS) tok_mma_kernel(const
   const int wd = warp % C::WD, wt = warp / C::WD % WT, wr = warp / C::WD / WT;
   const int g = lane >> 2, c2 = (lane & 3) * 2;
   int* pre = s_int + 16;
-  pdl_trigger();  // the merge may find its parts meanwhile
+  if (tok_followed(a)) pdl_trigger();  // the merge may find its parts meanwhile
   if (a.even) {
     if (tid < 32) tok_prefix(a, pre);
     __syncthreads();

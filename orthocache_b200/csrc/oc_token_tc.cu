@@ -1019,7 +1019,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();     // everything below, the lengths too, may come from the kernel before this one
-  pdl_trigger();  // the merge may find its parts meanwhile
+  if (tok_followed(x.t)) pdl_trigger();  // the merge may find its parts meanwhile
   if (x.t.even && warp == 0) tok_prefix(x.t, sm.pre);
   tc_fence_before();
   __syncthreads();
