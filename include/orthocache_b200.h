@@ -520,7 +520,9 @@ int oc_accumulate_attention(const void* q, const void* k, const void* v, int dty
  * largest); all stay when n <= keep.  The kept tokens are written in order of
  * position: k_out / v_out (B, keep, Hkv, D), weights_out and index (their
  * source positions) (B, Hkv, keep), new_lengths (B) = min(n, keep); behind
- * them zeros, and index -1.  1 <= keep <= seq_len, 0 <= recent <= keep;
+ * them zeros, and index -1.  The new cache is full at `keep` tokens, and places in it
+ * (what oc_chunk_attention's slopes and documents go by) are not the old positions.
+ * 1 <= keep <= seq_len, 0 <= recent <= keep;
  * head_dim * sizeof(dtype) a multiple of 16.  The outputs must not overlap the
  * inputs. */
 int oc_evict_tokens(const void* k, const void* v, int dtype, const float* weights, const int32_t* lengths, int batch,

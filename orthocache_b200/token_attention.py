@@ -283,6 +283,11 @@ def evict_tokens(keys, values, weights, keep, recent=0, lengths=None):
     the new cache: (B, keep, Hkv, D) twice, (B, Hkv, keep), the tokens' old
     positions (B, Hkv, keep) int32 in ascending order, and min(n, keep) (B,)
     int32; behind the last kept token zeros and index -1.
+
+    The new cache holds ``keep`` tokens and has no room for another: to go on
+    decoding, copy it into one of a larger capacity.  Its tokens are numbered
+    anew, so a distance bias (``slopes``) or a document mask over it goes by places
+    in the new cache; the old positions are in ``index``, one row per KV head.
     """
     k, v = _cache(keys, values)
     w = _on(weights, device=k.device, dtype=torch.float32)
