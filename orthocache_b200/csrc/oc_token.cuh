@@ -71,7 +71,7 @@ __device__ __forceinline__ int tok_len(const TokArgs& a, int b) {
 // Does another kernel of the same call follow the attention kernel?  Only then may it
 // let the next one start early: a kernel of another call may read its queries before
 // it waits, and they may be this call's output.
-__device__ __forceinline__ bool tok_followed(const TokArgs& a) { return a.even || a.lse; }
+__device__ __forceinline__ bool tok_followed(const TokArgs& a) { return a.even || (a.lse && a.S > 0); }
 
 // What one query row may see and how its scores are biased.
 struct TokRow {

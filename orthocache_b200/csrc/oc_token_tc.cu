@@ -8,7 +8,7 @@
 // take 2,048 cycles and their exponentials as many on the MUFU unit; a pair takes
 // about 3,200.  Measured: 4 x 2048 rows x 32 heads on 8K keys without a mask 0.92
 // ms = 1,200 TFLOP/s (0.72 of the measured bf16 burst peak), causal on 32K 1,160,
-// capped 925-950; D = 64 690; D = 256 705; few rows on a long cache read it at 5
+// capped 925-1,000; D = 64 690; D = 256 705; few rows on a long cache read it at 5
 // to 5.4 TB/s.
 //
 // Layout (one persistent CTA of 384 threads per SM):
